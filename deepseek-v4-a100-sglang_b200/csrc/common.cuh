@@ -18,8 +18,8 @@ namespace dsv4 {
 // here (first writer wins) and runs to completion with garbage output instead
 // of hanging the GPU; the host reads it with dsv4_b200_get_device_status().
 // ---------------------------------------------------------------------------
-// Defined here: the library is a single translation unit (dsv4_b200.cu).
-__device__ int g_device_status = 0;
+// One word per translation unit; the host call reads both.
+static __device__ int g_device_status = 0;
 
 enum DeviceErr : int {
   kErrNone = 0,

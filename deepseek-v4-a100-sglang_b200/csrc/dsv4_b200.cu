@@ -1,24 +1,21 @@
 // C ABI of the B200 MXFP4/INT8 MoE path (declared in include/dsv4_b200.h).
-// Single translation unit: the device status word and every kernel live here.
-
-#include <cudaTypedefs.h>
+// The MXFP4/INT8 kernels and their device status word live in this translation
+// unit; the 16-bit feed-forward kernels in feed_forward.cu.
 
 #include <cstdarg>
-#include <cstdlib>
-#include <utility>
 #include <cstdio>
-#include <cstring>
 #include <mutex>
 
 #include "common.cuh"
 #include "gemm_tc.cuh"
+#include "host_common.h"
 #include "small_kernels.cuh"
 
 namespace dsv4 {
 
 namespace {
-
 thread_local char g_last_error[512] = "";
+}  // namespace
 
 int fail(int code, const char* fmt, ...) {
   va_list ap;
@@ -34,13 +31,6 @@ int check_launch(const char* what) {
   return DSV4_OK;
 }
 
-#define DSV4_REQUIRE(cond, ...) \
-  do {                          \
-    if (!(cond)) return fail(DSV4_ERR_INVALID_ARGUMENT, __VA_ARGS__); \
-  } while (0)
-
-inline cudaStream_t as_stream(void* s) { return reinterpret_cast<cudaStream_t>(s); }
-
 // Kernels of the hot path are launched with programmatic stream
 // serialisation (each calls pdl_entry() before touching global memory), so a
 // kernel's launch and scheduling overlap its predecessor's tail.
@@ -53,44 +43,7 @@ bool pdl_enabled() {
   return on;
 }
 
-template <typename... KArgs, typename... Args>
-void launch_pdl(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t st,
-                Args&&... args) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = grid;
-  cfg.blockDim = block;
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = pdl_enabled() ? 1 : 0;
-  // errors surface through cudaGetLastError in check_launch
-  (void)cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...);
-}
-
-// Cluster-of-2 launch (CTA pairs of the 2-SM MMA), with programmatic
-// dependent launch as launch_pdl.
-template <typename... KArgs, typename... Args>
-void launch_pair(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t st,
-                 Args&&... args) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = grid;
-  cfg.blockDim = block;
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = st;
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = 2;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[1].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = pdl_enabled() ? 2 : 1;
-  (void)cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...);
-}
+namespace {
 
 // 256-token tiles run on CTA pairs only with DSV4_B200_PAIR=1 (read at each
 // launch, so one process can compare both forms).  Off by default: measured
@@ -134,6 +87,8 @@ int align_smem_bytes(int experts) { return (32 * experts + experts + 1 + 32) * 4
 
 cudaError_t set_router_align_attrs();
 
+}  // namespace
+
 int ensure_init() {
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
@@ -168,6 +123,7 @@ int ensure_init() {
                              align_smem_bytes(kAlignMaxExperts));
   if (e != cudaSuccess)
     return fail(DSV4_ERR_CUDA, "cudaFuncSetAttribute: %s", cudaGetErrorString(e));
+  if (int r = feed_forward_init()) return r;
   cudaDeviceGetAttribute(&g_sm_count[dev], cudaDevAttrMultiProcessorCount, dev);
   g_inited[dev] = true;
   return DSV4_OK;
@@ -179,6 +135,8 @@ int sm_count() {
   return g_sm_count[dev] > 0 ? g_sm_count[dev] : 148;
 }
 
+namespace {
+
 // Persistent launch of CTA pairs: one pair per two SMs, never more pairs than
 // pair items (an item = one token tile x two neighbouring row tiles).
 template <int EPI>
@@ -188,8 +146,8 @@ int launch_gemm_pair(int64_t max_pair_items, const TcGemmParams& p, cudaStream_t
   if (pairs <= 0) return DSV4_OK;
   const dim3 grid(static_cast<unsigned>(2 * pairs));
   constexpr int kE = EPI | kEpiPair;
-  launch_pair(&mxfp4_int8_tc_gemm_kernel<256, kE>, grid, TcGemmCfg<256, true>::kThreads,
-              GemmKernel<256, kE>::kSmem, st, p);
+  launch_cluster(&mxfp4_int8_tc_gemm_kernel<256, kE>, grid, TcGemmCfg<256, true>::kThreads,
+                 GemmKernel<256, kE>::kSmem, st, 2, p);
   return check_launch("mxfp4_int8_tc_gemm_kernel (CTA pairs)");
 }
 
@@ -217,6 +175,8 @@ int launch_gemm(int tn, int64_t max_items, const TcGemmParams& p, cudaStream_t s
   return check_launch("mxfp4_int8_tc_gemm_kernel");
 }
 
+}  // namespace
+
 // ---- tensor maps for the weight stream (driver entry point, no -lcuda) ----
 PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder() {
   static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
@@ -230,6 +190,8 @@ PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder() {
   });
   return fn;
 }
+
+namespace {
 
 CUresult encode_u8(CUtensorMap* map, int rank, const void* base, const cuuint64_t* dims,
                    const cuuint64_t* strides, const cuuint32_t* box, CUtensorMapSwizzle swz,
@@ -616,6 +578,9 @@ int dsv4_b200_get_device_status(int* status, int reset) {
     e = cudaMemcpyToSymbol(g_device_status, &zero, sizeof(int));
     if (e != cudaSuccess) return fail(DSV4_ERR_CUDA, "reset status: %s", cudaGetErrorString(e));
   }
+  int other = 0;
+  if (int r = feed_forward_status(&other, reset)) return r;
+  if (*status == 0) *status = other;
   return DSV4_OK;
 }
 

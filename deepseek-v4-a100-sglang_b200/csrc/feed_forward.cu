@@ -1,0 +1,359 @@
+// C ABI of the 16-bit feed-forward operators (declared in include/dsv4_b200.h):
+// products with bias, activation and residual, the gated block with its
+// backward pass, and activation checkpoints in 8 bits.
+
+#include <limits>
+
+#include "host_common.h"
+
+#include "feed_forward_kernels.cuh"
+#include "gemm_f16.cuh"
+
+namespace dsv4 {
+
+namespace {
+
+template <int EPI>
+cudaError_t pair_attrs() {
+  cudaError_t e = cudaFuncSetAttribute(reinterpret_cast<void*>(&f16_pair_gemm_kernel<EPI, true>),
+                                       cudaFuncAttributeMaxDynamicSharedMemorySize, kF16SmemMax);
+  if (e != cudaSuccess) return e;
+  return cudaFuncSetAttribute(reinterpret_cast<void*>(&f16_pair_gemm_kernel<EPI, false>),
+                              cudaFuncAttributeMaxDynamicSharedMemorySize, kF16SmemMax);
+}
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+F16Mat mat16(const void* p, int64_t ld) {
+  return {const_cast<void*>(p), ld, aligned16(p) && ld % 8 == 0};
+}
+
+int64_t round_up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
+
+// 2-D operand of `rows` x `k` 16-bit elements, 128-byte swizzled boxes: K-major
+// {64 of k, box_rows}, MN-major {64 rows, 64 of k}.
+int encode_operand(CUtensorMap* map, const char* what, const void* p, int64_t rows, int64_t k,
+                   int64_t ld, int mn, int box_rows, bool bf16) {
+  if (tensor_map_encoder() == nullptr) return fail(DSV4_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
+  const int64_t inner = mn ? rows : k, outer = mn ? k : rows;
+  DSV4_REQUIRE(aligned16(p) && ld % 8 == 0 && ld >= inner,
+               "%s must be 16-byte aligned with a row stride of at least its row and a multiple of "
+               "8 elements (row stride %lld, row %lld)", what, (long long)ld, (long long)inner);
+  cuuint64_t dims[2] = {static_cast<cuuint64_t>(inner), static_cast<cuuint64_t>(outer)};
+  cuuint64_t strides[1] = {static_cast<cuuint64_t>(ld) * 2};
+  cuuint32_t box[2] = {64, static_cast<cuuint32_t>(mn ? 64 : box_rows)};
+  cuuint32_t estr[2] = {1, 1};
+  const CUresult r = tensor_map_encoder()(
+      map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2,
+      const_cast<void*>(p), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+      CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(DSV4_ERR_CUDA, "tensor map (%s) encode failed: %d", what, (int)r);
+  return DSV4_OK;
+}
+
+// Columns of a pair tile.  A wave of tiles costs its MMA cycles (2 per column
+// and 64 of k) or its operand bytes from L2, whichever is longer; the tile
+// that needs the fewest wave-cycles wins, the wider one on a tie.
+int pick_tn(int64_t m, int64_t n, bool gated) {
+  const int64_t pairs = sm_count() / 2, tiles_m = (m + 255) / 256;
+  const int step = gated ? 64 : 32;
+  int best = 256;
+  double best_cost = 0;
+  for (int tn = 256; tn >= step; tn -= step) {
+    const int64_t width = gated ? tn / 2 : tn;
+    const int64_t tiles = tiles_m * ((n + width - 1) / width);
+    const double mma = 2.0 * tn, load = (16384.0 + 64.0 * tn) / 64.0;
+    const double cost = static_cast<double>((tiles + pairs - 1) / pairs) * (mma > load ? mma : load);
+    if (tn == 256 || cost < 0.98 * best_cost) best = tn, best_cost = cost;
+  }
+  return best;
+}
+
+template <int EPI>
+int launch_pair_gemm(F16GemmParams& p, const void* a, int64_t lda, int a_mn, const void* b,
+                     int64_t b_rows, int64_t ldb, int b_mn, bool bf16, cudaStream_t st) {
+  p.a_mn = a_mn != 0;
+  p.b_mn = b_mn != 0;
+  p.tn = pick_tn(p.m, p.n, EPI == kEpiGated);
+  const int half = p.tn / 2, width = EPI == kEpiGated ? half : p.tn;
+  p.b_stage = p.b_mn ? (half + 63) / 64 * 8192 : half * 128;
+  const int stage = kF16ABytes + p.b_stage;
+  const int fixed = 1024 + kF16EpiBytes + kF16BarBytes;
+  p.stages = (kF16SmemMax - fixed) / stage;
+  if (p.stages > kF16MaxStages) p.stages = kF16MaxStages;
+  p.tiles_m = (p.m + 255) / 256;
+  p.tiles_n = (p.n + width - 1) / width;
+  p.group_m = 8;
+  DSV4_REQUIRE(static_cast<int64_t>(p.tiles_m) * p.tiles_n < (1ll << 30), "product too large");
+  if (int r = encode_operand(&p.map_a, "a", a, p.m, p.k, lda, p.a_mn, 128, bf16)) return r;
+  if (int r = encode_operand(&p.map_b, "b", b, b_rows, p.k, ldb, p.b_mn, half, bf16)) return r;
+  int64_t pairs = sm_count() / 2;
+  const int64_t tiles = static_cast<int64_t>(p.tiles_m) * p.tiles_n;
+  if (tiles < pairs) pairs = tiles;
+  const dim3 grid(static_cast<unsigned>(2 * pairs));
+  const size_t smem = fixed + static_cast<size_t>(p.stages) * stage;
+  if (bf16) {
+    launch_cluster(&f16_pair_gemm_kernel<EPI, true>, grid, dim3(kF16Threads), smem, st, 2, p);
+  } else {
+    launch_cluster(&f16_pair_gemm_kernel<EPI, false>, grid, dim3(kF16Threads), smem, st, 2, p);
+  }
+  return check_launch("f16_pair_gemm_kernel");
+}
+
+constexpr int64_t kMaxDim = 1ll << 30;
+constexpr float kNoLimit = std::numeric_limits<float>::infinity();
+
+int check_common(int64_t m, int64_t n, int64_t k, int dtype, int act) {
+  DSV4_REQUIRE(dtype == DSV4_BF16 || dtype == DSV4_F16, "dtype must be fp16 or bf16 (got %d)", dtype);
+  DSV4_REQUIRE(m >= 0 && n >= 1 && k >= 1 && m < kMaxDim && n < kMaxDim && k < kMaxDim,
+               "bad shape m=%lld n=%lld k=%lld", (long long)m, (long long)n, (long long)k);
+  DSV4_REQUIRE(act >= kActNone && act <= kActGeluTanh, "unknown activation %d", act);
+  return DSV4_OK;
+}
+
+int check_limit(int has_limit, float limit, float* out) {
+  *out = kNoLimit;
+  if (!has_limit) return DSV4_OK;
+  DSV4_REQUIRE(limit > 0.f && limit < kNoLimit, "the clamp limit must be positive and finite");
+  *out = limit;
+  return DSV4_OK;
+}
+
+// 8-bit kept values are moved by 16-byte pieces
+int check_codes(const int8_t* zq, const float* zs) {
+  DSV4_REQUIRE((zq == nullptr) == (zs == nullptr), "codes and scales go together");
+  DSV4_REQUIRE(aligned16(zq), "codes must be 16-byte aligned");
+  return DSV4_OK;
+}
+
+}  // namespace
+
+int feed_forward_init() {
+  cudaError_t e = pair_attrs<kEpiLinear>();
+  if (e == cudaSuccess) e = pair_attrs<kEpiGated>();
+  if (e == cudaSuccess) e = pair_attrs<kEpiGatedBwd>();
+  if (e != cudaSuccess)
+    return fail(DSV4_ERR_CUDA, "cudaFuncSetAttribute: %s", cudaGetErrorString(e));
+  return DSV4_OK;
+}
+
+int feed_forward_status(int* status, int reset) {
+  cudaError_t e = cudaMemcpyFromSymbol(status, g_device_status, sizeof(int));
+  if (e != cudaSuccess) return fail(DSV4_ERR_CUDA, "read status: %s", cudaGetErrorString(e));
+  if (reset && *status != 0) {
+    const int zero = 0;
+    e = cudaMemcpyToSymbol(g_device_status, &zero, sizeof(int));
+    if (e != cudaSuccess) return fail(DSV4_ERR_CUDA, "reset status: %s", cudaGetErrorString(e));
+  }
+  return DSV4_OK;
+}
+
+}  // namespace dsv4
+
+using namespace dsv4;
+
+extern "C" {
+
+int dsv4_b200_dense_gemm(const void* a, int64_t lda, int a_mn, const void* b, int64_t ldb, int b_mn,
+                         int64_t m, int64_t n, int64_t k, int dtype, const void* bias,
+                         int activation, const void* residual, int64_t ldr, void* out, int64_t ldo,
+                         void* z, int64_t ldz, int8_t* z_codes, float* z_scales, void* stream) {
+  if (int r = ensure_init()) return r;
+  if (int r = check_common(m, n, k, dtype, activation)) return r;
+  if (int r = check_codes(z_codes, z_scales)) return r;
+  DSV4_REQUIRE(z == nullptr || z_codes == nullptr, "z is kept in 16 or in 8 bits, not both");
+  if (m == 0) return DSV4_OK;
+  DSV4_REQUIRE(a && b && out, "null pointer argument");
+  DSV4_REQUIRE(ldo >= n && (!residual || ldr >= n || ldr == 0) && (!z || ldz >= n),
+               "row stride below n");
+  F16GemmParams p = {};
+  p.m = static_cast<int>(m), p.n = static_cast<int>(n), p.k = static_cast<int>(k);
+  p.act = activation;
+  p.limit = kNoLimit;
+  p.bias = bias;
+  p.residual = mat16(residual, ldr);
+  p.out = mat16(out, ldo);
+  p.z0 = mat16(z, ldz);
+  p.zq = z_codes, p.zs = z_scales, p.n32 = round_up(n, kGroup);
+  return launch_pair_gemm<kEpiLinear>(p, a, lda, a_mn, b, n, ldb, b_mn, dtype == DSV4_BF16,
+                                      as_stream(stream));
+}
+
+int dsv4_b200_gated_gemm(const void* x, int64_t ldx, int x_mn, const void* w13, int64_t ldw, int w_mn,
+                         int64_t m, int64_t intermediate, int64_t k, int dtype, int activation,
+                         int has_clamp, float clamp_limit, void* h, int64_t ldh, void* z, int64_t ldz,
+                         int8_t* z_codes, float* z_scales, void* stream) {
+  if (int r = ensure_init()) return r;
+  if (int r = check_common(m, 2 * intermediate, k, dtype, activation)) return r;
+  if (int r = check_codes(z_codes, z_scales)) return r;
+  F16GemmParams p = {};
+  if (int r = check_limit(has_clamp, clamp_limit, &p.limit)) return r;
+  DSV4_REQUIRE(z == nullptr || z_codes == nullptr, "z is kept in 16 or in 8 bits, not both");
+  if (m == 0) return DSV4_OK;
+  DSV4_REQUIRE(x && w13 && h, "null pointer argument");
+  DSV4_REQUIRE(ldh >= intermediate && (!z || ldz >= 2 * intermediate), "row stride below the row");
+  // a TMA box starts at a multiple of 16 bytes
+  DSV4_REQUIRE(!w_mn || intermediate % 8 == 0,
+               "w13 stored by columns needs intermediate to be a multiple of 8 (got %lld)",
+               (long long)intermediate);
+  p.m = static_cast<int>(m), p.n = static_cast<int>(intermediate), p.k = static_cast<int>(k);
+  p.act = activation;
+  p.up_row = p.n;
+  p.out = mat16(h, ldh);
+  p.z0 = mat16(z, ldz);
+  p.z1 = z ? mat16(static_cast<uint16_t*>(z) + intermediate, ldz) : mat16(nullptr, 0);
+  p.zq = z_codes, p.zs = z_scales, p.n32 = round_up(intermediate, kGroup);
+  return launch_pair_gemm<kEpiGated>(p, x, ldx, x_mn, w13, 2 * intermediate, ldw, w_mn,
+                                     dtype == DSV4_BF16, as_stream(stream));
+}
+
+int dsv4_b200_gated_backward_gemm(const void* dy, int64_t lddy, int dy_mn, const void* w2,
+                                  int64_t ldw, int w_mn, int64_t m, int64_t intermediate, int64_t k,
+                                  int dtype, int activation, int has_clamp, float clamp_limit,
+                                  const void* z, int64_t ldz, const int8_t* z_codes,
+                                  const float* z_scales, void* dz, int64_t lddz, void* h, int64_t ldh,
+                                  void* stream) {
+  if (int r = ensure_init()) return r;
+  if (int r = check_common(m, 2 * intermediate, k, dtype, activation)) return r;
+  if (int r = check_codes(z_codes, z_scales)) return r;
+  F16GemmParams p = {};
+  if (int r = check_limit(has_clamp, clamp_limit, &p.limit)) return r;
+  if (m == 0) return DSV4_OK;
+  DSV4_REQUIRE(dy && w2 && dz, "null pointer argument");
+  DSV4_REQUIRE((z == nullptr) != (z_codes == nullptr), "one of z and its codes is needed");
+  DSV4_REQUIRE(lddz >= 2 * intermediate && (!z || ldz >= 2 * intermediate) &&
+                   (!h || ldh >= intermediate), "row stride below the row");
+  p.m = static_cast<int>(m), p.n = static_cast<int>(intermediate), p.k = static_cast<int>(k);
+  p.act = activation;
+  const auto half = [&](const void* q, int64_t ld) {
+    return q ? mat16(static_cast<const uint16_t*>(q) + intermediate, ld) : mat16(nullptr, 0);
+  };
+  p.out = mat16(h, ldh);
+  p.z0 = mat16(z, ldz), p.z1 = half(z, ldz);
+  p.d0 = mat16(dz, lddz), p.d1 = half(dz, lddz);
+  p.zq = const_cast<int8_t*>(z_codes), p.zs = const_cast<float*>(z_scales);
+  p.n32 = round_up(intermediate, kGroup);
+  return launch_pair_gemm<kEpiGatedBwd>(p, dy, lddy, dy_mn, w2, intermediate, ldw, w_mn,
+                                        dtype == DSV4_BF16, as_stream(stream));
+}
+
+int dsv4_b200_checkpoint_int8(const void* x, int dtype, int64_t m, int64_t k, int64_t ldx,
+                              int8_t* codes, float* scales, void* stream) {
+  if (int r = ensure_init()) return r;
+  DSV4_REQUIRE(dtype == DSV4_F32 || dtype == DSV4_F16 || dtype == DSV4_BF16, "unknown dtype %d", dtype);
+  DSV4_REQUIRE(m >= 0 && k >= 1 && m < kMaxDim && k < kMaxDim && (ldx >= k || m <= 1),
+               "bad shape m=%lld k=%lld ldx=%lld", (long long)m, (long long)k, (long long)ldx);
+  if (m == 0) return DSV4_OK;
+  DSV4_REQUIRE(x && codes && scales, "null pointer argument");
+  if (int r = check_codes(codes, scales)) return r;
+  const int64_t k32 = round_up(k, kGroup), cb = (k32 + 255) / 256, blocks = (m + 31) / 32 * cb;
+  DSV4_REQUIRE(blocks < (1ll << 31), "checkpoint too large");
+  const int per = dtype == DSV4_F32 ? 4 : 8;
+  const int vec = aligned16(x) && ldx % per == 0;
+  const dim3 grid(static_cast<unsigned>(blocks));
+  cudaStream_t st = as_stream(stream);
+  const auto go = [&](auto kernel) {
+    launch_pdl(kernel, grid, dim3(256), 0, st, x, ldx, vec, m, k, k32, cb, codes, scales);
+  };
+  if (dtype == DSV4_F32) go(&checkpoint_kernel<DSV4_F32>);
+  else if (dtype == DSV4_F16) go(&checkpoint_kernel<DSV4_F16>);
+  else go(&checkpoint_kernel<DSV4_BF16>);
+  return check_launch("checkpoint_kernel");
+}
+
+int dsv4_b200_restore_int8(const int8_t* codes, const float* scales, int64_t m, int64_t k, void* out,
+                           int dtype, int64_t ldo, void* stream) {
+  if (int r = ensure_init()) return r;
+  DSV4_REQUIRE(dtype == DSV4_F32 || dtype == DSV4_F16 || dtype == DSV4_BF16, "unknown dtype %d", dtype);
+  DSV4_REQUIRE(m >= 0 && k >= 1 && m < kMaxDim && k < kMaxDim && ldo >= k,
+               "bad shape m=%lld k=%lld ldo=%lld", (long long)m, (long long)k, (long long)ldo);
+  if (m == 0) return DSV4_OK;
+  DSV4_REQUIRE(out && codes && scales, "null pointer argument");
+  if (int r = check_codes(codes, scales)) return r;
+  const int64_t k32 = round_up(k, kGroup), cb = (k32 + 255) / 256, blocks = (m + 31) / 32 * cb;
+  DSV4_REQUIRE(blocks < (1ll << 31), "checkpoint too large");
+  const int per = dtype == DSV4_F32 ? 4 : 8;
+  const int vec = aligned16(out) && ldo % per == 0;
+  const dim3 grid(static_cast<unsigned>(blocks));
+  cudaStream_t st = as_stream(stream);
+  const auto go = [&](auto kernel) {
+    launch_pdl(kernel, grid, dim3(256), 0, st, codes, scales, m, k, k32, cb, out, ldo, vec);
+  };
+  if (dtype == DSV4_F32) go(&restore_kernel<DSV4_F32>);
+  else if (dtype == DSV4_F16) go(&restore_kernel<DSV4_F16>);
+  else go(&restore_kernel<DSV4_BF16>);
+  return check_launch("restore_kernel");
+}
+
+int dsv4_b200_act_backward_slabs(int64_t m, int64_t n, int64_t* slabs) {
+  DSV4_REQUIRE(slabs != nullptr, "slabs is null");
+  DSV4_REQUIRE(m >= 0 && n >= 1 && m < kMaxDim && n < kMaxDim, "bad shape m=%lld n=%lld", (long long)m,
+               (long long)n);
+  // four blocks per SM, of at least 32 rows
+  const int64_t cols = (n + 255) / 256;
+  int64_t s = (4 * 148 + cols - 1) / cols;
+  if (s > (m + 31) / 32) s = (m + 31) / 32;
+  *slabs = s < 1 ? 1 : s;
+  return DSV4_OK;
+}
+
+int dsv4_b200_act_backward(const void* dy, int64_t lddy, const void* z, int64_t ldz,
+                           const int8_t* z_codes, const float* z_scales, int64_t m, int64_t n,
+                           int dtype, int activation, void* dz, int64_t lddz, float* partial,
+                           int64_t slabs, void* dbias, void* stream) {
+  if (int r = ensure_init()) return r;
+  if (int r = check_common(m, n, 1, dtype, activation)) return r;
+  if (int r = check_codes(z_codes, z_scales)) return r;
+  int64_t need = 0;
+  if (int r = dsv4_b200_act_backward_slabs(m, n, &need)) return r;
+  DSV4_REQUIRE((dbias == nullptr) == (partial == nullptr), "dbias and its workspace go together");
+  DSV4_REQUIRE(!dbias || slabs >= need, "workspace of %lld slabs, %lld needed", (long long)slabs,
+               (long long)need);
+  DSV4_REQUIRE(activation == kActNone || m == 0 ||
+                   (dz && lddz >= n && (z == nullptr) != (z_codes == nullptr) && (!z || ldz >= n)),
+               "an activation needs dz and one of z and its codes");
+  DSV4_REQUIRE(m == 0 || (dy && (lddy >= n || m == 1)), "bad dy");
+  DSV4_REQUIRE(need < 65536, "too many rows");
+  cudaStream_t st = as_stream(stream);
+  ActBackward p = {};
+  p.dy = dy, p.lddy = lddy, p.vec_dy = mat16(dy, lddy).vec;
+  p.z = z, p.ldz = ldz, p.vec_z = mat16(z, ldz).vec;
+  p.zq = z_codes, p.zs = z_scales, p.n32 = round_up(n, kGroup);
+  p.dz = dz, p.lddz = lddz, p.vec_dz = mat16(dz, lddz).vec;
+  p.partial = partial;
+  p.m = m, p.n = n, p.act = activation;
+  p.slab_rows = (m + need - 1) / need;
+  const dim3 grid(static_cast<unsigned>((n + 255) / 256), static_cast<unsigned>(need));
+  const dim3 sum_grid(static_cast<unsigned>((n + 127) / 128));
+  const bool bf16 = dtype == DSV4_BF16;
+  if (activation != kActNone || dbias) {
+    if (m == 0 && !dbias) return DSV4_OK;
+    if (bf16) launch_pdl(&act_backward_kernel<true>, grid, dim3(256), 0, st, p);
+    else launch_pdl(&act_backward_kernel<false>, grid, dim3(256), 0, st, p);
+    if (int r = check_launch("act_backward_kernel")) return r;
+  }
+  if (dbias) {
+    if (bf16) launch_pdl(&column_sum_kernel<true>, sum_grid, dim3(128), 0, st, partial, need, n, dbias);
+    else launch_pdl(&column_sum_kernel<false>, sum_grid, dim3(128), 0, st, partial, need, n, dbias);
+    return check_launch("column_sum_kernel");
+  }
+  return DSV4_OK;
+}
+
+int dsv4_b200_pack_rows(const void* in, int64_t row_stride, int64_t col_stride, int64_t rows,
+                        int64_t cols, void* out, int64_t ldo, void* stream) {
+  if (int r = ensure_init()) return r;
+  DSV4_REQUIRE(rows >= 0 && cols >= 0 && rows < kMaxDim && cols < kMaxDim && row_stride >= 0 &&
+                   col_stride >= 0 && ldo >= cols, "bad shape");
+  if (rows == 0 || cols == 0) return DSV4_OK;
+  DSV4_REQUIRE(in && out, "null pointer argument");
+  const int64_t cb = (cols + 31) / 32, blocks = (rows + 31) / 32 * cb;
+  DSV4_REQUIRE(blocks < (1ll << 31), "matrix too large");
+  launch_pdl(&pack_rows_kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, as_stream(stream),
+             static_cast<const uint16_t*>(in), row_stride, col_stride, rows, cols, cb,
+             static_cast<uint16_t*>(out), ldo);
+  return check_launch("pack_rows_kernel");
+}
+
+}  // extern "C"

@@ -1,0 +1,516 @@
+// Arithmetic of the 16-bit feed-forward operators (activations, their slopes,
+// the 8-bit groups of activation checkpoints) and their memory-bound kernels.
+#pragma once
+
+#include <math_constants.h>
+
+#include "common.cuh"
+
+namespace dsv4 {
+
+// ---- shared memory ----
+__device__ __forceinline__ void st_shared_v4(uint32_t a, uint4 v) {
+  asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(a), "r"(v.x), "r"(v.y), "r"(v.z),
+               "r"(v.w)
+               : "memory");
+}
+__device__ __forceinline__ uint4 ld_shared_v4(uint32_t a) {
+  uint4 v;
+  asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "r"(a)
+               : "memory");
+  return v;
+}
+__device__ __forceinline__ uint32_t ld_shared_u32(uint32_t a) {
+  uint32_t v;
+  asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
+  return v;
+}
+
+// 32 lanes x 32 consecutive fp32 columns of TMEM, waited on at once.
+__device__ __forceinline__ void tmem_ld_f32x32(uint32_t taddr, float (&f)[32]) {
+  int32_t v[32];
+  tmem_ld_x32_wait(taddr, v);
+#pragma unroll
+  for (int j = 0; j < 32; ++j) f[j] = __int_as_float(v[j]);
+}
+
+// ---- 16-bit values ----
+template <bool BF16>
+__device__ __forceinline__ uint32_t pack_16(float lo, float hi) {
+  uint32_t r;
+  if constexpr (BF16) {
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  } else {
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  }
+  return r;
+}
+
+template <bool BF16>
+__device__ __forceinline__ float unpack_16(uint32_t w, int hi) {
+  if constexpr (BF16) {
+    return __uint_as_float(hi ? (w & 0xffff0000u) : (w << 16));
+  } else {
+    return __half2float(__ushort_as_half(static_cast<unsigned short>(hi ? w >> 16 : w)));
+  }
+}
+
+template <bool BF16>
+__device__ __forceinline__ float ld_16(const void* p, int64_t i) {
+  return unpack_16<BF16>(static_cast<const uint16_t*>(p)[i], 0);
+}
+
+template <bool BF16>
+__device__ __forceinline__ void pack_row(const float (&v)[32], uint32_t (&w)[16]) {
+#pragma unroll
+  for (int j = 0; j < 16; ++j) w[j] = pack_16<BF16>(v[2 * j], v[2 * j + 1]);
+}
+
+// Rounded to 16 bits, but on the same side of the clamp limit as before: the
+// backward pass asks |z| <= limit of the kept value, and a value rounded over
+// the border would lose or gain its whole gradient.  At most one 16-bit step
+// (against half a step) for values next to the limit; limit > 0.
+template <bool BF16>
+__device__ __forceinline__ uint32_t round_sided(float z, float limit) {
+  uint32_t b = pack_16<BF16>(z, 0.f) & 0xffffu;
+  const bool over = fabsf(z) > limit, kept = fabsf(unpack_16<BF16>(b, 0)) > limit;
+  if (over && !kept) ++b;
+  if (!over && kept && z == z) --b;
+  return b;
+}
+
+template <bool BF16>
+__device__ __forceinline__ void pack_row_sided(const float (&v)[32], uint32_t (&w)[16],
+                                               float limit) {
+#pragma unroll
+  for (int j = 0; j < 16; ++j)
+    w[j] = round_sided<BF16>(v[2 * j], limit) | (round_sided<BF16>(v[2 * j + 1], limit) << 16);
+}
+
+// ---- activations: value and slope ----
+// sigmoid(z) = 1 / (1 + exp(-z)) in fast fp32 (a few units of 2^-23, against
+// the 2^-9 and more of the 16-bit results); gelu_tanh is z sigmoid(2a) with
+// a = sqrt(2/pi) (z + 0.044715 z^3), since (1 + tanh a) / 2 = sigmoid(2a).
+enum Act : int { kActNone = 0, kActRelu = 1, kActSilu = 2, kActGelu = 3, kActGeluTanh = 4 };
+
+__device__ __forceinline__ float sigmoid_fast(float z) {
+  return __fdividef(1.f, 1.f + __expf(-z));
+}
+
+constexpr float kGeluC = 1.5957691216057308f;  // 2 sqrt(2 / pi)
+constexpr float kGeluK = 0.044715f;
+
+template <int ACT>
+__device__ __forceinline__ float act_value(float z) {
+  if constexpr (ACT == kActRelu) return z <= 0.f ? 0.f : z;
+  if constexpr (ACT == kActSilu) return z * sigmoid_fast(z);
+  if constexpr (ACT == kActGelu) return 0.5f * z * (1.f + erff(z * 0.70710678118654752f));
+  if constexpr (ACT == kActGeluTanh)
+    return z * sigmoid_fast(kGeluC * (z + kGeluK * z * z * z));
+  return z;
+}
+
+template <int ACT>
+__device__ __forceinline__ void act_both(float z, float& a, float& slope) {
+  if constexpr (ACT == kActRelu) {
+    a = z <= 0.f ? 0.f : z;
+    slope = z <= 0.f ? 0.f : 1.f;
+  } else if constexpr (ACT == kActSilu) {
+    const float s = sigmoid_fast(z);
+    a = z * s;
+    slope = s * (1.f + z * (1.f - s));
+  } else if constexpr (ACT == kActGelu) {
+    const float phi = 0.5f * (1.f + erff(z * 0.70710678118654752f));
+    a = z * phi;
+    slope = phi + z * 0.39894228040143268f * __expf(-0.5f * z * z);
+  } else if constexpr (ACT == kActGeluTanh) {
+    // past |z| = 100 the sigmoid is 0 or 1 and its slope 0: z^2 is held there
+    // so that infinity * 0 does not arise
+    const float z2 = fminf(z * z, 1e4f);
+    const float s = sigmoid_fast(kGeluC * (z + kGeluK * z * z * z));
+    a = z * s;
+    slope = s + s * (1.f - s) * kGeluC * (z + 3.f * kGeluK * z * z2);
+  } else {
+    a = z;
+    slope = 1.f;
+  }
+}
+
+template <typename F>
+__device__ __forceinline__ void act_dispatch(int act, F&& f) {
+  switch (act) {
+    case kActRelu: f(std::integral_constant<int, kActRelu>{}); break;
+    case kActSilu: f(std::integral_constant<int, kActSilu>{}); break;
+    case kActGelu: f(std::integral_constant<int, kActGelu>{}); break;
+    case kActGeluTanh: f(std::integral_constant<int, kActGeluTanh>{}); break;
+    default: f(std::integral_constant<int, kActNone>{}); break;
+  }
+}
+
+__device__ __forceinline__ void act_row(int act, float (&v)[32]) {
+  act_dispatch(act, [&](auto kind) {
+    constexpr int K = decltype(kind)::value;
+    if constexpr (K != kActNone) {
+#pragma unroll
+      for (int j = 0; j < 32; ++j) v[j] = act_value<K>(v[j]);
+    }
+  });
+}
+
+// min(g, limit) and clamp(u, -limit, limit), NaN kept (torch.clamp)
+__device__ __forceinline__ float clamp_top(float g, float limit) { return g > limit ? limit : g; }
+__device__ __forceinline__ float clamp_both(float u, float limit) {
+  return u > limit ? limit : (u < -limit ? -limit : u);
+}
+
+template <int ACT>
+__device__ __forceinline__ void gated_backward(float limit, float dh, float g, float u, float& dg,
+                                               float& du, float& h) {
+  const float gc = clamp_top(g, limit), uc = clamp_both(u, limit);
+  float a, s;
+  act_both<ACT>(gc, a, s);
+  dg = g <= limit ? dh * uc * s : 0.f;
+  du = fabsf(u) <= limit ? dh * a : 0.f;
+  h = a * uc;
+}
+
+template <bool BF16>
+__device__ __forceinline__ void gated_backward_row(int act, float limit, const float (&dh)[32],
+                                                   const float (&g)[32], const float (&u)[32],
+                                                   uint32_t (&wg)[16], uint32_t (&wu)[16],
+                                                   uint32_t (&wh)[16]) {
+  act_dispatch(act, [&](auto kind) {
+    constexpr int K = decltype(kind)::value;
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      float dg[2], du[2], h[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        gated_backward<K>(limit, dh[2 * j + i], g[2 * j + i], u[2 * j + i], dg[i], du[i], h[i]);
+      wg[j] = pack_16<BF16>(dg[0], dg[1]);
+      wu[j] = pack_16<BF16>(du[0], du[1]);
+      wh[j] = pack_16<BF16>(h[0], h[1]);
+    }
+  });
+}
+
+// ---- 8-bit groups ----
+// 32 values of a row share a scale: code = 127 v / amax rounded to the nearest
+// whole number (ties to even) of the exact quotient, value = code * (amax / 127).
+// 32 keeps a channel's outliers from costing its neighbours more than half a
+// step of their own group, at 1.125 bytes per value.  A group that holds an
+// infinity or a NaN has scale NaN (all of it decodes to NaN); one whose
+// largest magnitude is below 2^-100 holds zeros.
+constexpr int kGroup = 32;
+constexpr float kTinyGroup = 7.8886090522101181e-31f;  // 2^-100
+
+struct GroupScale {
+  float inv;    // 127 / amax, 0 for an empty or non-finite group
+  float amax;
+  float scale;
+};
+
+__device__ __forceinline__ GroupScale group_scale(uint32_t amax_bits) {
+  const float amax = __uint_as_float(amax_bits);
+  if (amax_bits >= 0x7f800000u) return {0.f, amax, CUDART_NAN_F};
+  if (amax < kTinyGroup) return {0.f, amax, 0.f};
+  // toward zero: 127 steps never pass amax, so the largest finite value stays finite
+  return {127.f / amax, amax, __fdiv_rz(amax, 127.f)};
+}
+
+// The quotient in fp32 is off by less than 2e-5 at 127; only within 6e-5 of a
+// half can that change the code.  There the sign of 127 v - (f + 1/2) amax
+// decides, taken exactly: both products as rounded part + remainder.
+__device__ __forceinline__ int quantize_code(float v, const GroupScale& g) {
+  const float q = v * g.inv;
+  const float f = floorf(fabsf(q));
+  const float frac = fabsf(q) - f;
+  if (fabsf(frac - 0.5f) < 6e-5f) {
+    const float shrink = g.amax > 1.8446744e19f ? 5.4210109e-20f : 1.f;  // 2^64, 2^-64
+    const float a = g.amax * shrink, x = fabsf(v) * shrink, c = f + 0.5f;
+    const float p = 127.f * x, pl = __fmaf_rn(127.f, x, -p);
+    const float t = c * a, tl = __fmaf_rn(c, a, -t);
+    const float d = (p - t) + (pl - tl);
+    const int fi = static_cast<int>(f);
+    const int r = d > 0.f ? fi + 1 : d < 0.f ? fi : fi + (fi & 1);
+    return q < 0.f ? -r : r;
+  }
+  return __float2int_rn(q);
+}
+
+// A thread's own group: codes (4 per word) and the scale.
+__device__ __forceinline__ float quantize_group(const float (&v)[32], uint32_t (&codes)[8]) {
+  uint32_t top = 0;
+#pragma unroll
+  for (int j = 0; j < 32; ++j) top = max(top, __float_as_uint(v[j]) & 0x7fffffffu);
+  const GroupScale g = group_scale(top);
+  if (g.inv == 0.f) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) codes[j] = 0;
+    return g.scale;
+  }
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    uint32_t w = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      w |= (static_cast<uint32_t>(quantize_code(v[4 * j + i], g)) & 0xffu) << (8 * i);
+    codes[j] = w;
+  }
+  return g.scale;
+}
+
+// 8 consecutive values of a 16- or 32-bit row; pieces past `cols` read as 0.
+template <int DT>
+__device__ __forceinline__ void load_piece8(const void* base, int64_t at, int64_t col,
+                                            int64_t cols, bool vec, float (&v)[8]) {
+  if constexpr (DT == DSV4_F32) {
+    const float* p = static_cast<const float*>(base) + at;
+    if (vec && col + 8 <= cols) {
+      const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
+      v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = col + j < cols ? p[j] : 0.f;
+    }
+  } else {
+    constexpr bool BF16 = DT == DSV4_BF16;
+    const uint16_t* p = static_cast<const uint16_t*>(base) + at;
+    if (vec && col + 8 <= cols) {
+      const uint4 a = *reinterpret_cast<const uint4*>(p);
+      const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = unpack_16<BF16>(w[j >> 1], j & 1);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = col + j < cols ? unpack_16<BF16>(p[j], 0) : 0.f;
+    }
+  }
+}
+
+template <int DT>
+__device__ __forceinline__ void store_piece8(void* base, int64_t at, int64_t col, int64_t cols,
+                                             bool vec, const float (&v)[8]) {
+  if constexpr (DT == DSV4_F32) {
+    float* p = static_cast<float*>(base) + at;
+    if (vec && col + 8 <= cols) {
+      *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+      *reinterpret_cast<float4*>(p + 4) = make_float4(v[4], v[5], v[6], v[7]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (col + j < cols) p[j] = v[j];
+    }
+  } else {
+    constexpr bool BF16 = DT == DSV4_BF16;
+    uint16_t* p = static_cast<uint16_t*>(base) + at;
+    const uint32_t w[4] = {pack_16<BF16>(v[0], v[1]), pack_16<BF16>(v[2], v[3]),
+                           pack_16<BF16>(v[4], v[5]), pack_16<BF16>(v[6], v[7])};
+    if (vec && col + 8 <= cols) {
+      *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (col + j < cols) p[j] = static_cast<uint16_t>(w[j >> 1] >> (16 * (j & 1)));
+    }
+  }
+}
+
+// ---- activation checkpoint: rows -> 8-bit groups ----
+// A block takes 32 rows x 256 columns.  A lane owns 8 columns (a quarter of a
+// group, 16 bytes of a 16-bit row), so a warp reads 512 contiguous bytes of a
+// row and writes 256 of codes.  Scales lie [group][row]; they pass through
+// shared memory so that a warp writes one group's 32 rows together.
+// Codes rows are padded to the group with zeros.
+template <int DT>
+__global__ void __launch_bounds__(256)
+    checkpoint_kernel(const void* __restrict__ x, int64_t ld, int vec, int64_t m, int64_t k,
+                      int64_t k32, int64_t col_blocks, int8_t* __restrict__ codes,
+                      float* __restrict__ scales) {
+  pdl_entry();
+  __shared__ float s_scale[8][33];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t row0 = (blockIdx.x / col_blocks) * 32;
+  const int64_t col = (blockIdx.x % col_blocks) * 256 + lane * 8;
+  float v[4][8];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int64_t row = row0 + warp + 8 * i;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[i][j] = 0.f;
+    if (row < m && col < k) load_piece8<DT>(x, row * ld + col, col, k, vec, v[i]);
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int64_t row = row0 + warp + 8 * i;
+    uint32_t top = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(v[i][j]) & 0x7fffffffu);
+    top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    const GroupScale g = group_scale(top);
+    if ((lane & 3) == 0) s_scale[lane >> 2][warp + 8 * i] = g.scale;
+    if (row < m && col < k32) {
+      uint32_t w[2] = {0, 0};
+      if (g.inv != 0.f) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          w[j >> 2] |= (static_cast<uint32_t>(quantize_code(v[i][j], g)) & 0xffu) << (8 * (j & 3));
+      }
+      *reinterpret_cast<uint2*>(codes + row * k32 + col) = make_uint2(w[0], w[1]);
+    }
+  }
+  __syncthreads();
+  const int64_t group = (blockIdx.x % col_blocks) * 8 + warp, row = row0 + lane;
+  if (group * kGroup < k32 && row < m) scales[group * m + row] = s_scale[warp][lane];
+}
+
+template <int DT>
+__global__ void __launch_bounds__(256)
+    restore_kernel(const int8_t* __restrict__ codes, const float* __restrict__ scales, int64_t m,
+                   int64_t k, int64_t k32, int64_t col_blocks, void* __restrict__ out, int64_t ldo,
+                   int vec) {
+  pdl_entry();
+  __shared__ float s_scale[8][33];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t row0 = (blockIdx.x / col_blocks) * 32;
+  const int64_t col = (blockIdx.x % col_blocks) * 256 + lane * 8;
+  uint2 c[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int64_t row = row0 + warp + 8 * i;
+    c[i] = make_uint2(0, 0);
+    if (row < m && col < k32) c[i] = *reinterpret_cast<const uint2*>(codes + row * k32 + col);
+  }
+  const int64_t group = (blockIdx.x % col_blocks) * 8 + warp, srow = row0 + lane;
+  s_scale[warp][lane] = group * kGroup < k32 && srow < m ? scales[group * m + srow] : 0.f;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int64_t row = row0 + warp + 8 * i;
+    const float s = s_scale[lane >> 2][warp + 8 * i];
+    const uint32_t w[2] = {c[i].x, c[i].y};
+    float v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      v[j] = s * static_cast<float>(static_cast<int8_t>(w[j >> 2] >> (8 * (j & 3))));
+    if (row < m && col < k) store_piece8<DT>(out, row * ldo + col, col, k, vec, v);
+  }
+}
+
+// ---- backward of activation and bias ----
+// dz = dy act'(z), and the column sums of dz over a slab of rows (the bias
+// gradient's partial sums, added by column_sum_kernel in slab order: the same
+// result every time).  One pass over dy and z.  Without an activation only
+// the sums are formed (dz = dy).  A lane owns 8 columns, a block 256; warps
+// take every eighth row of the slab.
+struct ActBackward {
+  const void* dy;
+  int64_t lddy;
+  int vec_dy;
+  const void* z;  // 16-bit z, or null: 8-bit codes, or none
+  int64_t ldz;
+  int vec_z;
+  const int8_t* zq;
+  const float* zs;
+  int64_t n32;
+  void* dz;       // null: sums only
+  int64_t lddz;
+  int vec_dz;
+  float* partial;  // [slabs][n] or null
+  int64_t m, n, slab_rows;
+  int act;
+};
+
+template <bool BF16>
+__global__ void __launch_bounds__(256) act_backward_kernel(const ActBackward p) {
+  pdl_entry();
+  constexpr int DT = BF16 ? DSV4_BF16 : DSV4_F16;
+  __shared__ float s_sum[8][256];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t col = static_cast<int64_t>(blockIdx.x) * 256 + lane * 8;
+  const int64_t begin = static_cast<int64_t>(blockIdx.y) * p.slab_rows;
+  const int64_t end = begin + p.slab_rows < p.m ? begin + p.slab_rows : p.m;
+  float sum[8] = {};
+  if (col < p.n) {
+    act_dispatch(p.act, [&](auto kind) {
+      constexpr int K = decltype(kind)::value;
+#pragma unroll 4
+      for (int64_t row = begin + warp; row < end; row += 8) {
+        float d[8];
+        load_piece8<DT>(p.dy, row * p.lddy + col, col, p.n, p.vec_dy, d);
+        if constexpr (K != kActNone) {
+          float z[8];
+          if (p.zq) {
+            const uint2 c = *reinterpret_cast<const uint2*>(p.zq + row * p.n32 + col);
+            const float s = p.zs[(col / kGroup) * p.m + row];
+            const uint32_t w[2] = {c.x, c.y};
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              z[j] = s * static_cast<float>(static_cast<int8_t>(w[j >> 2] >> (8 * (j & 3))));
+          } else {
+            load_piece8<DT>(p.z, row * p.ldz + col, col, p.n, p.vec_z, z);
+          }
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            float a, slope;
+            act_both<K>(z[j], a, slope);
+            d[j] = col + j < p.n ? d[j] * slope : 0.f;
+          }
+          store_piece8<DT>(p.dz, row * p.lddz + col, col, p.n, p.vec_dz, d);
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) sum[j] += d[j];
+      }
+    });
+  }
+  if (!p.partial) return;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) s_sum[warp][lane * 8 + j] = sum[j];
+  __syncthreads();
+  const int64_t c = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  if (c < p.n) {
+    float t = 0.f;
+#pragma unroll
+    for (int w = 0; w < 8; ++w) t += s_sum[w][threadIdx.x];
+    p.partial[blockIdx.y * p.n + c] = t;
+  }
+}
+
+template <bool BF16>
+__global__ void __launch_bounds__(128)
+    column_sum_kernel(const float* __restrict__ partial, int64_t slabs, int64_t n,
+                      void* __restrict__ out) {
+  pdl_entry();
+  const int64_t c = static_cast<int64_t>(blockIdx.x) * 128 + threadIdx.x;
+  if (c >= n) return;
+  float t = 0.f;
+#pragma unroll 8
+  for (int64_t s = 0; s < slabs; ++s) t += partial[s * n + c];
+  static_cast<uint16_t*>(out)[c] = static_cast<uint16_t>(pack_16<BF16>(t, 0.f) & 0xffffu);
+}
+
+// ---- rows of any strides -> rows that TMA can read (16-byte aligned) ----
+// 32 x 32 tiles through shared memory: reads follow the smaller stride.
+__global__ void __launch_bounds__(256)
+    pack_rows_kernel(const uint16_t* __restrict__ in, int64_t s0, int64_t s1, int64_t rows,
+                     int64_t cols, int64_t col_blocks, uint16_t* __restrict__ out, int64_t ldo) {
+  pdl_entry();
+  __shared__ uint16_t tile[32][33];
+  const int a = threadIdx.x & 31, b = threadIdx.x >> 5;
+  const int64_t r0 = (blockIdx.x / col_blocks) * 32, c0 = (blockIdx.x % col_blocks) * 32;
+  const bool by_rows = s1 <= s0 || s0 == 0;
+#pragma unroll
+  for (int i = 0; i < 32; i += 8) {
+    const int r = by_rows ? b + i : a, c = by_rows ? a : b + i;
+    if (r0 + r < rows && c0 + c < cols) tile[r][c] = in[(r0 + r) * s0 + (c0 + c) * s1];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 32; i += 8)
+    if (r0 + b + i < rows && c0 + a < cols) out[(r0 + b + i) * ldo + c0 + a] = tile[b + i][a];
+}
+
+}  // namespace dsv4

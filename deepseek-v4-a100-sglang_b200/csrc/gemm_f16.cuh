@@ -1,0 +1,531 @@
+// 16-bit (bf16 / fp16) products on CTA pairs, with the feed-forward epilogues.
+//
+//   D[m][n] = sum_k A[m][k] B[n][k]      fp32 sums in tensor memory
+//
+// Either operand may lie in memory with its rows contiguous (K-major) or with
+// its contraction axis outermost (MN-major): the forward product reads both
+// K-major, the gradient of the input reads the weight MN-major, the gradient
+// of the weight reads both operands MN-major.  The matrix descriptors express
+// the difference; no operand is transposed in memory.
+//
+// One pair of CTAs (cta_group::2) computes a 256 x tn tile: each CTA stages
+// its own 128 rows of A and tn/2 rows of B, and the pair's MMA reads both
+// halves of B, so an operand byte fetched from L2 is used twice as often as by
+// single CTAs.  Roles: warp 0 TMA producer, warp 1 of the leader MMA issuer,
+// warps 4-11 epilogue.  The two 256-column accumulators in TMEM let the
+// epilogue of one tile overlap the products of the next.
+//
+// Epilogues (all arithmetic in fp32, one rounding when a value is stored):
+//   kEpiLinear    y = act(D + bias) + residual; optionally z = D + bias is
+//                 kept for the backward pass (16 bits, or 8 bits per group)
+//   kEpiGated     B holds gate rows [0, n) and up rows [n, 2n); the tile takes
+//                 tn/2 of each, so a thread has both factors of
+//                 h = act(min(g, L)) * clamp(u, -L, L) in its registers
+//   kEpiGatedBwd  D = dh; reads the kept g and u and writes
+//                 dg = dh u' act'(g') [g <= L], du = dh act(g') [|u| <= L]
+//                 (and h where it has to be formed again)
+#pragma once
+
+#include "common.cuh"
+#include "feed_forward_kernels.cuh"
+
+namespace dsv4 {
+
+enum F16Epi : int { kEpiLinear = 0, kEpiGated = 1, kEpiGatedBwd = 2 };
+
+enum F16DeviceErr : int {
+  kErrF16WaitEmpty = 0x201,
+  kErrF16WaitFull = 0x202,
+  kErrF16WaitAccFull = 0x203,
+  kErrF16WaitAccEmpty = 0x204,
+};
+
+constexpr int kF16Threads = 384;
+constexpr int kF16EpiWarps = 8;
+constexpr int kF16ABytes = 128 * 128;          // 128 rows x 64 elements of A per stage
+constexpr int kF16StageSlice = 2048;           // 32 x 32 16-bit values
+constexpr int kF16EpiBytes = kF16EpiWarps * 2 * kF16StageSlice;
+constexpr int kF16MaxStages = 12;
+constexpr int kF16SmemMax = 232448;
+constexpr int kF16BarBytes = 256;
+static_assert((2 * kF16MaxStages + 4) * 8 + 8 <= kF16BarBytes, "barrier area");
+
+// A row-major matrix that the epilogue reads or writes by 16-byte pieces where
+// its address and row stride allow it.
+struct F16Mat {
+  void* p;
+  int64_t ld;  // elements
+  int vec;     // 16-byte aligned base and rows
+};
+
+struct F16GemmParams {
+  CUtensorMap map_a, map_b;
+  int m, n, k;            // n: columns of D (kEpiGated: of h)
+  int tn;                 // B rows of a pair tile (kEpiGated: gate and up together)
+  int stages, b_stage;    // ring depth, bytes of B per stage and CTA
+  int a_mn, b_mn;         // 1: the operand is MN-major
+  int tiles_m, tiles_n, group_m;
+  int up_row;             // kEpiGated: B row of up row 0
+  int act;
+  float limit;            // infinity where there is none
+  const void* bias;
+  F16Mat residual, out;   // out: y, h (kEpiGatedBwd: h, or null)
+  F16Mat z0, z1;          // kept z (kEpiLinear: z0), or g and u; written forward, read backward
+  F16Mat d0, d1;          // kEpiGatedBwd: dg and du
+  int8_t* zq;             // 8-bit kept values: codes [m][halves * n32] ...
+  float* zs;              // ... and scales [halves * n32 / 32][m]
+  int64_t n32;            // n rounded up to the group
+};
+
+// ---- tcgen05 / TMA forms of the pair ----
+__device__ __forceinline__ void tma_load_2d_pair(uint32_t dst, const CUtensorMap* map, int c0,
+                                                 int c1, uint32_t cl_bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(cl_bar)
+      : "memory");
+}
+
+__device__ __forceinline__ void mma_f16_ss_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc,
+                                                uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+// Arrive on the barrier at this shared-memory offset in both CTAs of the pair
+// once all pair MMAs issued so far by this thread complete.
+__device__ __forceinline__ void mma_commit_both(uint32_t bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64"
+      " [%0], %1;" ::"r"(bar),
+      "h"(static_cast<uint16_t>(3))
+      : "memory");
+}
+
+// MN-major operand, 128-byte swizzle: 64 elements of the row axis side by side
+// (128 B), contraction steps 128 B apart.  Groups of 8 contraction steps are
+// 1024 B apart (SBO), groups of 64 rows one 8-KB box apart (LBO).
+__device__ __forceinline__ uint64_t smem_desc_sw128_mn(uint32_t saddr) {
+  uint64_t d = 0;
+  d |= static_cast<uint64_t>((saddr & 0x3FFFFu) >> 4);
+  d |= static_cast<uint64_t>(8192u >> 4) << 16;
+  d |= static_cast<uint64_t>(1024u >> 4) << 32;
+  d |= static_cast<uint64_t>(1u) << 46;
+  d |= static_cast<uint64_t>(2u) << 61;
+  return d;
+}
+
+// kind::f16, fp32 accumulator; A and B of the same type.
+__device__ __forceinline__ uint32_t idesc_f16(bool bf16, uint32_t m, uint32_t n, uint32_t a_mn,
+                                              uint32_t b_mn) {
+  const uint32_t t = bf16 ? 1u : 0u;
+  return (1u << 4) | (t << 7) | (t << 10) | (a_mn << 15) | (b_mn << 16) | ((n >> 3) << 17) |
+         ((m >> 4) << 24);
+}
+
+// ---- 32 x 32 chunks of 16-bit matrices: global <-> registers of a row ----
+// Lane l moves the 16-byte pieces of rows 8i + l/4, columns 8 (l & 3): four
+// lanes cover a row's 64 bytes, so accesses are whole sectors.  The shared
+// slice turns that into one row per lane; its 16-byte units are XORed with
+// bits of the row, which leaves both sides free of bank conflicts.
+__device__ __forceinline__ uint32_t slice_off(int row, int piece) {
+  return static_cast<uint32_t>(row * 64 + ((piece ^ ((row >> 1) & 3)) << 4));
+}
+
+__device__ __forceinline__ void chunk_fetch(uint4 (&r)[4], const F16Mat& mat, int lane, int row0,
+                                            int rows, int col0, int cols) {
+  const int col = col0 + 8 * (lane & 3);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int row = row0 + 8 * i + (lane >> 2);
+    r[i] = make_uint4(0, 0, 0, 0);
+    if (row < rows && col < cols) {
+      const uint16_t* p = static_cast<const uint16_t*>(mat.p) + row * mat.ld + col;
+      if (mat.vec && col + 8 <= cols) {
+        r[i] = *reinterpret_cast<const uint4*>(p);
+      } else {
+        uint16_t e[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) e[j] = col + j < cols ? p[j] : uint16_t(0);
+        r[i] = make_uint4(e[0] | (e[1] << 16), e[2] | (e[3] << 16), e[4] | (e[5] << 16),
+                          e[6] | (e[7] << 16));
+      }
+    }
+  }
+}
+
+__device__ __forceinline__ void chunk_to_rows(uint32_t slice, int lane, const uint4 (&r)[4],
+                                              uint32_t (&w)[16]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    st_shared_v4(slice + slice_off(8 * i + (lane >> 2), lane & 3), r[i]);
+  __syncwarp();
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    const uint4 v = ld_shared_v4(slice + slice_off(lane, c));
+    w[4 * c] = v.x, w[4 * c + 1] = v.y, w[4 * c + 2] = v.z, w[4 * c + 3] = v.w;
+  }
+  __syncwarp();
+}
+
+__device__ __forceinline__ void chunk_store(uint32_t slice, int lane, const uint32_t (&w)[16],
+                                            const F16Mat& mat, int row0, int rows, int col0,
+                                            int cols) {
+#pragma unroll
+  for (int c = 0; c < 4; ++c)
+    st_shared_v4(slice + slice_off(lane, c),
+                 make_uint4(w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]));
+  __syncwarp();
+  const int col = col0 + 8 * (lane & 3);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int row = row0 + 8 * i + (lane >> 2);
+    const uint4 v = ld_shared_v4(slice + slice_off(8 * i + (lane >> 2), lane & 3));
+    if (row < rows && col < cols) {
+      uint16_t* p = static_cast<uint16_t*>(mat.p) + row * mat.ld + col;
+      if (mat.vec && col + 8 <= cols) {
+        *reinterpret_cast<uint4*>(p) = v;
+      } else {
+        const uint32_t e[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (col + j < cols) p[j] = static_cast<uint16_t>(e[j >> 1] >> (16 * (j & 1)));
+      }
+    }
+  }
+  __syncwarp();
+}
+
+// 8-bit codes of a 32 x 32 chunk (rows of 32 bytes, always whole: the code
+// rows are padded to the group).
+__device__ __forceinline__ void codes_store(uint32_t slice, int lane, const uint32_t (&q)[8],
+                                            int8_t* base, int64_t ld, int row0, int rows,
+                                            int64_t col0) {
+  st_shared_v4(slice + lane * 32 + (((lane >> 2) & 1) << 4), make_uint4(q[0], q[1], q[2], q[3]));
+  st_shared_v4(slice + lane * 32 + ((((lane >> 2) & 1) ^ 1) << 4),
+               make_uint4(q[4], q[5], q[6], q[7]));
+  __syncwarp();
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int r = 16 * i + (lane >> 1), half = lane & 1;
+    const uint4 v = ld_shared_v4(slice + r * 32 + ((half ^ ((r >> 2) & 1)) << 4));
+    if (row0 + r < rows)
+      *reinterpret_cast<uint4*>(base + (row0 + r) * ld + col0 + 16 * half) = v;
+  }
+  __syncwarp();
+}
+
+__device__ __forceinline__ void codes_fetch(uint4 (&v)[2], const int8_t* base, int64_t ld,
+                                            int lane, int row0, int rows, int64_t col0) {
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int r = 16 * i + (lane >> 1);
+    v[i] = make_uint4(0, 0, 0, 0);
+    if (row0 + r < rows)
+      v[i] = *reinterpret_cast<const uint4*>(base + (row0 + r) * ld + col0 + 16 * (lane & 1));
+  }
+}
+
+__device__ __forceinline__ void codes_to_rows(uint32_t slice, int lane, const uint4 (&v)[2],
+                                              float scale, float (&x)[32]) {
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int r = 16 * i + (lane >> 1);
+    st_shared_v4(slice + r * 32 + (((lane & 1) ^ ((r >> 2) & 1)) << 4), v[i]);
+  }
+  __syncwarp();
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+    const uint4 c = ld_shared_v4(slice + lane * 32 + ((half ^ ((lane >> 2) & 1)) << 4));
+    const uint32_t w[4] = {c.x, c.y, c.z, c.w};
+#pragma unroll
+    for (int j = 0; j < 16; ++j)
+      x[16 * half + j] =
+          scale * static_cast<float>(static_cast<int8_t>(w[j >> 2] >> (8 * (j & 3))));
+  }
+  __syncwarp();
+}
+
+template <int EPI, bool BF16>
+__global__ void __launch_bounds__(kF16Threads, 1)
+    f16_pair_gemm_kernel(const __grid_constant__ F16GemmParams p) {
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t smem = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_ctarank();
+  const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+  const int stage_bytes = kF16ABytes + p.b_stage;
+  const uint32_t epi_smem = smem + p.stages * stage_bytes;
+  const uint32_t bars = epi_smem + kF16EpiBytes;
+  const auto full = [&](int s) { return bars + 8u * s; };
+  const auto empty = [&](int s) { return bars + 8u * (kF16MaxStages + s); };
+  const auto acc_full = [&](int b) { return bars + 8u * (2 * kF16MaxStages + b); };
+  const auto acc_empty = [&](int b) { return bars + 8u * (2 * kF16MaxStages + 2 + b); };
+  const uint32_t tmem_slot = bars + 8u * (2 * kF16MaxStages + 4);
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < p.stages; ++s) {
+      mbar_init(full(s), 1);
+      mbar_init(empty(s), 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(acc_full(b), 1);
+      mbar_init(acc_empty(b), 2 * kF16EpiWarps);
+    }
+    mbar_fence_init();
+    tma_prefetch_desc(&p.map_a);
+    tma_prefetch_desc(&p.map_b);
+  }
+  if (warp == 2) {
+    tmem_alloc_pair(tmem_slot, 512);
+    tmem_relinquish_pair();
+    tc_fence_before();
+  }
+  __syncthreads();
+  cluster_sync_all();
+  tc_fence_after();
+  const uint32_t tmem = ld_shared_u32(tmem_slot);
+  pdl_entry();
+
+  const int kblocks = (p.k + 63) >> 6;
+  const int tiles = p.tiles_m * p.tiles_n;
+  const int half_n = p.tn >> 1;
+  // tile -> (row tile, column tile): columns advance after group_m row tiles,
+  // so the tiles in flight share both operands in L2
+  const auto tile_at = [&](int t, int& tm, int& tc) {
+    const int per = p.group_m * p.tiles_n;
+    const int g = t / per, first = g * p.group_m;
+    const int rows = min(p.group_m, p.tiles_m - first);
+    const int r = t - g * per;
+    tm = first + r % rows;
+    tc = r / rows;
+  };
+
+  if (warp == 0 && lane == 0) {
+    // ---- TMA producer of this CTA's halves ----
+    uint32_t it = 0;
+    bool ok = true;
+    const int b_rows = p.b_mn ? (half_n + 63) >> 6 : 1;
+    for (int t = pair; t < tiles && ok; t += pairs) {
+      int tm, tc;
+      tile_at(t, tm, tc);
+      const int row = tm * 256 + static_cast<int>(rank) * 128;
+      const int brow = EPI == kEpiGated ? tc * half_n + (rank ? p.up_row : 0)
+                                        : tc * p.tn + static_cast<int>(rank) * half_n;
+      for (int kb = 0; kb < kblocks; ++kb, ++it) {
+        const int s = it % p.stages;
+        const uint32_t round = it / p.stages;
+        if (round > 0 && !mbar_wait_cl(empty(s), (round - 1) & 1, kErrF16WaitEmpty)) {
+          ok = false;
+          break;
+        }
+        if (rank == 0) mbar_arrive_expect_tx(full(s), 2 * stage_bytes);
+        const uint32_t bar = mapa_shared(full(s), 0);
+        const uint32_t a = smem + s * stage_bytes, b = a + kF16ABytes;
+        if (p.a_mn) {
+          tma_load_2d_pair(a, &p.map_a, row, kb * 64, bar);
+          tma_load_2d_pair(a + 8192, &p.map_a, row + 64, kb * 64, bar);
+        } else {
+          tma_load_2d_pair(a, &p.map_a, kb * 64, row, bar);
+        }
+        if (p.b_mn) {
+          for (int j = 0; j < b_rows; ++j)
+            tma_load_2d_pair(b + j * 8192, &p.map_b, brow + j * 64, kb * 64, bar);
+        } else {
+          tma_load_2d_pair(b, &p.map_b, kb * 64, brow, bar);
+        }
+      }
+    }
+    // the last commits arrive here before this CTA may exit
+    const uint32_t tail = it < static_cast<uint32_t>(p.stages) ? it : p.stages;
+    for (uint32_t i = it - tail; ok && i < it; ++i)
+      ok = mbar_wait_cl(empty(i % p.stages), (i / p.stages) & 1, kErrF16WaitEmpty);
+    if (!ok) {  // copies in flight land before shared memory is given up
+      const unsigned long long t0 = globaltimer_ns();
+      while (globaltimer_ns() - t0 < 1000000ull) {
+      }
+    }
+  } else if (warp == 1 && rank == 0 && lane == 0) {
+    // ---- MMA issuer of the pair ----
+    const uint32_t idesc = idesc_f16(BF16, 256, p.tn, p.a_mn, p.b_mn);
+    const uint32_t a_step = p.a_mn ? 2048u : 32u, b_step = p.b_mn ? 2048u : 32u;
+    uint32_t it = 0, nt = 0;
+    bool ok = true;
+    for (int t = pair; t < tiles && ok; t += pairs, ++nt) {
+      const uint32_t buf = nt & 1, use = nt >> 1;
+      if (use > 0 && !mbar_wait_cl(acc_empty(buf), (use - 1) & 1, kErrF16WaitAccEmpty)) break;
+      tc_fence_after();
+      const uint32_t d = tmem + buf * 256;
+      for (int kb = 0; kb < kblocks; ++kb, ++it) {
+        const int s = it % p.stages;
+        if (!mbar_wait_cl(full(s), (it / p.stages) & 1, kErrF16WaitFull)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        const uint32_t a = smem + s * stage_bytes, b = a + kF16ABytes;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const uint64_t ad = p.a_mn ? smem_desc_sw128_mn(a + j * a_step)
+                                     : smem_desc_sw128(a + j * a_step);
+          const uint64_t bd = p.b_mn ? smem_desc_sw128_mn(b + j * b_step)
+                                     : smem_desc_sw128(b + j * b_step);
+          mma_f16_ss_pair(d, ad, bd, idesc, (kb | j) != 0);
+        }
+        mma_commit_both(empty(s));
+      }
+      if (ok) mma_commit_both(acc_full(buf));
+    }
+  } else if (warp >= 4) {
+    // ---- epilogue: warp w reads TMEM lanes 32 (w & 3).., every second chunk ----
+    const int quarter = warp & 3, side = (warp - 4) >> 2;
+    const uint32_t slice0 = epi_smem + (warp - 4) * 2 * kF16StageSlice;
+    const uint32_t slice1 = slice0 + kF16StageSlice;
+    const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
+    const bool limited = p.limit < CUDART_INF_F;
+    uint32_t nt = 0;
+    for (int t = pair; t < tiles; t += pairs, ++nt) {
+      int tm, tc;
+      tile_at(t, tm, tc);
+      const uint32_t buf = nt & 1, use = nt >> 1;
+      const int row0 = tm * 256 + static_cast<int>(rank) * 128 + quarter * 32;
+      const int row = row0 + lane;
+      if (!mbar_wait_cl(acc_full(buf), use & 1, kErrF16WaitAccFull)) break;
+      tc_fence_after();
+      const uint32_t acc = tmem + buf * 256 + lanes;
+      const int width = EPI == kEpiGated ? half_n : p.tn;
+      const int cbase = tc * width;
+      for (int c0 = side * 32; c0 < width; c0 += 64) {
+        const int col = cbase + c0;
+        if (col >= p.n) break;
+        if constexpr (EPI == kEpiLinear) {
+          uint4 rres[4];
+          if (p.residual.p) chunk_fetch(rres, p.residual, lane, row0, p.m, col, p.n);
+          float v[32];
+          tmem_ld_f32x32(acc + c0, v);
+          if (p.bias) {
+            const float bl = col + lane < p.n ? ld_16<BF16>(p.bias, col + lane) : 0.f;
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[j] += __shfl_sync(0xffffffffu, bl, j);
+          }
+          uint32_t w[16];
+          if (p.z0.p) {
+            pack_row<BF16>(v, w);
+            chunk_store(slice0, lane, w, p.z0, row0, p.m, col, p.n);
+          } else if (p.zq) {
+            if (col + 32 > p.n) {
+#pragma unroll
+              for (int j = 0; j < 32; ++j)
+                if (col + j >= p.n) v[j] = 0.f;
+            }
+            uint32_t q[8];
+            const float s = quantize_group(v, q);
+            codes_store(slice0, lane, q, p.zq, p.n32, row0, p.m, col);
+            if (row < p.m) p.zs[static_cast<int64_t>(col >> 5) * p.m + row] = s;
+          }
+          act_row(p.act, v);
+          if (p.residual.p) {
+            chunk_to_rows(slice1, lane, rres, w);
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[j] += unpack_16<BF16>(w[j >> 1], j & 1);
+          }
+          pack_row<BF16>(v, w);
+          chunk_store(slice0, lane, w, p.out, row0, p.m, col, p.n);
+        } else if constexpr (EPI == kEpiGated) {
+          float g[32], u[32];
+          tmem_ld_f32x32(acc + c0, g);
+          tmem_ld_f32x32(acc + half_n + c0, u);
+          uint32_t w[16];
+          if (p.z0.p) {
+            if (limited) {
+              pack_row_sided<BF16>(g, w, p.limit);
+            } else {
+              pack_row<BF16>(g, w);
+            }
+            chunk_store(slice0, lane, w, p.z0, row0, p.m, col, p.n);
+            if (limited) {
+              pack_row_sided<BF16>(u, w, p.limit);
+            } else {
+              pack_row<BF16>(u, w);
+            }
+            chunk_store(slice1, lane, w, p.z1, row0, p.m, col, p.n);
+          } else if (p.zq) {
+            if (col + 32 > p.n) {
+#pragma unroll
+              for (int j = 0; j < 32; ++j)
+                if (col + j >= p.n) g[j] = u[j] = 0.f;
+            }
+            uint32_t q[8];
+            const float sg = quantize_group(g, q);
+            codes_store(slice0, lane, q, p.zq, 2 * p.n32, row0, p.m, col);
+            const float su = quantize_group(u, q);
+            codes_store(slice1, lane, q, p.zq, 2 * p.n32, row0, p.m, p.n32 + col);
+            if (row < p.m) {
+              p.zs[static_cast<int64_t>(col >> 5) * p.m + row] = sg;
+              p.zs[((p.n32 + col) >> 5) * p.m + row] = su;
+            }
+          }
+#pragma unroll
+          for (int j = 0; j < 32; ++j) {
+            g[j] = clamp_top(g[j], p.limit);
+            u[j] = clamp_both(u[j], p.limit);
+          }
+          act_row(p.act, g);
+#pragma unroll
+          for (int j = 0; j < 32; ++j) g[j] *= u[j];
+          pack_row<BF16>(g, w);
+          chunk_store(slice0, lane, w, p.out, row0, p.m, col, p.n);
+        } else {
+          float g[32], u[32];
+          if (p.zq) {
+            uint4 cg[2], cu[2];
+            codes_fetch(cg, p.zq, 2 * p.n32, lane, row0, p.m, col);
+            codes_fetch(cu, p.zq, 2 * p.n32, lane, row0, p.m, p.n32 + col);
+            float sg = 0.f, su = 0.f;
+            if (row < p.m) {
+              sg = p.zs[static_cast<int64_t>(col >> 5) * p.m + row];
+              su = p.zs[((p.n32 + col) >> 5) * p.m + row];
+            }
+            codes_to_rows(slice0, lane, cg, sg, g);
+            codes_to_rows(slice1, lane, cu, su, u);
+          } else {
+            uint4 rg[4], ru[4];
+            chunk_fetch(rg, p.z0, lane, row0, p.m, col, p.n);
+            chunk_fetch(ru, p.z1, lane, row0, p.m, col, p.n);
+            uint32_t w[16];
+            chunk_to_rows(slice0, lane, rg, w);
+#pragma unroll
+            for (int j = 0; j < 32; ++j) g[j] = unpack_16<BF16>(w[j >> 1], j & 1);
+            chunk_to_rows(slice1, lane, ru, w);
+#pragma unroll
+            for (int j = 0; j < 32; ++j) u[j] = unpack_16<BF16>(w[j >> 1], j & 1);
+          }
+          float v[32];
+          tmem_ld_f32x32(acc + c0, v);
+          uint32_t w[16], wu[16], wh[16];
+          gated_backward_row<BF16>(p.act, p.limit, v, g, u, w, wu, wh);
+          chunk_store(slice0, lane, w, p.d0, row0, p.m, col, p.n);
+          chunk_store(slice1, lane, wu, p.d1, row0, p.m, col, p.n);
+          if (p.out.p) chunk_store(slice0, lane, wh, p.out, row0, p.m, col, p.n);
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_cl(mapa_shared(acc_empty(buf), 0));
+    }
+  }
+  tc_fence_before();
+  __syncwarp();
+  cluster_sync_all();
+  if (warp == 2) {
+    tc_fence_after();
+    tmem_dealloc_pair(tmem, 512);
+  }
+}
+
+}  // namespace dsv4

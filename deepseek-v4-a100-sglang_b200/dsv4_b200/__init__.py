@@ -37,3 +37,16 @@ from .jit_ops import (  # noqa: F401
     prewarm_mxfp4_int8_moe_jit_modules,
 )
 from ._native import DeviceTimeoutError, check_device_status  # noqa: F401,E402
+from .feed_forward import (  # noqa: F401,E402
+    Int8Checkpoint,
+    SavedDense,
+    SavedFeedForward,
+    checkpoint_int8,
+    dense_backward,
+    dense_forward,
+    dense_forward_save,
+    gated_feed_forward,
+    gated_feed_forward_backward,
+    gated_feed_forward_save,
+    restore_int8,
+)

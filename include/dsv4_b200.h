@@ -383,6 +383,77 @@ DSV4_API int dsv4_b200_mxfp4_int8_dense_gemm_noalloc(const int8_t* a_q, const fl
                                                      const float* b_channel_scale, int64_t n,
                                                      void* out, void* stream);
 
+/* ---- 16-bit feed-forward operators (bf16 / fp16, fp32 sums) ----
+ *
+ * The shared expert, dense layers and projections beside the routed experts,
+ * with the backward passes that fine-tuning them needs.  Matrices are 2-D
+ * with a row stride (ld, elements).  Operands of a product (a, b, x, w, dy)
+ * are 16-byte aligned with a row stride that is a multiple of 8; `*_mn` = 0
+ * means rows of the contraction axis ([rows][k]), 1 the transposed storage
+ * ([k][rows]).  dsv4_b200_pack_rows lays out an operand of any strides.
+ * Results and `residual` have any alignment.  activation: dsv4_activation.
+ * 8-bit kept values: int8 codes [m][ceil32(k)] and fp32 scales
+ * [ceil32(k) / 32][m]: groups of 32 values of a row share a scale amax / 127
+ * (rounded toward zero);
+ * code = 127 v / amax rounded to nearest even; a group with an infinity or a
+ * NaN decodes to NaN, one whose amax is below 2^-100 to zeros.  Codes and
+ * scales of gate and up lie behind each other (ceil32(intermediate) each). */
+typedef enum dsv4_activation {
+  DSV4_ACT_NONE = 0,
+  DSV4_ACT_RELU = 1,
+  DSV4_ACT_SILU = 2,
+  DSV4_ACT_GELU = 3,      /* 0.5 z (1 + erf(z / sqrt 2)) */
+  DSV4_ACT_GELU_TANH = 4  /* 0.5 z (1 + tanh(sqrt(2/pi) (z + 0.044715 z^3))) */
+} dsv4_activation;
+
+/* out[m][n] = act(a b^T + bias) + residual; bias [n] and residual may be NULL;
+ * ldr = 0 adds the same row everywhere.
+ * z (or z_codes + z_scales) receives a b^T + bias for the backward pass. */
+DSV4_API int dsv4_b200_dense_gemm(const void* a, int64_t lda, int a_mn, const void* b, int64_t ldb,
+                                  int b_mn, int64_t m, int64_t n, int64_t k, int dtype,
+                                  const void* bias, int activation, const void* residual,
+                                  int64_t ldr, void* out, int64_t ldo, void* z, int64_t ldz,
+                                  int8_t* z_codes, float* z_scales, void* stream);
+
+/* h[m][intermediate] = act(min(g, L)) * clamp(u, -L, L), g and u the products
+ * of x with rows [0, intermediate) and [intermediate, 2 intermediate) of w13.
+ * z [m][2 intermediate] (or its codes) receives g and u before the clamp.
+ * w_mn = 1 needs intermediate % 8 == 0. */
+DSV4_API int dsv4_b200_gated_gemm(const void* x, int64_t ldx, int x_mn, const void* w13, int64_t ldw,
+                                  int w_mn, int64_t m, int64_t intermediate, int64_t k, int dtype,
+                                  int activation, int has_clamp, float clamp_limit, void* h,
+                                  int64_t ldh, void* z, int64_t ldz, int8_t* z_codes,
+                                  float* z_scales, void* stream);
+
+/* Backward of the gate: dh = dy w2 (w2 [k][intermediate], or with w_mn = 0 its
+ * transpose) stays in registers; dz [m][2 intermediate] = the gradients of g
+ * and u; h (may be NULL) is formed again from the kept z. */
+DSV4_API int dsv4_b200_gated_backward_gemm(const void* dy, int64_t lddy, int dy_mn, const void* w2,
+                                           int64_t ldw, int w_mn, int64_t m, int64_t intermediate,
+                                           int64_t k, int dtype, int activation, int has_clamp,
+                                           float clamp_limit, const void* z, int64_t ldz,
+                                           const int8_t* z_codes, const float* z_scales, void* dz,
+                                           int64_t lddz, void* h, int64_t ldh, void* stream);
+
+/* Activations in 8 bits: x [m][k] fp32 / fp16 / bf16 -> codes, scales; and back. */
+DSV4_API int dsv4_b200_checkpoint_int8(const void* x, int dtype, int64_t m, int64_t k, int64_t ldx,
+                                       int8_t* codes, float* scales, void* stream);
+DSV4_API int dsv4_b200_restore_int8(const int8_t* codes, const float* scales, int64_t m, int64_t k,
+                                    void* out, int dtype, int64_t ldo, void* stream);
+
+/* dz = dy act'(z) and dbias = the column sums of dz (dbias may be NULL; with
+ * DSV4_ACT_NONE dz = dy is not written).  partial: fp32 [slabs][n], at least
+ * the number of slabs that dsv4_b200_act_backward_slabs reports. */
+DSV4_API int dsv4_b200_act_backward_slabs(int64_t m, int64_t n, int64_t* slabs);
+DSV4_API int dsv4_b200_act_backward(const void* dy, int64_t lddy, const void* z, int64_t ldz,
+                                    const int8_t* z_codes, const float* z_scales, int64_t m,
+                                    int64_t n, int dtype, int activation, void* dz, int64_t lddz,
+                                    float* partial, int64_t slabs, void* dbias, void* stream);
+
+/* 16-bit elements of any strides -> rows with stride ldo. */
+DSV4_API int dsv4_b200_pack_rows(const void* in, int64_t row_stride, int64_t col_stride,
+                                 int64_t rows, int64_t cols, void* out, int64_t ldo, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
