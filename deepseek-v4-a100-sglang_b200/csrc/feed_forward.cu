@@ -8,6 +8,7 @@
 
 #include "feed_forward_kernels.cuh"
 #include "gemm_f16.cuh"
+#include "gemm_f16_stream.cuh"
 
 namespace dsv4 {
 
@@ -101,6 +102,60 @@ int launch_pair_gemm(F16GemmParams& p, const void* a, int64_t lda, int a_mn, con
   return check_launch("f16_pair_gemm_kernel");
 }
 
+// Few tokens: the weight-streaming kernel.  Clusters as large as still run at
+// once (one CTA per SM) and leave every CTA two blocks of k; a deep ring then,
+// half of it where more CTAs than SMs share them.
+template <int EPI>
+int launch_stream_gemm(const F16GemmParams& q, const void* x, int64_t ldx, int x_mn, const void* w,
+                       int64_t w_rows, int64_t ldw, int w_mn, bool bf16, cudaStream_t st) {
+  F16StreamParams p = {};
+  p.m = q.m, p.n = q.n, p.k = q.k;
+  p.tn = static_cast<int>(round_up(q.m < kStreamMaxTokens ? q.m : kStreamMaxTokens, 16));
+  p.tmem_cols = 32;
+  while (p.tmem_cols < p.tn) p.tmem_cols *= 2;
+  p.w_mn = w_mn != 0, p.x_mn = x_mn != 0;
+  p.up_row = q.up_row, p.act = q.act, p.limit = q.limit, p.bias = q.bias;
+  p.residual = q.residual, p.out = q.out;
+  const int width = EPI == kEpiGated ? 64 : 128;
+  p.row_tiles = (q.n + width - 1) / width;
+  const int64_t tiles = static_cast<int64_t>(p.row_tiles) * ((q.m + p.tn - 1) / p.tn);
+  const int kblocks = (q.k + 63) / 64;
+  p.cluster = 1;
+  while (p.cluster < 8 && tiles * p.cluster * 2 <= sm_count() && kblocks >= p.cluster * 4)
+    p.cluster *= 2;
+  const int64_t ctas = tiles * p.cluster;
+  DSV4_REQUIRE(ctas < (1ll << 31), "product too large");
+  p.x_stage = p.x_mn ? (p.tn + 63) / 64 * 8192 : p.tn * 128;
+  const int stage = kF16ABytes + p.x_stage, fixed = 1024 + kStreamBarBytes;
+  p.stages = ((ctas <= sm_count() ? 200 * 1024 : 112 * 1024) - fixed) / stage;
+  if (p.stages > kStreamMaxStages) p.stages = kStreamMaxStages;
+  if (int r = encode_operand(&p.map_w, "b", w, w_rows, p.k, ldw, p.w_mn, width, bf16)) return r;
+  if (int r = encode_operand(&p.map_x, "a", x, p.m, p.k, ldx, p.x_mn, p.tn, bf16)) return r;
+  const size_t smem = fixed + static_cast<size_t>(p.stages) * stage;
+  const dim3 grid(static_cast<unsigned>(ctas));
+  const unsigned cl = static_cast<unsigned>(p.cluster);
+  if (bf16) {
+    launch_cluster(&f16_stream_gemm_kernel<EPI, true>, grid, dim3(kStreamThreads), smem, st, cl, p);
+  } else {
+    launch_cluster(&f16_stream_gemm_kernel<EPI, false>, grid, dim3(kStreamThreads), smem, st, cl, p);
+  }
+  return check_launch("f16_stream_gemm_kernel");
+}
+
+template <int EPI>
+cudaError_t stream_attrs() {
+  cudaError_t e = cudaFuncSetAttribute(reinterpret_cast<void*>(&f16_stream_gemm_kernel<EPI, true>),
+                                       cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024);
+  if (e != cudaSuccess) return e;
+  return cudaFuncSetAttribute(reinterpret_cast<void*>(&f16_stream_gemm_kernel<EPI, false>),
+                              cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024);
+}
+
+// Up to 128 tokens whose values before the activation are not kept.
+bool takes_stream(const F16GemmParams& p) {
+  return p.m <= kStreamMaxTokens && p.z0.p == nullptr && p.zq == nullptr;
+}
+
 constexpr int64_t kMaxDim = 1ll << 30;
 constexpr float kNoLimit = std::numeric_limits<float>::infinity();
 
@@ -133,6 +188,8 @@ int feed_forward_init() {
   cudaError_t e = pair_attrs<kEpiLinear>();
   if (e == cudaSuccess) e = pair_attrs<kEpiGated>();
   if (e == cudaSuccess) e = pair_attrs<kEpiGatedBwd>();
+  if (e == cudaSuccess) e = stream_attrs<kEpiLinear>();
+  if (e == cudaSuccess) e = stream_attrs<kEpiGated>();
   if (e != cudaSuccess)
     return fail(DSV4_ERR_CUDA, "cudaFuncSetAttribute: %s", cudaGetErrorString(e));
   return DSV4_OK;
@@ -176,6 +233,9 @@ int dsv4_b200_dense_gemm(const void* a, int64_t lda, int a_mn, const void* b, in
   p.out = mat16(out, ldo);
   p.z0 = mat16(z, ldz);
   p.zq = z_codes, p.zs = z_scales, p.n32 = round_up(n, kGroup);
+  if (takes_stream(p))
+    return launch_stream_gemm<kEpiLinear>(p, a, lda, a_mn, b, n, ldb, b_mn, dtype == DSV4_BF16,
+                                          as_stream(stream));
   return launch_pair_gemm<kEpiLinear>(p, a, lda, a_mn, b, n, ldb, b_mn, dtype == DSV4_BF16,
                                       as_stream(stream));
 }
@@ -204,6 +264,9 @@ int dsv4_b200_gated_gemm(const void* x, int64_t ldx, int x_mn, const void* w13, 
   p.z0 = mat16(z, ldz);
   p.z1 = z ? mat16(static_cast<uint16_t*>(z) + intermediate, ldz) : mat16(nullptr, 0);
   p.zq = z_codes, p.zs = z_scales, p.n32 = round_up(intermediate, kGroup);
+  if (takes_stream(p))
+    return launch_stream_gemm<kEpiGated>(p, x, ldx, x_mn, w13, 2 * intermediate, ldw, w_mn,
+                                         dtype == DSV4_BF16, as_stream(stream));
   return launch_pair_gemm<kEpiGated>(p, x, ldx, x_mn, w13, 2 * intermediate, ldw, w_mn,
                                      dtype == DSV4_BF16, as_stream(stream));
 }

@@ -207,58 +207,92 @@ constexpr int kGroup = 32;
 constexpr float kTinyGroup = 7.8886090522101181e-31f;  // 2^-100
 
 struct GroupScale {
-  float inv;    // 127 / amax, 0 for an empty or non-finite group
-  float amax;
+  float mul;    // 127, or 127 * 2^-64 where 127 v could overflow
+  float amax;   // times the same power of two
+  float rcp;    // 1 / amax, 0 for an empty or non-finite group
   float scale;
 };
 
 __device__ __forceinline__ GroupScale group_scale(uint32_t amax_bits) {
   const float amax = __uint_as_float(amax_bits);
-  if (amax_bits >= 0x7f800000u) return {0.f, amax, CUDART_NAN_F};
-  if (amax < kTinyGroup) return {0.f, amax, 0.f};
-  // toward zero: 127 steps never pass amax, so the largest finite value stays finite
-  return {127.f / amax, amax, __fdiv_rz(amax, 127.f)};
+  if (amax_bits >= 0x7f800000u) return {0.f, 1.f, 0.f, CUDART_NAN_F};
+  if (amax < kTinyGroup) return {0.f, 1.f, 0.f, 0.f};
+  const float shrink = amax > 1.8446744e19f ? 5.4210109e-20f : 1.f;  // 2^64, 2^-64
+  const float a = amax * shrink;
+  // the scale toward zero: 127 steps never pass amax, so the largest finite
+  // value stays finite
+  return {127.f * shrink, a, __frcp_rn(a), __fdiv_rz(amax, 127.f)};
 }
 
-// The quotient in fp32 is off by less than 2e-5 at 127; only within 6e-5 of a
-// half can that change the code.  There the sign of 127 v - (f + 1/2) amax
-// decides, taken exactly: both products as rounded part + remainder.
-__device__ __forceinline__ int quantize_code(float v, const GroupScale& g) {
-  const float q = v * g.inv;
+// The quotient 127 v / amax.  p = 127 v is exact for 16-bit v; the first
+// estimate p rcp is off by a few units of the last place, and one step with
+// the exact remainder p - q amax makes it the correctly rounded quotient: a tie
+// (k + 1/2) comes out as itself, and other quotients of 16-bit values lie at
+// least 2^-18 (relative) away from one, against 2^-24.
+__device__ __forceinline__ float group_quotient(float v, const GroupScale& g) {
+  const float p = v * g.mul, q = p * g.rcp;
+  return __fmaf_rn(__fmaf_rn(-q, g.amax, p), g.rcp, q);
+}
+
+// fp32 values: within 6e-5 of a half the sign of 127 v - (f + 1/2) amax
+// decides, taken exactly (both products as rounded part + remainder).
+__device__ __noinline__ int quantize_code_near(float v, float q, const GroupScale& g) {
   const float f = floorf(fabsf(q));
-  const float frac = fabsf(q) - f;
-  if (fabsf(frac - 0.5f) < 6e-5f) {
-    const float shrink = g.amax > 1.8446744e19f ? 5.4210109e-20f : 1.f;  // 2^64, 2^-64
-    const float a = g.amax * shrink, x = fabsf(v) * shrink, c = f + 0.5f;
-    const float p = 127.f * x, pl = __fmaf_rn(127.f, x, -p);
-    const float t = c * a, tl = __fmaf_rn(c, a, -t);
-    const float d = (p - t) + (pl - tl);
-    const int fi = static_cast<int>(f);
-    const int r = d > 0.f ? fi + 1 : d < 0.f ? fi : fi + (fi & 1);
-    return q < 0.f ? -r : r;
-  }
-  return __float2int_rn(q);
+  if (fabsf(fabsf(q) - f - 0.5f) >= 6e-5f) return __float2int_rn(q);
+  const float x = fabsf(v) * (g.mul > 1.f ? 1.f : 5.4210109e-20f), c = f + 0.5f;
+  const float p = 127.f * x, pl = __fmaf_rn(127.f, x, -p);
+  const float t = c * g.amax, tl = __fmaf_rn(c, g.amax, -t);
+  const float d = (p - t) + (pl - tl);
+  const int fi = static_cast<int>(f);
+  const int r = d > 0.f ? fi + 1 : d < 0.f ? fi : fi + (fi & 1);
+  return q < 0.f ? -r : r;
 }
 
-// A thread's own group: codes (4 per word) and the scale.
+// Four quotients -> four code bytes: adding 1.5 * 2^23 rounds to the nearest
+// whole number (ties to even) and leaves it in the low bits.
+__device__ __forceinline__ uint32_t pack_codes(float a, float b, float c, float d) {
+  constexpr float kMagic = 12582912.f;
+  const uint32_t lo = prmt(__float_as_uint(a + kMagic), __float_as_uint(b + kMagic), 0x0040u);
+  const uint32_t hi = prmt(__float_as_uint(c + kMagic), __float_as_uint(d + kMagic), 0x0040u);
+  return prmt(lo, hi, 0x5410u);
+}
+
+// 4 codes; EXACT32 for values with all of fp32's digits
+template <bool EXACT32>
+__device__ __forceinline__ uint32_t quantize4(float a, float b, float c, float d,
+                                              const GroupScale& g) {
+  const float q[4] = {group_quotient(a, g), group_quotient(b, g), group_quotient(c, g),
+                      group_quotient(d, g)};
+  if constexpr (EXACT32) {
+    const float v[4] = {a, b, c, d};
+    float near = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) near = fmaxf(near, fabsf(q[i] - rintf(q[i])));
+    if (near > 0.4999f) {
+      uint32_t w = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        w |= (static_cast<uint32_t>(quantize_code_near(v[i], q[i], g)) & 0xffu) << (8 * i);
+      return w;
+    }
+  }
+  return pack_codes(q[0], q[1], q[2], q[3]);
+}
+
+// A thread's own group of fp32 sums: codes (4 per word) and the scale.
 __device__ __forceinline__ float quantize_group(const float (&v)[32], uint32_t (&codes)[8]) {
   uint32_t top = 0;
 #pragma unroll
   for (int j = 0; j < 32; ++j) top = max(top, __float_as_uint(v[j]) & 0x7fffffffu);
   const GroupScale g = group_scale(top);
-  if (g.inv == 0.f) {
+  if (g.rcp == 0.f) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) codes[j] = 0;
     return g.scale;
   }
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    uint32_t w = 0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      w |= (static_cast<uint32_t>(quantize_code(v[4 * j + i], g)) & 0xffu) << (8 * i);
-    codes[j] = w;
-  }
+  for (int j = 0; j < 8; ++j)
+    codes[j] = quantize4<false>(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3], g);
   return g.scale;
 }
 
@@ -354,10 +388,11 @@ __global__ void __launch_bounds__(256)
     if ((lane & 3) == 0) s_scale[lane >> 2][warp + 8 * i] = g.scale;
     if (row < m && col < k32) {
       uint32_t w[2] = {0, 0};
-      if (g.inv != 0.f) {
+      if (g.rcp != 0.f) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-          w[j >> 2] |= (static_cast<uint32_t>(quantize_code(v[i][j], g)) & 0xffu) << (8 * (j & 3));
+        for (int j = 0; j < 2; ++j)
+          w[j] = quantize4<DT == DSV4_F32>(v[i][4 * j], v[i][4 * j + 1], v[i][4 * j + 2],
+                                           v[i][4 * j + 3], g);
       }
       *reinterpret_cast<uint2*>(codes + row * k32 + col) = make_uint2(w[0], w[1]);
     }

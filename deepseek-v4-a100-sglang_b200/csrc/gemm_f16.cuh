@@ -120,6 +120,25 @@ __device__ __forceinline__ uint64_t smem_desc_sw128_mn(uint32_t saddr) {
   return d;
 }
 
+// Place in a ring of `stages`: slot and parity of its current use, stepped
+// without divisions (one thread walks it: its latency is the loop's).
+struct RingCursor {
+  int slot = 0;
+  uint32_t parity = 0;
+  __device__ __forceinline__ void step(int stages) {
+    if (++slot == stages) slot = 0, parity ^= 1;
+  }
+};
+
+// Descriptor of an operand at shared address 0; desc_addr() is added to it.
+// In a cluster a shared address carries the CTA's rank above its 18 bits of
+// offset: without the mask they would run into the LBO field.
+__device__ __forceinline__ uint32_t desc_addr(uint32_t saddr) { return (saddr & 0x3FFFFu) >> 4; }
+
+__device__ __forceinline__ uint64_t operand_desc(int mn) {
+  return mn ? smem_desc_sw128_mn(0) : smem_desc_sw128(0);
+}
+
 // kind::f16, fp32 accumulator; A and B of the same type.
 __device__ __forceinline__ uint32_t idesc_f16(bool bf16, uint32_t m, uint32_t n, uint32_t a_mn,
                                               uint32_t b_mn) {
@@ -308,43 +327,53 @@ __global__ void __launch_bounds__(kF16Threads, 1)
 
   if (warp == 0 && lane == 0) {
     // ---- TMA producer of this CTA's halves ----
-    uint32_t it = 0;
+    RingCursor ring;
+    uint32_t filled = 0;  // slots in use at the end, up to the ring's depth
     bool ok = true;
-    const int b_rows = p.b_mn ? (half_n + 63) >> 6 : 1;
+    const int b_boxes = p.b_mn ? (half_n + 63) >> 6 : 1;
+    const uint32_t leader = mapa_shared(bars, 0);
     for (int t = pair; t < tiles && ok; t += pairs) {
       int tm, tc;
       tile_at(t, tm, tc);
       const int row = tm * 256 + static_cast<int>(rank) * 128;
       const int brow = EPI == kEpiGated ? tc * half_n + (rank ? p.up_row : 0)
                                         : tc * p.tn + static_cast<int>(rank) * half_n;
-      for (int kb = 0; kb < kblocks; ++kb, ++it) {
-        const int s = it % p.stages;
-        const uint32_t round = it / p.stages;
-        if (round > 0 && !mbar_wait_cl(empty(s), (round - 1) & 1, kErrF16WaitEmpty)) {
-          ok = false;
-          break;
+      for (int kk = 0; kk < kblocks * 64; kk += 64) {
+        const int s = ring.slot;
+        if (filled == static_cast<uint32_t>(p.stages)) {
+          if (!mbar_wait_cl(empty(s), ring.parity ^ 1, kErrF16WaitEmpty)) {
+            ok = false;
+            break;
+          }
+        } else {
+          ++filled;
         }
         if (rank == 0) mbar_arrive_expect_tx(full(s), 2 * stage_bytes);
-        const uint32_t bar = mapa_shared(full(s), 0);
+        const uint32_t bar = leader + 8u * s;
         const uint32_t a = smem + s * stage_bytes, b = a + kF16ABytes;
         if (p.a_mn) {
-          tma_load_2d_pair(a, &p.map_a, row, kb * 64, bar);
-          tma_load_2d_pair(a + 8192, &p.map_a, row + 64, kb * 64, bar);
+          tma_load_2d_pair(a, &p.map_a, row, kk, bar);
+          tma_load_2d_pair(a + 8192, &p.map_a, row + 64, kk, bar);
         } else {
-          tma_load_2d_pair(a, &p.map_a, kb * 64, row, bar);
+          tma_load_2d_pair(a, &p.map_a, kk, row, bar);
         }
         if (p.b_mn) {
-          for (int j = 0; j < b_rows; ++j)
-            tma_load_2d_pair(b + j * 8192, &p.map_b, brow + j * 64, kb * 64, bar);
+          for (int j = 0; j < b_boxes; ++j)
+            tma_load_2d_pair(b + j * 8192, &p.map_b, brow + j * 64, kk, bar);
         } else {
-          tma_load_2d_pair(b, &p.map_b, kb * 64, brow, bar);
+          tma_load_2d_pair(b, &p.map_b, kk, brow, bar);
         }
+        ring.step(p.stages);
       }
     }
-    // the last commits arrive here before this CTA may exit
-    const uint32_t tail = it < static_cast<uint32_t>(p.stages) ? it : p.stages;
-    for (uint32_t i = it - tail; ok && i < it; ++i)
-      ok = mbar_wait_cl(empty(i % p.stages), (i / p.stages) & 1, kErrF16WaitEmpty);
+    // the last commits arrive here before this CTA may exit: the slots in use,
+    // oldest first
+    if (filled < static_cast<uint32_t>(p.stages)) ring = RingCursor{};
+    else ring.parity ^= 1;
+    for (uint32_t i = 0; ok && i < filled; ++i) {
+      ok = mbar_wait_cl(empty(ring.slot), ring.parity, kErrF16WaitEmpty);
+      ring.step(p.stages);
+    }
     if (!ok) {  // copies in flight land before shared memory is given up
       const unsigned long long t0 = globaltimer_ns();
       while (globaltimer_ns() - t0 < 1000000ull) {
@@ -353,31 +382,34 @@ __global__ void __launch_bounds__(kF16Threads, 1)
   } else if (warp == 1 && rank == 0 && lane == 0) {
     // ---- MMA issuer of the pair ----
     const uint32_t idesc = idesc_f16(BF16, 256, p.tn, p.a_mn, p.b_mn);
-    const uint32_t a_step = p.a_mn ? 2048u : 32u, b_step = p.b_mn ? 2048u : 32u;
-    uint32_t it = 0, nt = 0;
+    const uint32_t a_step = p.a_mn ? 128u : 2u, b_step = p.b_mn ? 128u : 2u;  // 16 of k, /16 bytes
+    const uint64_t a_desc = operand_desc(p.a_mn), b_desc = operand_desc(p.b_mn);
+    RingCursor ring;
+    uint32_t nt = 0;
     bool ok = true;
     for (int t = pair; t < tiles && ok; t += pairs, ++nt) {
       const uint32_t buf = nt & 1, use = nt >> 1;
       if (use > 0 && !mbar_wait_cl(acc_empty(buf), (use - 1) & 1, kErrF16WaitAccEmpty)) break;
       tc_fence_after();
       const uint32_t d = tmem + buf * 256;
-      for (int kb = 0; kb < kblocks; ++kb, ++it) {
-        const int s = it % p.stages;
-        if (!mbar_wait_cl(full(s), (it / p.stages) & 1, kErrF16WaitFull)) {
+      uint32_t accumulate = 0;
+      for (int kb = 0; kb < kblocks; ++kb) {
+        const int s = ring.slot;
+        if (!mbar_wait_cl(full(s), ring.parity, kErrF16WaitFull)) {
           ok = false;
           break;
         }
         tc_fence_after();
-        const uint32_t a = smem + s * stage_bytes, b = a + kF16ABytes;
+        const uint32_t a = desc_addr(smem + s * stage_bytes);
+        uint64_t ad = a_desc + a, bd = b_desc + (a + (kF16ABytes >> 4));
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const uint64_t ad = p.a_mn ? smem_desc_sw128_mn(a + j * a_step)
-                                     : smem_desc_sw128(a + j * a_step);
-          const uint64_t bd = p.b_mn ? smem_desc_sw128_mn(b + j * b_step)
-                                     : smem_desc_sw128(b + j * b_step);
-          mma_f16_ss_pair(d, ad, bd, idesc, (kb | j) != 0);
+          mma_f16_ss_pair(d, ad, bd, idesc, accumulate);
+          accumulate = 1;
+          ad += a_step, bd += b_step;
         }
         mma_commit_both(empty(s));
+        ring.step(p.stages);
       }
       if (ok) mma_commit_both(acc_full(buf));
     }

@@ -77,6 +77,10 @@ def _on(device: torch.device):
     return torch.cuda.device(device)
 
 
+def _stream(t: torch.Tensor) -> int:
+    return torch._C._cuda_getCurrentRawStream(t.device.index)
+
+
 # ---- operands ----
 
 def _up(v: int, to: int) -> int:
@@ -115,7 +119,7 @@ class _Operand:
                 return
         self.t = _rows_buffer(rows, cols, t)
         self.ptr, self.ld, self.mn = self.t.data_ptr(), self.t.stride(0), 0
-        N.call("dsv4_b200_pack_rows", ptr, s0, s1, rows, cols, self.ptr, self.ld, N.stream_of(t))
+        N.call("dsv4_b200_pack_rows", ptr, s0, s1, rows, cols, self.ptr, self.ld, _stream(t))
 
 
 def _plain_rows(t: torch.Tensor) -> torch.Tensor:
@@ -136,7 +140,7 @@ def _gemm(a: _Operand, a_mn: int, b: _Operand, b_mn: int, m: int, n: int, k: int
            N.ptr(bias), ACTIVATIONS[activation], N.ptr(residual),
            0 if residual is None else _row_stride(residual), out.data_ptr(), _row_stride(out),
            N.ptr(z), 0 if z is None else z.stride(0), N.ptr(codes), N.ptr(scales),
-           N.stream_of(out))
+           _stream(out))
 
 
 # ---- 8-bit checkpoints ----
@@ -178,7 +182,7 @@ def checkpoint_int8(x: torch.Tensor) -> Int8Checkpoint:
     with _on(x.device):
         codes, scales = _empty_codes(m, k, x.device)
         N.call("dsv4_b200_checkpoint_int8", x.data_ptr(), _CHECKPOINT_DTYPES[x.dtype], m, k,
-               _row_stride(x), codes.data_ptr(), scales.data_ptr(), N.stream_of(x))
+               _row_stride(x), codes.data_ptr(), scales.data_ptr(), _stream(x))
     return Int8Checkpoint(codes, scales, (m, k), x.dtype)
 
 
@@ -202,7 +206,7 @@ def restore_int8(checkpoint: Int8Checkpoint, dtype: Optional[torch.dtype] = None
 
 def _restore(codes, scales, m, k, out):
     N.call("dsv4_b200_restore_int8", codes.data_ptr(), scales.data_ptr(), m, k, out.data_ptr(),
-           _CHECKPOINT_DTYPES[out.dtype], _row_stride(out), N.stream_of(out))
+           _CHECKPOINT_DTYPES[out.dtype], _row_stride(out), _stream(out))
     return out
 
 
@@ -331,7 +335,7 @@ def dense_backward(grad_out, saved: SavedDense, *, need_x=True, need_weight=True
                    0 if z is None else z.stride(0), N.ptr(codes), N.ptr(scales), m, n, _DTYPES[dt],
                    ACTIVATIONS[act], None if act is None else dz.data_ptr(),
                    n if act is None else dz.stride(0), N.ptr(partial), slabs, N.ptr(gb),
-                   N.stream_of(dy))
+                   _stream(dy))
             if act is None:
                 dz = dy
         if need_x or need_weight:
@@ -485,7 +489,7 @@ def _ffn(x, w13, w2, activation, clamp_limit, residual, checkpoint, keep_x, keep
             N.call("dsv4_b200_gated_gemm", a.ptr, a.ld, a.mn, b.ptr, b.ld, b.mn, m, inter, hidden,
                    _DTYPES[x.dtype], ACTIVATIONS[activation], *_limit_args(clamp_limit),
                    h.data_ptr(), h.stride(0), N.ptr(z),
-                   0 if z is None else z.stride(0), N.ptr(codes), N.ptr(scales), N.stream_of(x))
+                   0 if z is None else z.stride(0), N.ptr(codes), N.ptr(scales), _stream(x))
             a, b = _Operand(h), _Operand(w2)
             _gemm(a, a.mn, b, b.mn, m, n, inter, x.dtype, out,
                   residual=None if residual is None else _plain_rows(residual))
@@ -546,7 +550,7 @@ def gated_feed_forward_backward(grad_out, saved: SavedFeedForward, *, need_x=Tru
                    *_limit_args(saved.clamp_limit), N.ptr(z), 0 if z is None else z.stride(0),
                    N.ptr(codes), N.ptr(scales), dz.data_ptr(), dz.stride(0),
                    h.data_ptr() if form_h else None, h.stride(0) if form_h else 0,
-                   N.stream_of(grad_out))
+                   _stream(grad_out))
         if need_w2:
             ho = _Operand(h)
             _gemm(dy, 1 - dy.mn, ho, 1 - ho.mn, n, inter, m, dt, g2)
