@@ -32,9 +32,9 @@ F16Mat mat16(const void* p, int64_t ld) {
 int64_t round_up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
 
 // 2-D operand of `rows` x `k` 16-bit elements, 128-byte swizzled boxes: K-major
-// {64 of k, box_rows}, MN-major {64 rows, 64 of k}.
+// {64 of k, box_rows}, MN-major {64 rows, box_k of k}.
 int encode_operand(CUtensorMap* map, const char* what, const void* p, int64_t rows, int64_t k,
-                   int64_t ld, int mn, int box_rows, bool bf16) {
+                   int64_t ld, int mn, int box_rows, bool bf16, int box_k = 64) {
   if (tensor_map_encoder() == nullptr) return fail(DSV4_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
   const int64_t inner = mn ? rows : k, outer = mn ? k : rows;
   DSV4_REQUIRE(aligned16(p) && ld % 8 == 0 && ld >= inner,
@@ -42,12 +42,36 @@ int encode_operand(CUtensorMap* map, const char* what, const void* p, int64_t ro
                "8 elements (row stride %lld, row %lld)", what, (long long)ld, (long long)inner);
   cuuint64_t dims[2] = {static_cast<cuuint64_t>(inner), static_cast<cuuint64_t>(outer)};
   cuuint64_t strides[1] = {static_cast<cuuint64_t>(ld) * 2};
-  cuuint32_t box[2] = {64, static_cast<cuuint32_t>(mn ? 64 : box_rows)};
+  cuuint32_t box[2] = {64, static_cast<cuuint32_t>(mn ? box_k : box_rows)};
   cuuint32_t estr[2] = {1, 1};
   const CUresult r = tensor_map_encoder()(
       map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2,
       const_cast<void*>(p), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
       CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(DSV4_ERR_CUDA, "tensor map (%s) encode failed: %d", what, (int)r);
+  return DSV4_OK;
+}
+
+// K-major operand whose k is a whole number of 64s, as {64, rows, k / 64} (or,
+// for gate and up, {64, rows of a half, 2, k / 64}): one box holds several
+// blocks of k, each laid out as encode_operand's.
+int encode_wide(CUtensorMap* map, const char* what, const void* p, int64_t rows, int64_t k,
+                int64_t ld, int box_rows, int atoms, bool gated, bool bf16) {
+  if (tensor_map_encoder() == nullptr) return fail(DSV4_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
+  DSV4_REQUIRE(aligned16(p) && ld % 8 == 0 && ld >= k,
+               "%s must be 16-byte aligned with a row stride of at least its row and a multiple of "
+               "8 elements (row stride %lld, row %lld)", what, (long long)ld, (long long)k);
+  const cuuint64_t row = static_cast<cuuint64_t>(ld) * 2, blocks = static_cast<cuuint64_t>(k / 64);
+  const cuuint64_t half = static_cast<cuuint64_t>(rows / 2);
+  const cuuint32_t br = static_cast<cuuint32_t>(box_rows), ba = static_cast<cuuint32_t>(atoms);
+  const cuuint64_t dims3[3] = {64, static_cast<cuuint64_t>(rows), blocks}, str3[2] = {row, 128};
+  const cuuint64_t dims4[4] = {64, half, 2, blocks}, str4[3] = {row, row * half, 128};
+  const cuuint32_t box3[3] = {64, br, ba}, box4[4] = {64, br, 2, ba}, one[4] = {1, 1, 1, 1};
+  const CUresult r = tensor_map_encoder()(
+      map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, gated ? 4 : 3,
+      const_cast<void*>(p), gated ? dims4 : dims3, gated ? str4 : str3, gated ? box4 : box3, one,
+      CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
       CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return fail(DSV4_ERR_CUDA, "tensor map (%s) encode failed: %d", what, (int)r);
   return DSV4_OK;
@@ -102,36 +126,78 @@ int launch_pair_gemm(F16GemmParams& p, const void* a, int64_t lda, int a_mn, con
   return check_launch("f16_pair_gemm_kernel");
 }
 
-// Few tokens: the weight-streaming kernel.  Clusters as large as still run at
-// once (one CTA per SM) and leave every CTA two blocks of k; a deep ring then,
-// half of it where more CTAs than SMs share them.
+// Few tokens: the weight-streaming kernel.  A launch takes as long as its
+// busiest SM.  A CTA brings its share of the weights and tokens and reads its
+// part sums; an SM takes in 48 GB/s with one CTA and 56 with two (measured,
+// 4096 x 7168 and 7168 x 2048 for one token).  A larger cluster costs 0.15 us
+// each time it doubles.  Of the tile heights and cluster sizes the fastest
+// pair by that count is taken; 1 to 128 tokens, measured choices are within 8 %
+// of the best of all pairs.
+void pick_stream(const F16GemmParams& q, bool gated, F16StreamParams& p) {
+  const int sms = sm_count(), kblocks = (q.k + 63) / 64;
+  const int step = gated ? 32 : 16;
+  const int64_t token_tiles = (q.m + p.tn - 1) / p.tn;
+  double best = 0;
+  p.rows = 0;
+  for (int rows = 128; rows >= (p.w_mn ? 128 : 64); rows -= step) {
+    const int cols = gated ? rows / 2 : rows;
+    const int64_t tiles = (q.n + cols - 1) / cols * token_tiles;
+    for (int cl = 1, log2 = 0; cl <= 8 && (cl == 1 || kblocks >= 2 * cl); cl *= 2, ++log2) {
+      const int64_t ctas = tiles * cl;
+      const double kb = 1e-3 * (128.0 * (rows + p.tn) * ((kblocks + cl - 1) / cl) + 4.0 * p.tn * rows);
+      // 16 SMs' worth of slots may stay empty: clusters do not cross a GPC
+      const int64_t room = cl == 1 ? 2 * sms : 2 * (sms - 16);
+      const double waves = static_cast<double>((ctas + room - 1) / room);
+      const double us = (ctas <= sms - (cl == 1 ? 0 : 16) ? kb / 48 : waves * 2 * kb / 56) + 0.15 * log2;
+      if (p.rows == 0 || us < best) best = us, p.rows = rows, p.cluster = cl;
+    }
+  }
+}
+
 template <int EPI>
 int launch_stream_gemm(const F16GemmParams& q, const void* x, int64_t ldx, int x_mn, const void* w,
                        int64_t w_rows, int64_t ldw, int w_mn, bool bf16, cudaStream_t st) {
+  constexpr bool gated = EPI == kEpiGated;
   F16StreamParams p = {};
   p.m = q.m, p.n = q.n, p.k = q.k;
   p.tn = static_cast<int>(round_up(q.m < kStreamMaxTokens ? q.m : kStreamMaxTokens, 16));
-  p.tmem_cols = 32;
-  while (p.tmem_cols < p.tn) p.tmem_cols *= 2;
   p.w_mn = w_mn != 0, p.x_mn = x_mn != 0;
   p.up_row = q.up_row, p.act = q.act, p.limit = q.limit, p.bias = q.bias;
   p.residual = q.residual, p.out = q.out;
-  const int width = EPI == kEpiGated ? 64 : 128;
+  pick_stream(q, gated, p);
+  const int kblocks = (p.k + 63) / 64;
+  const int width = gated ? p.rows / 2 : p.rows;
   p.row_tiles = (q.n + width - 1) / width;
-  const int64_t tiles = static_cast<int64_t>(p.row_tiles) * ((q.m + p.tn - 1) / p.tn);
-  const int kblocks = (q.k + 63) / 64;
-  p.cluster = 1;
-  while (p.cluster < 8 && tiles * p.cluster * 2 <= sm_count() && kblocks >= p.cluster * 4)
-    p.cluster *= 2;
-  const int64_t ctas = tiles * p.cluster;
+  const int64_t ctas = static_cast<int64_t>(p.row_tiles) * ((q.m + p.tn - 1) / p.tn) * p.cluster;
   DSV4_REQUIRE(ctas < (1ll << 31), "product too large");
-  p.x_stage = p.x_mn ? (p.tn + 63) / 64 * 8192 : p.tn * 128;
-  const int stage = kF16ABytes + p.x_stage, fixed = 1024 + kStreamBarBytes;
-  p.stages = ((ctas <= sm_count() ? 200 * 1024 : 112 * 1024) - fixed) / stage;
+  const int x_groups = p.x_mn ? (p.tn + 63) / 64 : 1, w_groups = p.w_mn ? 2 : 1;
+  p.x_atom = p.x_mn ? 8192 : p.tn * 128;
+  p.w_atom = p.w_mn ? 8192 : p.rows * 128;
+  const int block = p.x_atom * x_groups + p.w_atom * w_groups, fixed = 1024 + kStreamBarBytes;
+  // two blocks a stage where three such stages fit
+  p.atoms = kblocks >= 2 * p.cluster && 6 * block <= kStreamSmem - fixed ? 2 : 1;
+  const int stage = p.atoms * block;
+  p.x_stage = p.x_atom * x_groups * p.atoms;
+  p.w_stage = p.w_atom * w_groups * p.atoms;
+  p.stages = (kStreamSmem - fixed) / stage;
   if (p.stages > kStreamMaxStages) p.stages = kStreamMaxStages;
-  if (int r = encode_operand(&p.map_w, "b", w, w_rows, p.k, ldw, p.w_mn, width, bf16)) return r;
-  if (int r = encode_operand(&p.map_x, "a", x, p.m, p.k, ldx, p.x_mn, p.tn, bf16)) return r;
-  const size_t smem = fixed + static_cast<size_t>(p.stages) * stage;
+  while (fixed + stream_ring_bytes(p.stages, stage, p.atoms, p.x_atom) > kStreamSmem) --p.stages;
+  p.ring_bytes = stream_ring_bytes(p.stages, stage, p.atoms, p.x_atom);
+  const bool whole = p.k % 64 == 0;
+  p.w_wide = !p.w_mn && whole, p.x_wide = !p.x_mn && whole;
+  if (p.w_wide) {
+    if (int r = encode_wide(&p.map_w, "b", w, w_rows, p.k, ldw, width, p.atoms, gated, bf16)) return r;
+  } else {
+    if (int r = encode_operand(&p.map_w, "b", w, w_rows, p.k, ldw, p.w_mn, width, bf16, 64 * p.atoms))
+      return r;
+  }
+  if (p.x_wide) {
+    if (int r = encode_wide(&p.map_x, "a", x, p.m, p.k, ldx, p.tn, p.atoms, false, bf16)) return r;
+  } else {
+    if (int r = encode_operand(&p.map_x, "a", x, p.m, p.k, ldx, p.x_mn, p.tn, bf16, 64 * p.atoms))
+      return r;
+  }
+  const size_t smem = fixed + static_cast<size_t>(p.ring_bytes);
   const dim3 grid(static_cast<unsigned>(ctas));
   const unsigned cl = static_cast<unsigned>(p.cluster);
   if (bf16) {
@@ -144,11 +210,16 @@ int launch_stream_gemm(const F16GemmParams& q, const void* x, int64_t ldx, int x
 
 template <int EPI>
 cudaError_t stream_attrs() {
-  cudaError_t e = cudaFuncSetAttribute(reinterpret_cast<void*>(&f16_stream_gemm_kernel<EPI, true>),
-                                       cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024);
-  if (e != cudaSuccess) return e;
-  return cudaFuncSetAttribute(reinterpret_cast<void*>(&f16_stream_gemm_kernel<EPI, false>),
-                              cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024);
+  void* const fns[2] = {reinterpret_cast<void*>(&f16_stream_gemm_kernel<EPI, true>),
+                        reinterpret_cast<void*>(&f16_stream_gemm_kernel<EPI, false>)};
+  for (void* fn : fns) {
+    cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, kStreamSmem);
+    if (e == cudaSuccess)
+      e = cudaFuncSetAttribute(fn, cudaFuncAttributePreferredSharedMemoryCarveout,
+                               cudaSharedmemCarveoutMaxShared);
+    if (e != cudaSuccess) return e;
+  }
+  return cudaSuccess;
 }
 
 // Up to 128 tokens whose values before the activation are not kept.

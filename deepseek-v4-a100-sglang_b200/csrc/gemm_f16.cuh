@@ -109,11 +109,10 @@ __device__ __forceinline__ void mma_commit_both(uint32_t bar) {
 
 // MN-major operand, 128-byte swizzle: 64 elements of the row axis side by side
 // (128 B), contraction steps 128 B apart.  Groups of 8 contraction steps are
-// 1024 B apart (SBO), groups of 64 rows one 8-KB box apart (LBO).
-__device__ __forceinline__ uint64_t smem_desc_sw128_mn(uint32_t saddr) {
+// 1024 B apart (SBO), groups of 64 rows one box apart (LBO).
+__device__ __forceinline__ uint64_t smem_desc_sw128_mn(uint32_t box_bytes) {
   uint64_t d = 0;
-  d |= static_cast<uint64_t>((saddr & 0x3FFFFu) >> 4);
-  d |= static_cast<uint64_t>(8192u >> 4) << 16;
+  d |= static_cast<uint64_t>(box_bytes >> 4) << 16;
   d |= static_cast<uint64_t>(1024u >> 4) << 32;
   d |= static_cast<uint64_t>(1u) << 46;
   d |= static_cast<uint64_t>(2u) << 61;
@@ -135,8 +134,8 @@ struct RingCursor {
 // offset: without the mask they would run into the LBO field.
 __device__ __forceinline__ uint32_t desc_addr(uint32_t saddr) { return (saddr & 0x3FFFFu) >> 4; }
 
-__device__ __forceinline__ uint64_t operand_desc(int mn) {
-  return mn ? smem_desc_sw128_mn(0) : smem_desc_sw128(0);
+__device__ __forceinline__ uint64_t operand_desc(int mn, uint32_t box_bytes) {
+  return mn ? smem_desc_sw128_mn(box_bytes) : smem_desc_sw128(0);
 }
 
 // kind::f16, fp32 accumulator; A and B of the same type.
@@ -383,7 +382,7 @@ __global__ void __launch_bounds__(kF16Threads, 1)
     // ---- MMA issuer of the pair ----
     const uint32_t idesc = idesc_f16(BF16, 256, p.tn, p.a_mn, p.b_mn);
     const uint32_t a_step = p.a_mn ? 128u : 2u, b_step = p.b_mn ? 128u : 2u;  // 16 of k, /16 bytes
-    const uint64_t a_desc = operand_desc(p.a_mn), b_desc = operand_desc(p.b_mn);
+    const uint64_t a_desc = operand_desc(p.a_mn, 8192), b_desc = operand_desc(p.b_mn, 8192);
     RingCursor ring;
     uint32_t nt = 0;
     bool ok = true;
