@@ -77,6 +77,26 @@ int encode_wide(CUtensorMap* map, const char* what, const void* p, int64_t rows,
   return DSV4_OK;
 }
 
+// MN-major operand with a whole number of 64s of rows, as {64, k, rows / 64}:
+// one box holds all of a CTA's rows, laid out as encode_operand's boxes.
+int encode_wide_mn(CUtensorMap* map, const char* what, const void* p, int64_t rows, int64_t k,
+                   int64_t ld, int box_rows, bool bf16) {
+  if (tensor_map_encoder() == nullptr) return fail(DSV4_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
+  DSV4_REQUIRE(aligned16(p) && ld % 8 == 0 && ld >= rows,
+               "%s must be 16-byte aligned with a row stride of at least its row and a multiple of "
+               "8 elements (row stride %lld, row %lld)", what, (long long)ld, (long long)rows);
+  const cuuint64_t dims[3] = {64, static_cast<cuuint64_t>(k), static_cast<cuuint64_t>(rows / 64)};
+  const cuuint64_t strides[2] = {static_cast<cuuint64_t>(ld) * 2, 128};
+  const cuuint32_t box[3] = {64, 64, static_cast<cuuint32_t>(box_rows / 64)}, one[3] = {1, 1, 1};
+  const CUresult r = tensor_map_encoder()(
+      map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
+      const_cast<void*>(p), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+      CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(DSV4_ERR_CUDA, "tensor map (%s) encode failed: %d", what, (int)r);
+  return DSV4_OK;
+}
+
 // Columns of a pair tile.  A wave of tiles costs its MMA cycles (2 per column
 // and 64 of k) or its operand bytes from L2, whichever is longer; the tile
 // that needs the fewest wave-cycles wins, the wider one on a tie.
@@ -111,8 +131,14 @@ int launch_pair_gemm(F16GemmParams& p, const void* a, int64_t lda, int a_mn, con
   p.tiles_n = (p.n + width - 1) / width;
   p.group_m = 8;
   DSV4_REQUIRE(static_cast<int64_t>(p.tiles_m) * p.tiles_n < (1ll << 30), "product too large");
-  if (int r = encode_operand(&p.map_a, "a", a, p.m, p.k, lda, p.a_mn, 128, bf16)) return r;
-  if (int r = encode_operand(&p.map_b, "b", b, b_rows, p.k, ldb, p.b_mn, half, bf16)) return r;
+  p.a_wide = p.a_mn && p.m % 64 == 0;
+  p.b_wide = p.b_mn && b_rows % 64 == 0 && half % 64 == 0 && p.up_row % 64 == 0;
+  if (int r = p.a_wide ? encode_wide_mn(&p.map_a, "a", a, p.m, p.k, lda, 128, bf16)
+                       : encode_operand(&p.map_a, "a", a, p.m, p.k, lda, p.a_mn, 128, bf16))
+    return r;
+  if (int r = p.b_wide ? encode_wide_mn(&p.map_b, "b", b, b_rows, p.k, ldb, half, bf16)
+                       : encode_operand(&p.map_b, "b", b, b_rows, p.k, ldb, p.b_mn, half, bf16))
+    return r;
   int64_t pairs = sm_count() / 2;
   const int64_t tiles = static_cast<int64_t>(p.tiles_m) * p.tiles_n;
   if (tiles < pairs) pairs = tiles;
@@ -340,6 +366,22 @@ int dsv4_b200_gated_gemm(const void* x, int64_t ldx, int x_mn, const void* w13, 
                                          dtype == DSV4_BF16, as_stream(stream));
   return launch_pair_gemm<kEpiGated>(p, x, ldx, x_mn, w13, 2 * intermediate, ldw, w_mn,
                                      dtype == DSV4_BF16, as_stream(stream));
+}
+
+int dsv4_b200_gated_feed_forward(const void* x, int64_t ldx, int x_mn, const void* w13, int64_t ldw13,
+                                 int w13_mn, const void* w2, int64_t ldw2, int w2_mn, int64_t m,
+                                 int64_t hidden, int64_t intermediate, int64_t out_cols, int dtype,
+                                 int activation, int has_clamp, float clamp_limit,
+                                 const void* residual, int64_t ldr, void* h, int64_t ldh, void* out,
+                                 int64_t ldo, void* z, int64_t ldz, int8_t* z_codes,
+                                 float* z_scales, void* stream) {
+  if (int r = dsv4_b200_gated_gemm(x, ldx, x_mn, w13, ldw13, w13_mn, m, intermediate, hidden, dtype,
+                                   activation, has_clamp, clamp_limit, h, ldh, z, ldz, z_codes,
+                                   z_scales, stream))
+    return r;
+  return dsv4_b200_dense_gemm(h, ldh, 0, w2, ldw2, w2_mn, m, out_cols, intermediate, dtype, nullptr,
+                              DSV4_ACT_NONE, residual, ldr, out, ldo, nullptr, 0, nullptr, nullptr,
+                              stream);
 }
 
 int dsv4_b200_gated_backward_gemm(const void* dy, int64_t lddy, int dy_mn, const void* w2,

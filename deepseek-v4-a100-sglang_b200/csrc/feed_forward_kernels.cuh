@@ -213,6 +213,13 @@ struct GroupScale {
   float scale;
 };
 
+// 1 / a to about one unit of the last place, a in [2^-100, 2^64]
+__device__ __forceinline__ float rcp_approx(float a) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(a));
+  return r;
+}
+
 __device__ __forceinline__ GroupScale group_scale(uint32_t amax_bits) {
   const float amax = __uint_as_float(amax_bits);
   if (amax_bits >= 0x7f800000u) return {0.f, 1.f, 0.f, CUDART_NAN_F};
@@ -221,7 +228,7 @@ __device__ __forceinline__ GroupScale group_scale(uint32_t amax_bits) {
   const float a = amax * shrink;
   // the scale toward zero: 127 steps never pass amax, so the largest finite
   // value stays finite
-  return {127.f * shrink, a, __frcp_rn(a), __fdiv_rz(amax, 127.f)};
+  return {127.f * shrink, a, rcp_approx(a), __fdiv_rz(amax, 127.f)};
 }
 
 // The quotient 127 v / amax.  p = 127 v is exact for 16-bit v; the first
@@ -357,6 +364,7 @@ __device__ __forceinline__ void store_piece8(void* base, int64_t at, int64_t col
 // group, 16 bytes of a 16-bit row), so a warp reads 512 contiguous bytes of a
 // row and writes 256 of codes.  Scales lie [group][row]; they pass through
 // shared memory so that a warp writes one group's 32 rows together.
+// The four lanes of a group compute one row's scale each and share it.
 // Codes rows are padded to the group with zeros.
 template <int DT>
 __global__ void __launch_bounds__(256)
@@ -376,16 +384,25 @@ __global__ void __launch_bounds__(256)
     for (int j = 0; j < 8; ++j) v[i][j] = 0.f;
     if (row < m && col < k) load_piece8<DT>(x, row * ld + col, col, k, vec, v[i]);
   }
+  uint32_t top[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    top[i] = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) top[i] = max(top[i], __float_as_uint(v[i][j]) & 0x7fffffffu);
+    top[i] = max(top[i], __shfl_xor_sync(0xffffffffu, top[i], 1));
+    top[i] = max(top[i], __shfl_xor_sync(0xffffffffu, top[i], 2));
+  }
+  const int sub = lane & 3;
+  const GroupScale own = group_scale(sub == 0 ? top[0] : sub == 1 ? top[1] : sub == 2 ? top[2] : top[3]);
+  s_scale[lane >> 2][warp + 8 * sub] = own.scale;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int64_t row = row0 + warp + 8 * i;
-    uint32_t top = 0;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(v[i][j]) & 0x7fffffffu);
-    top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-    top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-    const GroupScale g = group_scale(top);
-    if ((lane & 3) == 0) s_scale[lane >> 2][warp + 8 * i] = g.scale;
+    GroupScale g;
+    g.mul = __shfl_sync(0xffffffffu, own.mul, (lane & 28) + i);
+    g.amax = __shfl_sync(0xffffffffu, own.amax, (lane & 28) + i);
+    g.rcp = __shfl_sync(0xffffffffu, own.rcp, (lane & 28) + i);
     if (row < m && col < k32) {
       uint32_t w[2] = {0, 0};
       if (g.rcp != 0.f) {

@@ -11,8 +11,9 @@
 // One pair of CTAs (cta_group::2) computes a 256 x tn tile: each CTA stages
 // its own 128 rows of A and tn/2 rows of B, and the pair's MMA reads both
 // halves of B, so an operand byte fetched from L2 is used twice as often as by
-// single CTAs.  Roles: warp 0 TMA producer, warp 1 of the leader MMA issuer,
-// warps 4-11 epilogue.  The two 256-column accumulators in TMEM let the
+// single CTAs.  Roles: warps 0 and 3 TMA producers (A and B: one thread that
+// issued all copies took longer for a stage than the 512 cycles of its MMAs),
+// warp 1 of the leader MMA issuer, warps 4-11 epilogue.  The two 256-column accumulators in TMEM let the
 // epilogue of one tile overlap the products of the next.
 //
 // Epilogues (all arithmetic in fp32, one rounding when a value is stored):
@@ -64,6 +65,7 @@ struct F16GemmParams {
   int tn;                 // B rows of a pair tile (kEpiGated: gate and up together)
   int stages, b_stage;    // ring depth, bytes of B per stage and CTA
   int a_mn, b_mn;         // 1: the operand is MN-major
+  int a_wide, b_wide;     // MN-major in whole 64s of rows: one copy per stage
   int tiles_m, tiles_n, group_m;
   int up_row;             // kEpiGated: B row of up row 0
   int act;
@@ -85,6 +87,27 @@ __device__ __forceinline__ void tma_load_2d_pair(uint32_t dst, const CUtensorMap
       " [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
       "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(cl_bar)
       : "memory");
+}
+
+__device__ __forceinline__ void tma_load_3d_pair_plain(uint32_t dst, const CUtensorMap* map, int c0,
+                                                       int c1, int c2, uint32_t cl_bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(cl_bar)
+      : "memory");
+}
+
+// One CTA's `rows` rows of an operand at row `row`, 64 of k from `kk`.
+__device__ __forceinline__ void load_operand(uint32_t dst, const CUtensorMap* map, int mn, int wide,
+                                             int rows, int row, int kk, uint32_t cl_bar) {
+  if (!mn) {
+    tma_load_2d_pair(dst, map, kk, row, cl_bar);
+  } else if (wide) {
+    tma_load_3d_pair_plain(dst, map, 0, kk, row >> 6, cl_bar);
+  } else {
+    for (int j = 0; j < rows; j += 64) tma_load_2d_pair(dst + j * 128, map, row + j, kk, cl_bar);
+  }
 }
 
 __device__ __forceinline__ void mma_f16_ss_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc,
@@ -324,12 +347,12 @@ __global__ void __launch_bounds__(kF16Threads, 1)
     tc = r / rows;
   };
 
-  if (warp == 0 && lane == 0) {
-    // ---- TMA producer of this CTA's halves ----
+  if ((warp == 0 || warp == 3) && lane == 0) {
+    // ---- TMA producers: warp 0 this CTA's rows of A, warp 3 of B ----
+    const bool first = warp == 0;
     RingCursor ring;
     uint32_t filled = 0;  // slots in use at the end, up to the ring's depth
     bool ok = true;
-    const int b_boxes = p.b_mn ? (half_n + 63) >> 6 : 1;
     const uint32_t leader = mapa_shared(bars, 0);
     for (int t = pair; t < tiles && ok; t += pairs) {
       int tm, tc;
@@ -347,20 +370,12 @@ __global__ void __launch_bounds__(kF16Threads, 1)
         } else {
           ++filled;
         }
-        if (rank == 0) mbar_arrive_expect_tx(full(s), 2 * stage_bytes);
-        const uint32_t bar = leader + 8u * s;
-        const uint32_t a = smem + s * stage_bytes, b = a + kF16ABytes;
-        if (p.a_mn) {
-          tma_load_2d_pair(a, &p.map_a, row, kk, bar);
-          tma_load_2d_pair(a + 8192, &p.map_a, row + 64, kk, bar);
+        const uint32_t bar = leader + 8u * s, a = smem + s * stage_bytes;
+        if (first) {
+          if (rank == 0) mbar_arrive_expect_tx(full(s), 2 * stage_bytes);
+          load_operand(a, &p.map_a, p.a_mn, p.a_wide, 128, row, kk, bar);
         } else {
-          tma_load_2d_pair(a, &p.map_a, kk, row, bar);
-        }
-        if (p.b_mn) {
-          for (int j = 0; j < b_boxes; ++j)
-            tma_load_2d_pair(b + j * 8192, &p.map_b, brow + j * 64, kk, bar);
-        } else {
-          tma_load_2d_pair(b, &p.map_b, kk, brow, bar);
+          load_operand(a + kF16ABytes, &p.map_b, p.b_mn, p.b_wide, half_n, brow, kk, bar);
         }
         ring.step(p.stages);
       }

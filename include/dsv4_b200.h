@@ -425,6 +425,16 @@ DSV4_API int dsv4_b200_gated_gemm(const void* x, int64_t ldx, int x_mn, const vo
                                   int64_t ldh, void* z, int64_t ldz, int8_t* z_codes,
                                   float* z_scales, void* stream);
 
+/* The whole block, y = h w2^T + residual: dsv4_b200_gated_gemm into h, then
+ * dsv4_b200_dense_gemm (w2 [out_cols][intermediate]).  h is a workspace that
+ * the backward pass may use; ldh % 8 == 0, 16-byte aligned. */
+DSV4_API int dsv4_b200_gated_feed_forward(
+    const void* x, int64_t ldx, int x_mn, const void* w13, int64_t ldw13, int w13_mn, const void* w2,
+    int64_t ldw2, int w2_mn, int64_t m, int64_t hidden, int64_t intermediate, int64_t out_cols,
+    int dtype, int activation, int has_clamp, float clamp_limit, const void* residual, int64_t ldr,
+    void* h, int64_t ldh, void* out, int64_t ldo, void* z, int64_t ldz, int8_t* z_codes,
+    float* z_scales, void* stream);
+
 /* Backward of the gate: dh = dy w2 (w2 [k][intermediate], or with w_mn = 0 its
  * transpose) stays in registers; dz [m][2 intermediate] = the gradients of g
  * and u; h (may be NULL) is formed again from the kept z. */
