@@ -206,49 +206,60 @@ __device__ __forceinline__ void gated_backward_row(int act, float limit, const f
 constexpr int kGroup = 32;
 constexpr float kTinyGroup = 7.8886090522101181e-31f;  // 2^-100
 
-struct GroupScale {
-  float mul;    // 127, or 127 * 2^-64 where 127 v could overflow
-  float amax;   // times the same power of two
-  float rcp;    // 1 / amax, 0 for an empty or non-finite group
-  float scale;
-};
 
-// 1 / a to about one unit of the last place, a in [2^-100, 2^64]
+// 1 / a to about one unit of the last place, a in [2^-100, 2^128)
 __device__ __forceinline__ float rcp_approx(float a) {
   float r;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(a));
   return r;
 }
 
-__device__ __forceinline__ GroupScale group_scale(uint32_t amax_bits) {
+// The scale is rounded toward zero: 127 steps never pass amax, so the largest
+// finite value stays finite.
+__device__ __forceinline__ float group_step(uint32_t amax_bits) {
   const float amax = __uint_as_float(amax_bits);
-  if (amax_bits >= 0x7f800000u) return {0.f, 1.f, 0.f, CUDART_NAN_F};
-  if (amax < kTinyGroup) return {0.f, 1.f, 0.f, 0.f};
-  const float shrink = amax > 1.8446744e19f ? 5.4210109e-20f : 1.f;  // 2^64, 2^-64
-  const float a = amax * shrink;
-  // the scale toward zero: 127 steps never pass amax, so the largest finite
-  // value stays finite
-  return {127.f * shrink, a, rcp_approx(a), __fdiv_rz(amax, 127.f)};
+  if (amax_bits >= 0x7f800000u) return CUDART_NAN_F;
+  return amax < kTinyGroup ? 0.f : __fdiv_rz(amax, 127.f);
 }
 
-// The quotient 127 v / amax.  p = 127 v is exact for 16-bit v; the first
-// estimate p rcp is off by a few units of the last place, and one step with
-// the exact remainder p - q amax makes it the correctly rounded quotient: a tie
-// (k + 1/2) comes out as itself, and other quotients of 16-bit values lie at
-// least 2^-18 (relative) away from one, against 2^-24.
-__device__ __forceinline__ float group_quotient(float v, const GroupScale& g) {
-  const float p = v * g.mul, q = p * g.rcp;
-  return __fmaf_rn(__fmaf_rn(-q, g.amax, p), g.rcp, q);
+// 127 / amax to about 2^-22; 0 for a group that holds zeros or decodes to NaN
+__device__ __forceinline__ float group_inverse(uint32_t amax_bits) {
+  const float amax = __uint_as_float(amax_bits);
+  if (amax_bits >= 0x7f800000u || amax < kTinyGroup) return 0.f;
+  return amax > 1.8446744e19f ? (127.f * 5.4210109e-20f) * rcp_approx(amax * 5.4210109e-20f)
+                              : 127.f * rcp_approx(amax);  // 2^64, 2^-64
+}
+
+// Correctly rounded 127 v / amax for 16-bit v: p = 127 v is exact, the first
+// estimate is off by a few units of the last place, and one step with the
+// exact remainder p - q amax mends that.  A tie (k + 1/2) comes out as itself.
+__device__ __forceinline__ float group_quotient(float v, float amax) {
+  const float shrink = amax > 1.8446744e19f ? 5.4210109e-20f : 1.f;
+  const float a = amax * shrink, r = rcp_approx(a), p = v * (127.f * shrink), q = p * r;
+  return __fmaf_rn(__fmaf_rn(-q, a, p), r, q);
+}
+
+// 16-bit values.  A tie 254 v = (2k + 1) amax needs k = 63 unless amax's
+// significand is a multiple of 127: then |v| = amax / 2 and the code is 64, the
+// even neighbour, away from zero.  No other quotient of 16-bit values lies
+// within 2^-19 (relative) of a half.  So v * inverse * (1 + 2^-21), off by at
+// most 2^-22 more, rounds every value of such a group as the exact quotient.
+// Groups with the special significand (1 in 128) take the exact one.
+constexpr float kTieBias = 1.f + 1.f / 2097152.f;
+
+__device__ __forceinline__ bool group_special(uint32_t amax_bits) {
+  return (((amax_bits >> 13) & 0x3ffu) + 1024u) % 127u == 0;
 }
 
 // fp32 values: within 6e-5 of a half the sign of 127 v - (f + 1/2) amax
 // decides, taken exactly (both products as rounded part + remainder).
-__device__ __noinline__ int quantize_code_near(float v, float q, const GroupScale& g) {
+__device__ __noinline__ int quantize_code_near(float v, float q, float amax) {
   const float f = floorf(fabsf(q));
   if (fabsf(fabsf(q) - f - 0.5f) >= 6e-5f) return __float2int_rn(q);
-  const float x = fabsf(v) * (g.mul > 1.f ? 1.f : 5.4210109e-20f), c = f + 0.5f;
+  const float shrink = amax > 1.8446744e19f ? 5.4210109e-20f : 1.f;
+  const float x = fabsf(v) * shrink, a = amax * shrink, c = f + 0.5f;
   const float p = 127.f * x, pl = __fmaf_rn(127.f, x, -p);
-  const float t = c * g.amax, tl = __fmaf_rn(c, g.amax, -t);
+  const float t = c * a, tl = __fmaf_rn(c, a, -t);
   const float d = (p - t) + (pl - tl);
   const int fi = static_cast<int>(f);
   const int r = d > 0.f ? fi + 1 : d < 0.f ? fi : fi + (fi & 1);
@@ -264,43 +275,40 @@ __device__ __forceinline__ uint32_t pack_codes(float a, float b, float c, float 
   return prmt(lo, hi, 0x5410u);
 }
 
-// 4 codes; EXACT32 for values with all of fp32's digits
-template <bool EXACT32>
-__device__ __forceinline__ uint32_t quantize4(float a, float b, float c, float d,
-                                              const GroupScale& g) {
-  const float q[4] = {group_quotient(a, g), group_quotient(b, g), group_quotient(c, g),
-                      group_quotient(d, g)};
-  if constexpr (EXACT32) {
-    const float v[4] = {a, b, c, d};
-    float near = 0.f;
+// 4 codes of fp32 values
+__device__ __forceinline__ uint32_t quantize4_f32(const float (&v)[4], float inverse, float amax) {
+  float q[4], near = 0.f;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) near = fmaxf(near, fabsf(q[i] - rintf(q[i])));
-    if (near > 0.4999f) {
-      uint32_t w = 0;
+  for (int i = 0; i < 4; ++i) {
+    q[i] = v[i] * inverse;
+    near = fmaxf(near, fabsf(q[i] - rintf(q[i])));
+  }
+  if (near > 0.4999f) {
+    uint32_t w = 0;
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        w |= (static_cast<uint32_t>(quantize_code_near(v[i], q[i], g)) & 0xffu) << (8 * i);
-      return w;
-    }
+    for (int i = 0; i < 4; ++i)
+      w |= (static_cast<uint32_t>(quantize_code_near(v[i], q[i], amax)) & 0xffu) << (8 * i);
+    return w;
   }
   return pack_codes(q[0], q[1], q[2], q[3]);
 }
 
-// A thread's own group of fp32 sums: codes (4 per word) and the scale.
+// A thread's own group of fp32 sums: codes (4 per word) and the scale.  (A sum
+// next to the border of two codes is itself only known to its last bits.)
 __device__ __forceinline__ float quantize_group(const float (&v)[32], uint32_t (&codes)[8]) {
   uint32_t top = 0;
 #pragma unroll
   for (int j = 0; j < 32; ++j) top = max(top, __float_as_uint(v[j]) & 0x7fffffffu);
-  const GroupScale g = group_scale(top);
-  if (g.rcp == 0.f) {
+  const float inv = group_inverse(top);
+  if (inv == 0.f) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) codes[j] = 0;
-    return g.scale;
-  }
+  } else {
 #pragma unroll
-  for (int j = 0; j < 8; ++j)
-    codes[j] = quantize4<false>(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3], g);
-  return g.scale;
+    for (int j = 0; j < 8; ++j)
+      codes[j] = pack_codes(v[4 * j] * inv, v[4 * j + 1] * inv, v[4 * j + 2] * inv, v[4 * j + 3] * inv);
+  }
+  return group_step(top);
 }
 
 // 8 consecutive values of a 16- or 32-bit row; pieces past `cols` read as 0.
@@ -362,60 +370,121 @@ __device__ __forceinline__ void store_piece8(void* base, int64_t at, int64_t col
 // ---- activation checkpoint: rows -> 8-bit groups ----
 // A block takes 32 rows x 256 columns.  A lane owns 8 columns (a quarter of a
 // group, 16 bytes of a 16-bit row), so a warp reads 512 contiguous bytes of a
-// row and writes 256 of codes.  Scales lie [group][row]; they pass through
-// shared memory so that a warp writes one group's 32 rows together.
-// The four lanes of a group compute one row's scale each and share it.
-// Codes rows are padded to the group with zeros.
+// row and writes 256 of codes; it keeps its four rows' loads in flight
+// together.  The four lanes of a group work out one row's scale each and share
+// it.  Scales lie [group][row]; they pass through shared memory so that a warp
+// writes one group's 32 rows together.  Codes rows are padded to the group
+// with zeros.  Bound by issue slots next to memory: 16-bit rows stay packed
+// through the maximum (two values an instruction) and a code costs one product
+// and one addition.
 template <int DT>
 __global__ void __launch_bounds__(256)
     checkpoint_kernel(const void* __restrict__ x, int64_t ld, int vec, int64_t m, int64_t k,
                       int64_t k32, int64_t col_blocks, int8_t* __restrict__ codes,
                       float* __restrict__ scales) {
   pdl_entry();
+  constexpr bool F32 = DT == DSV4_F32;
+  constexpr int kWords = F32 ? 8 : 4;
   __shared__ float s_scale[8][33];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t row0 = (blockIdx.x / col_blocks) * 32;
+  const int64_t row0 = (blockIdx.x / col_blocks) * 32 + warp;
   const int64_t col = (blockIdx.x % col_blocks) * 256 + lane * 8;
-  float v[4][8];
+  const uint32_t* const p =
+      reinterpret_cast<const uint32_t*>(static_cast<const uint8_t*>(x) + (row0 * ld + col) * (F32 ? 4 : 2));
+  const int64_t step = 8 * ld * (F32 ? 4 : 2);
+  uint32_t raw[4][kWords];
+  if (vec && col + 8 <= k) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int64_t row = row0 + warp + 8 * i;
+    for (int i = 0; i < 4; ++i) {
+      const uint8_t* q = reinterpret_cast<const uint8_t*>(p) + i * step;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[i][j] = 0.f;
-    if (row < m && col < k) load_piece8<DT>(x, row * ld + col, col, k, vec, v[i]);
+      for (int h = 0; h < kWords; h += 4) {
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if (row0 + 8 * i < m) v = *reinterpret_cast<const uint4*>(q + 4 * h);
+        raw[i][h] = v.x, raw[i][h + 1] = v.y, raw[i][h + 2] = v.z, raw[i][h + 3] = v.w;
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint8_t* q = reinterpret_cast<const uint8_t*>(p) + i * step;
+#pragma unroll
+      for (int j = 0; j < kWords; ++j) raw[i][j] = 0;
+      if (row0 + 8 * i >= m) continue;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        if (col + j >= k) continue;
+        if constexpr (F32) {
+          raw[i][j] = reinterpret_cast<const uint32_t*>(q)[j];
+        } else {
+          raw[i][j >> 1] |= static_cast<uint32_t>(reinterpret_cast<const uint16_t*>(q)[j]) << (16 * (j & 1));
+        }
+      }
+    }
   }
+  // the bits of |largest value|: as whole numbers they order like the values,
+  // infinities and NaN above all
   uint32_t top[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    top[i] = 0;
+    if constexpr (F32) {
+      uint32_t t = 0;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) top[i] = max(top[i], __float_as_uint(v[i][j]) & 0x7fffffffu);
-    top[i] = max(top[i], __shfl_xor_sync(0xffffffffu, top[i], 1));
-    top[i] = max(top[i], __shfl_xor_sync(0xffffffffu, top[i], 2));
-  }
-  const int sub = lane & 3;
-  const GroupScale own = group_scale(sub == 0 ? top[0] : sub == 1 ? top[1] : sub == 2 ? top[2] : top[3]);
-  s_scale[lane >> 2][warp + 8 * sub] = own.scale;
+      for (int j = 0; j < 8; ++j) t = max(t, raw[i][j] & 0x7fffffffu);
+      t = max(t, __shfl_xor_sync(0xffffffffu, t, 1));
+      top[i] = max(t, __shfl_xor_sync(0xffffffffu, t, 2));
+    } else {
+      uint32_t t = raw[i][0] & 0x7fff7fffu;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int64_t row = row0 + warp + 8 * i;
-    GroupScale g;
-    g.mul = __shfl_sync(0xffffffffu, own.mul, (lane & 28) + i);
-    g.amax = __shfl_sync(0xffffffffu, own.amax, (lane & 28) + i);
-    g.rcp = __shfl_sync(0xffffffffu, own.rcp, (lane & 28) + i);
-    if (row < m && col < k32) {
-      uint32_t w[2] = {0, 0};
-      if (g.rcp != 0.f) {
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-          w[j] = quantize4<DT == DSV4_F32>(v[i][4 * j], v[i][4 * j + 1], v[i][4 * j + 2],
-                                           v[i][4 * j + 3], g);
-      }
-      *reinterpret_cast<uint2*>(codes + row * k32 + col) = make_uint2(w[0], w[1]);
+      for (int j = 1; j < 4; ++j) t = __vmaxu2(t, raw[i][j] & 0x7fff7fffu);
+      t = __vmaxu2(t, __shfl_xor_sync(0xffffffffu, t, 1));
+      t = __vmaxu2(t, __shfl_xor_sync(0xffffffffu, t, 2));
+      t = max(t & 0xffffu, t >> 16);
+      top[i] = __float_as_uint(unpack_16<DT == DSV4_BF16>(t, 0));
     }
   }
+  const int sub = lane & 3;
+  const uint32_t mine = sub == 0 ? top[0] : sub == 1 ? top[1] : sub == 2 ? top[2] : top[3];
+  s_scale[lane >> 2][warp + 8 * sub] = group_step(mine);
+  float own = group_inverse(mine);
+  if (!F32) own = group_special(mine) ? -own : own * kTieBias;
+  int8_t* const c = codes + row0 * k32 + col;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float inv = __shfl_sync(0xffffffffu, own, (lane & 28) + i);
+    uint32_t w[2] = {0, 0};
+    if constexpr (F32) {
+      if (inv != 0.f) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          float v[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) v[j] = __uint_as_float(raw[i][4 * h + j]);
+          w[h] = quantize4_f32(v, inv, __uint_as_float(top[i]));
+        }
+      }
+    } else {
+      float q[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) q[j] = unpack_16<DT == DSV4_BF16>(raw[i][j >> 1], j & 1);
+      if (inv > 0.f) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) q[j] *= inv;
+      } else if (inv < 0.f) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) q[j] = group_quotient(q[j], __uint_as_float(top[i]));
+      } else {  // zeros, or a group that holds an infinity or a NaN
+#pragma unroll
+        for (int j = 0; j < 8; ++j) q[j] = 0.f;
+      }
+      w[0] = pack_codes(q[0], q[1], q[2], q[3]);
+      w[1] = pack_codes(q[4], q[5], q[6], q[7]);
+    }
+    if (row0 + 8 * i < m && col < k32)
+      *reinterpret_cast<uint2*>(c + i * 8 * k32) = make_uint2(w[0], w[1]);
+  }
   __syncthreads();
-  const int64_t group = (blockIdx.x % col_blocks) * 8 + warp, row = row0 + lane;
+  const int64_t group = (blockIdx.x % col_blocks) * 8 + warp, row = row0 - warp + lane;
   if (group * kGroup < k32 && row < m) scales[group * m + row] = s_scale[warp][lane];
 }
 

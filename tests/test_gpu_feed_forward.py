@@ -175,3 +175,24 @@ def test_checkpoint_near_ties_in_fp32():
     x = torch.stack(rows)
     q = 127 * x.double() / x.double().abs().amax(1, keepdim=True)
     assert torch.equal(D.checkpoint_int8(x).codes.double(), torch.round(q))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_checkpoint_codes_of_every_pair(dtype):
+    """The code of every value below every largest value of one binade (all
+    16-bit significands): exactly the rounded exact quotient, ties to even."""
+    import dsv4_b200 as D
+    bits = 7 if dtype == BF16 else 10
+    top = (1 + torch.arange(2 ** bits, device="cuda").double() / 2 ** bits)
+    for scale in (1.0, 2.0 ** -6, 2.0 ** 9):
+        part = torch.cat([top * 2.0 ** -e for e in range(1, 8)]) if bits == 7 else \
+            torch.cat([top * 2.0 ** -e for e in (1, 2, 3)])
+        sign = torch.where(torch.arange(part.numel(), device="cuda") % 2 == 0, 1.0, -1.0)
+        cols = -(-part.numel() // 31) * 31
+        part = torch.nn.functional.pad(part * sign, (0, cols - part.numel())).reshape(-1, 31)
+        x = torch.cat((top[:, None, None].expand(-1, part.shape[0], 1),
+                       part[None].expand(top.numel(), -1, -1)), 2).reshape(top.numel(), -1) * scale
+        assert torch.equal(x.to(dtype).double(), x)
+        g = x.reshape(x.shape[0], -1, 32)
+        want = torch.round(127 * g / g.abs().amax(2, keepdim=True)).reshape(x.shape)
+        assert torch.equal(D.checkpoint_int8(x.to(dtype)).codes.double(), want)
