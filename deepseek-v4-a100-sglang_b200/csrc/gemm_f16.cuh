@@ -161,6 +161,19 @@ __device__ __forceinline__ uint64_t operand_desc(int mn, uint32_t box_bytes) {
   return mn ? smem_desc_sw128_mn(box_bytes) : smem_desc_sw128(0);
 }
 
+// One lane of a warp that runs together.  The issuing roles run as whole warps
+// and elect the lane only where an instruction is issued: descriptors, slots
+// and counters then live in uniform registers.  (As a branch of lane 0 an MMA
+// cost its issuer 71 cycles and a stage of four 587, more than the 512 of the
+// tensor cores.)
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile(
+      "{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(p));
+  return p != 0;
+}
+
 // kind::f16, fp32 accumulator; A and B of the same type.
 __device__ __forceinline__ uint32_t idesc_f16(bool bf16, uint32_t m, uint32_t n, uint32_t a_mn,
                                               uint32_t b_mn) {
@@ -297,7 +310,7 @@ __global__ void __launch_bounds__(kF16Threads, 1)
     f16_pair_gemm_kernel(const __grid_constant__ F16GemmParams p) {
   extern __shared__ uint8_t smem_raw[];
   const uint32_t smem = (smem_u32(smem_raw) + 1023u) & ~1023u;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const uint32_t rank = cluster_ctarank();
   const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
   const int stage_bytes = kF16ABytes + p.b_stage;
@@ -347,7 +360,7 @@ __global__ void __launch_bounds__(kF16Threads, 1)
     tc = r / rows;
   };
 
-  if ((warp == 0 || warp == 3) && lane == 0) {
+  if (warp == 0 || warp == 3) {
     // ---- TMA producers: warp 0 this CTA's rows of A, warp 3 of B ----
     const bool first = warp == 0;
     RingCursor ring;
@@ -371,11 +384,13 @@ __global__ void __launch_bounds__(kF16Threads, 1)
           ++filled;
         }
         const uint32_t bar = leader + 8u * s, a = smem + s * stage_bytes;
-        if (first) {
-          if (rank == 0) mbar_arrive_expect_tx(full(s), 2 * stage_bytes);
-          load_operand(a, &p.map_a, p.a_mn, p.a_wide, 128, row, kk, bar);
-        } else {
-          load_operand(a + kF16ABytes, &p.map_b, p.b_mn, p.b_wide, half_n, brow, kk, bar);
+        if (elect_one()) {
+          if (first) {
+            if (rank == 0) mbar_arrive_expect_tx(full(s), 2 * stage_bytes);
+            load_operand(a, &p.map_a, p.a_mn, p.a_wide, 128, row, kk, bar);
+          } else {
+            load_operand(a + kF16ABytes, &p.map_b, p.b_mn, p.b_wide, half_n, brow, kk, bar);
+          }
         }
         ring.step(p.stages);
       }
@@ -393,7 +408,7 @@ __global__ void __launch_bounds__(kF16Threads, 1)
       while (globaltimer_ns() - t0 < 1000000ull) {
       }
     }
-  } else if (warp == 1 && rank == 0 && lane == 0) {
+  } else if (warp == 1 && rank == 0) {
     // ---- MMA issuer of the pair ----
     const uint32_t idesc = idesc_f16(BF16, 256, p.tn, p.a_mn, p.b_mn);
     const uint32_t a_step = p.a_mn ? 128u : 2u, b_step = p.b_mn ? 128u : 2u;  // 16 of k, /16 bytes
@@ -406,7 +421,6 @@ __global__ void __launch_bounds__(kF16Threads, 1)
       if (use > 0 && !mbar_wait_cl(acc_empty(buf), (use - 1) & 1, kErrF16WaitAccEmpty)) break;
       tc_fence_after();
       const uint32_t d = tmem + buf * 256;
-      uint32_t accumulate = 0;
       for (int kb = 0; kb < kblocks; ++kb) {
         const int s = ring.slot;
         if (!mbar_wait_cl(full(s), ring.parity, kErrF16WaitFull)) {
@@ -415,17 +429,16 @@ __global__ void __launch_bounds__(kF16Threads, 1)
         }
         tc_fence_after();
         const uint32_t a = desc_addr(smem + s * stage_bytes);
-        uint64_t ad = a_desc + a, bd = b_desc + (a + (kF16ABytes >> 4));
+        const uint64_t ad = a_desc + a, bd = b_desc + (a + (kF16ABytes >> 4));
+        if (elect_one()) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          mma_f16_ss_pair(d, ad, bd, idesc, accumulate);
-          accumulate = 1;
-          ad += a_step, bd += b_step;
+          for (int j = 0; j < 4; ++j)
+            mma_f16_ss_pair(d, ad + j * a_step, bd + j * b_step, idesc, (kb | j) != 0);
+          mma_commit_both(empty(s));
         }
-        mma_commit_both(empty(s));
         ring.step(p.stages);
       }
-      if (ok) mma_commit_both(acc_full(buf));
+      if (ok && elect_one()) mma_commit_both(acc_full(buf));
     }
   } else if (warp >= 4) {
     // ---- epilogue: warp w reads TMEM lanes 32 (w & 3).., every second chunk ----

@@ -181,7 +181,7 @@ __global__ void __launch_bounds__(kStreamThreads)
     f16_stream_gemm_kernel(const __grid_constant__ F16StreamParams p) {
   extern __shared__ uint8_t smem_raw[];
   const uint32_t smem = (smem_u32(smem_raw) + 1023u) & ~1023u;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int rank = static_cast<int>(cluster_ctarank());
   const int tile = blockIdx.x / p.cluster;
   const int row_tile = tile % p.row_tiles, token0 = tile / p.row_tiles * p.tn;
@@ -229,7 +229,7 @@ __global__ void __launch_bounds__(kStreamThreads)
   const uint32_t tmem = ld_shared_u32(tmem_slot);
   pdl_entry();
 
-  if (warp == 0 && lane == 0) {
+  if (warp == 0) {
     RingCursor ring;
     bool ok = true;
     for (int i = 0; i < nkb; ++i) {
@@ -240,26 +240,26 @@ __global__ void __launch_bounds__(kStreamThreads)
       }
       ring.step(p.stages);
       const uint32_t x = smem + s * stage_bytes;
-      mbar_arrive_expect_tx(full(s), stage_bytes);
-      load_stage<EPI>(p, x, x + p.x_stage, full(s), token0, col0, (kb0 + i) * kspan);
+      if (elect_one()) {
+        mbar_arrive_expect_tx(full(s), stage_bytes);
+        load_stage<EPI>(p, x, x + p.x_stage, full(s), token0, col0, (kb0 + i) * kspan);
+      }
     }
     if (!ok) {  // copies in flight land before shared memory is used again
       const unsigned long long t0 = globaltimer_ns();
       while (globaltimer_ns() - t0 < 1000000ull) {
       }
     }
-  } else if (warp == 1 && lane == 0) {
+  } else if (warp == 1) {
     // M = 128 whatever the tokens: the rows behind them are other bytes of the
     // ring, and only fill lanes that nobody reads
     const uint32_t idesc = idesc_f16(BF16, 128, p.rows, p.x_mn, p.w_mn);
     const uint32_t w_step = p.w_mn ? 128u : 2u, x_step = p.x_mn ? 128u : 2u;
     const uint64_t w_desc = operand_desc(p.w_mn, p.w_atom * p.atoms);
     const uint64_t x_desc = operand_desc(p.x_mn, p.x_atom * p.atoms);
-    // from the last 16 of a block to the next block (MN-major: k just goes on)
-    const uint32_t w_next = p.w_mn ? 128u : (p.w_atom >> 4) - 6u;
-    const uint32_t x_next = p.x_mn ? 128u : (p.x_atom >> 4) - 6u;
+    // from one block to the next (MN-major: k just goes on)
+    const uint32_t w_next = p.w_mn ? 512u : p.w_atom >> 4, x_next = p.x_mn ? 512u : p.x_atom >> 4;
     RingCursor ring;
-    uint32_t accumulate = 0;
     bool ok = true;
     for (int i = 0; i < nkb; ++i) {
       const int s = ring.slot;
@@ -270,19 +270,18 @@ __global__ void __launch_bounds__(kStreamThreads)
       tc_fence_after();
       const uint32_t at = smem + s * stage_bytes;
       uint64_t xd = x_desc + desc_addr(at), wd = w_desc + desc_addr(at + p.x_stage);
-      for (int a = 0; a < p.atoms; ++a) {
+      if (elect_one()) {
+        for (int a = 0; a < p.atoms; ++a) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          mma_f16_ss(tmem, xd, wd, idesc, accumulate);
-          accumulate = 1;
-          wd += j < 3 ? w_step : w_next;
-          xd += j < 3 ? x_step : x_next;
+          for (int j = 0; j < 4; ++j)
+            mma_f16_ss(tmem, xd + j * x_step, wd + j * w_step, idesc, (i | a | j) != 0);
+          wd += w_next, xd += x_next;
         }
+        mma_commit(empty(s));
       }
-      mma_commit(empty(s));
       ring.step(p.stages);
     }
-    if (ok) mma_commit(acc_full);
+    if (ok && elect_one()) mma_commit(acc_full);
   }
   __syncwarp();
 
