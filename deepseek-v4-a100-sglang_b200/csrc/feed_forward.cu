@@ -152,30 +152,66 @@ int launch_pair_gemm(F16GemmParams& p, const void* a, int64_t lda, int a_mn, con
   return check_launch("f16_pair_gemm_kernel");
 }
 
+// Clusters that run at once, by [two CTAs per SM][log2 of the cluster size]
+// (a cluster does not cross a GPC, so this is less than SMs / size).
+constexpr int kMaxDevices = 64;
+int g_stream_room[kMaxDevices][2][4];
+
+int stream_room(bool two, int log2) {
+  int dev = 0;
+  cudaGetDevice(&dev);
+  return dev >= 0 && dev < kMaxDevices ? g_stream_room[dev][two][log2] : 1;
+}
+
+cudaError_t query_stream_room() {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess || dev < 0 || dev >= kMaxDevices) return e;
+  for (int two = 0; two < 2; ++two)
+    for (int log2 = 0; log2 < 4; ++log2) {
+      cudaLaunchConfig_t cfg = {};
+      cfg.gridDim = dim3(1024);
+      cfg.blockDim = dim3(kStreamThreads);
+      cfg.dynamicSmemBytes = two ? kStreamSmem : kStreamSmemAlone;
+      cudaLaunchAttribute attr[1];
+      attr[0].id = cudaLaunchAttributeClusterDimension;
+      attr[0].val.clusterDim.x = 1u << log2;
+      attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+      cfg.attrs = attr;
+      cfg.numAttrs = 1;
+      int n = 0;
+      e = cudaOccupancyMaxActiveClusters(&n, &f16_stream_gemm_kernel<kEpiLinear, true>, &cfg);
+      if (e != cudaSuccess) return e;
+      g_stream_room[dev][two][log2] = n > 0 ? n : 1;
+    }
+  return cudaSuccess;
+}
+
 // Few tokens: the weight-streaming kernel.  A launch takes as long as its
-// busiest SM.  A CTA brings its share of the weights and tokens and reads its
-// part sums; an SM takes in 48 GB/s with one CTA and 56 with two (measured,
-// 4096 x 7168 and 7168 x 2048 for one token).  A larger cluster costs 0.15 us
-// each time it doubles.  Of the tile heights and cluster sizes the fastest
-// pair by that count is taken; 1 to 128 tokens, measured choices are within 8 %
-// of the best of all pairs.
-void pick_stream(const F16GemmParams& q, bool gated, F16StreamParams& p) {
-  const int sms = sm_count(), kblocks = (q.k + 63) / 64;
-  const int step = gated ? 32 : 16;
+// busiest SM, whose work is counted in weight rows x blocks of k: a block of a
+// CTA costs its weight rows and, from L2, a third as much for its tokens; the
+// part sums of a tile count as tokens x rows / 32.  One CTA per SM with all of
+// the shared memory is 8 % slower than the same work in two halves; two need
+// at least 8 blocks each.  Doubling the cluster costs 2 %.  The least of all
+// tile heights and cluster sizes is taken.  (Fitted to 6 shapes, 512 x 1024 to
+// 14336 x 1024 and 4096 x 7168, at 1 to 128 tokens: the choice is on average
+// 2 %, at most 10 % slower than the best of all measured.)
+void pick_stream(const F16GemmParams& q, bool gated, F16StreamParams& p, bool* two_per_sm) {
+  const int kblocks = (q.k + 63) / 64, step = gated ? 32 : 16;
   const int64_t token_tiles = (q.m + p.tn - 1) / p.tn;
   double best = 0;
   p.rows = 0;
   for (int rows = 128; rows >= (p.w_mn ? 128 : 64); rows -= step) {
     const int cols = gated ? rows / 2 : rows;
     const int64_t tiles = (q.n + cols - 1) / cols * token_tiles;
-    for (int cl = 1, log2 = 0; cl <= 8 && (cl == 1 || kblocks >= 2 * cl); cl *= 2, ++log2) {
-      const int64_t ctas = tiles * cl;
-      const double kb = 1e-3 * (128.0 * (rows + p.tn) * ((kblocks + cl - 1) / cl) + 4.0 * p.tn * rows);
-      // 16 SMs' worth of slots may stay empty: clusters do not cross a GPC
-      const int64_t room = cl == 1 ? 2 * sms : 2 * (sms - 16);
-      const double waves = static_cast<double>((ctas + room - 1) / room);
-      const double us = (ctas <= sms - (cl == 1 ? 0 : 16) ? kb / 48 : waves * 2 * kb / 56) + 0.15 * log2;
-      if (p.rows == 0 || us < best) best = us, p.rows = rows, p.cluster = cl;
+    for (int log2 = 0; log2 < 4 && (log2 == 0 || kblocks >= 2 << log2); ++log2) {
+      const int blocks = (kblocks + (1 << log2) - 1) >> log2;
+      const bool two = tiles > stream_room(false, log2);
+      if (two && log2 > 0 && blocks < 8) continue;
+      const double waves = two ? static_cast<double>((tiles + stream_room(true, log2) - 1) / stream_room(true, log2)) : 1;
+      const double work = (rows + p.tn / 3.0) * blocks + p.tn * rows / 32.0;
+      const double cost = work * (two ? 2 * waves : 1.08) * (1 + 0.02 * log2);
+      if (p.rows == 0 || cost < best) best = cost, p.rows = rows, p.cluster = 1 << log2, *two_per_sm = two;
     }
   }
 }
@@ -190,7 +226,9 @@ int launch_stream_gemm(const F16GemmParams& q, const void* x, int64_t ldx, int x
   p.w_mn = w_mn != 0, p.x_mn = x_mn != 0;
   p.up_row = q.up_row, p.act = q.act, p.limit = q.limit, p.bias = q.bias;
   p.residual = q.residual, p.out = q.out;
-  pick_stream(q, gated, p);
+  bool two = false;
+  pick_stream(q, gated, p, &two);
+  const int room = two ? kStreamSmem : kStreamSmemAlone;
   const int kblocks = (p.k + 63) / 64;
   const int width = gated ? p.rows / 2 : p.rows;
   p.row_tiles = (q.n + width - 1) / width;
@@ -201,13 +239,13 @@ int launch_stream_gemm(const F16GemmParams& q, const void* x, int64_t ldx, int x
   p.w_atom = p.w_mn ? 8192 : p.rows * 128;
   const int block = p.x_atom * x_groups + p.w_atom * w_groups, fixed = 1024 + kStreamBarBytes;
   // two blocks a stage where three such stages fit
-  p.atoms = kblocks >= 2 * p.cluster && 6 * block <= kStreamSmem - fixed ? 2 : 1;
+  p.atoms = kblocks >= 2 * p.cluster && 6 * block <= room - fixed ? 2 : 1;
   const int stage = p.atoms * block;
   p.x_stage = p.x_atom * x_groups * p.atoms;
   p.w_stage = p.w_atom * w_groups * p.atoms;
-  p.stages = (kStreamSmem - fixed) / stage;
+  p.stages = (room - fixed) / stage;
   if (p.stages > kStreamMaxStages) p.stages = kStreamMaxStages;
-  while (fixed + stream_ring_bytes(p.stages, stage, p.atoms, p.x_atom) > kStreamSmem) --p.stages;
+  while (fixed + stream_ring_bytes(p.stages, stage, p.atoms, p.x_atom) > room) --p.stages;
   p.ring_bytes = stream_ring_bytes(p.stages, stage, p.atoms, p.x_atom);
   const bool whole = p.k % 64 == 0;
   p.w_wide = !p.w_mn && whole, p.x_wide = !p.x_mn && whole;
@@ -239,7 +277,8 @@ cudaError_t stream_attrs() {
   void* const fns[2] = {reinterpret_cast<void*>(&f16_stream_gemm_kernel<EPI, true>),
                         reinterpret_cast<void*>(&f16_stream_gemm_kernel<EPI, false>)};
   for (void* fn : fns) {
-    cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, kStreamSmem);
+    cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         kStreamSmemAlone);
     if (e == cudaSuccess)
       e = cudaFuncSetAttribute(fn, cudaFuncAttributePreferredSharedMemoryCarveout,
                                cudaSharedmemCarveoutMaxShared);
@@ -287,6 +326,7 @@ int feed_forward_init() {
   if (e == cudaSuccess) e = pair_attrs<kEpiGatedBwd>();
   if (e == cudaSuccess) e = stream_attrs<kEpiLinear>();
   if (e == cudaSuccess) e = stream_attrs<kEpiGated>();
+  if (e == cudaSuccess) e = query_stream_room();
   if (e != cudaSuccess)
     return fail(DSV4_ERR_CUDA, "cudaFuncSetAttribute: %s", cudaGetErrorString(e));
   return DSV4_OK;
@@ -349,7 +389,8 @@ int dsv4_b200_gated_gemm(const void* x, int64_t ldx, int x_mn, const void* w13, 
   DSV4_REQUIRE(z == nullptr || z_codes == nullptr, "z is kept in 16 or in 8 bits, not both");
   if (m == 0) return DSV4_OK;
   DSV4_REQUIRE(x && w13 && h, "null pointer argument");
-  DSV4_REQUIRE(ldh >= intermediate && (!z || ldz >= 2 * intermediate), "row stride below the row");
+  DSV4_REQUIRE(ldh >= intermediate && (!z || ldz >= intermediate + round_up(intermediate, 8)),
+               "row stride below the row");
   // a TMA box starts at a multiple of 16 bytes
   DSV4_REQUIRE(!w_mn || intermediate % 8 == 0,
                "w13 stored by columns needs intermediate to be a multiple of 8 (got %lld)",
@@ -359,7 +400,7 @@ int dsv4_b200_gated_gemm(const void* x, int64_t ldx, int x_mn, const void* w13, 
   p.up_row = p.n;
   p.out = mat16(h, ldh);
   p.z0 = mat16(z, ldz);
-  p.z1 = z ? mat16(static_cast<uint16_t*>(z) + intermediate, ldz) : mat16(nullptr, 0);
+  p.z1 = z ? mat16(static_cast<uint16_t*>(z) + round_up(intermediate, 8), ldz) : mat16(nullptr, 0);
   p.zq = z_codes, p.zs = z_scales, p.n32 = round_up(intermediate, kGroup);
   if (takes_stream(p))
     return launch_stream_gemm<kEpiGated>(p, x, ldx, x_mn, w13, 2 * intermediate, ldw, w_mn,
@@ -398,16 +439,16 @@ int dsv4_b200_gated_backward_gemm(const void* dy, int64_t lddy, int dy_mn, const
   if (m == 0) return DSV4_OK;
   DSV4_REQUIRE(dy && w2 && dz, "null pointer argument");
   DSV4_REQUIRE((z == nullptr) != (z_codes == nullptr), "one of z and its codes is needed");
-  DSV4_REQUIRE(lddz >= 2 * intermediate && (!z || ldz >= 2 * intermediate) &&
+  DSV4_REQUIRE(lddz >= 2 * intermediate && (!z || ldz >= intermediate + round_up(intermediate, 8)) &&
                    (!h || ldh >= intermediate), "row stride below the row");
   p.m = static_cast<int>(m), p.n = static_cast<int>(intermediate), p.k = static_cast<int>(k);
   p.act = activation;
-  const auto half = [&](const void* q, int64_t ld) {
-    return q ? mat16(static_cast<const uint16_t*>(q) + intermediate, ld) : mat16(nullptr, 0);
+  const auto half = [&](const void* q, int64_t ld, int64_t at) {
+    return q ? mat16(static_cast<const uint16_t*>(q) + at, ld) : mat16(nullptr, 0);
   };
   p.out = mat16(h, ldh);
-  p.z0 = mat16(z, ldz), p.z1 = half(z, ldz);
-  p.d0 = mat16(dz, lddz), p.d1 = half(dz, lddz);
+  p.z0 = mat16(z, ldz), p.z1 = half(z, ldz, round_up(intermediate, 8));
+  p.d0 = mat16(dz, lddz), p.d1 = half(dz, lddz, intermediate);
   p.zq = const_cast<int8_t*>(z_codes), p.zs = const_cast<float*>(z_scales);
   p.n32 = round_up(intermediate, kGroup);
   return launch_pair_gemm<kEpiGatedBwd>(p, dy, lddy, dy_mn, w2, intermediate, ldw, w_mn,

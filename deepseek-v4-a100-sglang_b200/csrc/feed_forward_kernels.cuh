@@ -28,6 +28,20 @@ __device__ __forceinline__ uint32_t ld_shared_u32(uint32_t a) {
   return v;
 }
 
+__device__ __forceinline__ void st_shared_u16(uint32_t a, uint32_t v) {
+  asm volatile("{\n\t.reg .b16 h;\n\tcvt.u16.u32 h, %1;\n\tst.shared.b16 [%0], h;\n\t}" ::"r"(a),
+               "r"(v)
+               : "memory");
+}
+__device__ __forceinline__ uint32_t ld_shared_u16(uint32_t a) {
+  uint32_t v;
+  asm volatile("{\n\t.reg .b16 h;\n\tld.shared.b16 h, [%1];\n\tcvt.u32.u16 %0, h;\n\t}"
+               : "=r"(v)
+               : "r"(a)
+               : "memory");
+  return v;
+}
+
 // 32 lanes x 32 consecutive fp32 columns of TMEM, waited on at once.
 __device__ __forceinline__ void tmem_ld_f32x32(uint32_t taddr, float (&f)[32]) {
   int32_t v[32];

@@ -183,41 +183,67 @@ __device__ __forceinline__ uint32_t idesc_f16(bool bf16, uint32_t m, uint32_t n,
 }
 
 // ---- 32 x 32 chunks of 16-bit matrices: global <-> registers of a row ----
-// Lane l moves the 16-byte pieces of rows 8i + l/4, columns 8 (l & 3): four
-// lanes cover a row's 64 bytes, so accesses are whole sectors.  The shared
-// slice turns that into one row per lane; its 16-byte units are XORed with
-// bits of the row, which leaves both sides free of bank conflicts.
+// Where rows are 16-byte aligned (mat.vec) and the chunk is whole, lane l moves
+// the 16-byte pieces of rows 8i + l/4, columns 8 (l & 3): four lanes cover a
+// row's 64 bytes, so accesses are whole sectors.  Otherwise a lane moves its
+// column, row by row: 64 contiguous bytes an access.  The shared slice turns
+// either into one row per lane; its 16-byte units are XORed with bits of the
+// row, which leaves both sides free of bank conflicts.
 __device__ __forceinline__ uint32_t slice_off(int row, int piece) {
   return static_cast<uint32_t>(row * 64 + ((piece ^ ((row >> 1) & 3)) << 4));
 }
 
+__device__ __forceinline__ uint32_t slice_elem(int row, int col) {
+  return slice_off(row, col >> 3) + 2 * (col & 7);
+}
+
+__device__ __forceinline__ bool chunk_whole(const F16Mat& mat, int col0, int cols) {
+  return mat.vec && col0 + 32 <= cols;
+}
+
+// In the second form register word i holds rows 2i and 2i + 1 of the column.
 __device__ __forceinline__ void chunk_fetch(uint4 (&r)[4], const F16Mat& mat, int lane, int row0,
                                             int rows, int col0, int cols) {
-  const int col = col0 + 8 * (lane & 3);
+  const uint16_t* base = static_cast<const uint16_t*>(mat.p) + row0 * mat.ld + col0;
+  if (chunk_whole(mat, col0, cols)) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int row = row0 + 8 * i + (lane >> 2);
-    r[i] = make_uint4(0, 0, 0, 0);
-    if (row < rows && col < cols) {
-      const uint16_t* p = static_cast<const uint16_t*>(mat.p) + row * mat.ld + col;
-      if (mat.vec && col + 8 <= cols) {
-        r[i] = *reinterpret_cast<const uint4*>(p);
-      } else {
-        uint16_t e[8];
+    for (int i = 0; i < 4; ++i) {
+      const int row = 8 * i + (lane >> 2);
+      r[i] = make_uint4(0, 0, 0, 0);
+      if (row0 + row < rows) r[i] = *reinterpret_cast<const uint4*>(base + row * mat.ld + 8 * (lane & 3));
+    }
+  } else {
+    uint32_t w[16];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) e[j] = col + j < cols ? p[j] : uint16_t(0);
-        r[i] = make_uint4(e[0] | (e[1] << 16), e[2] | (e[3] << 16), e[4] | (e[5] << 16),
-                          e[6] | (e[7] << 16));
+    for (int i = 0; i < 16; ++i) {
+      w[i] = 0;
+      if (col0 + lane < cols) {
+        if (row0 + 2 * i < rows) w[i] = base[2 * i * mat.ld + lane];
+        if (row0 + 2 * i + 1 < rows) w[i] |= static_cast<uint32_t>(base[(2 * i + 1) * mat.ld + lane]) << 16;
       }
     }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
   }
 }
 
 __device__ __forceinline__ void chunk_to_rows(uint32_t slice, int lane, const uint4 (&r)[4],
-                                              uint32_t (&w)[16]) {
+                                              bool whole, uint32_t (&w)[16]) {
+  if (whole) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
-    st_shared_v4(slice + slice_off(8 * i + (lane >> 2), lane & 3), r[i]);
+    for (int i = 0; i < 4; ++i)
+      st_shared_v4(slice + slice_off(8 * i + (lane >> 2), lane & 3), r[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t v[4] = {r[i].x, r[i].y, r[i].z, r[i].w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        st_shared_u16(slice + slice_elem(8 * i + 2 * j, lane), v[j]);
+        st_shared_u16(slice + slice_elem(8 * i + 2 * j + 1, lane), v[j] >> 16);
+      }
+    }
+  }
   __syncwarp();
 #pragma unroll
   for (int c = 0; c < 4; ++c) {
@@ -235,22 +261,19 @@ __device__ __forceinline__ void chunk_store(uint32_t slice, int lane, const uint
     st_shared_v4(slice + slice_off(lane, c),
                  make_uint4(w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]));
   __syncwarp();
-  const int col = col0 + 8 * (lane & 3);
+  uint16_t* base = static_cast<uint16_t*>(mat.p) + row0 * mat.ld + col0;
+  if (chunk_whole(mat, col0, cols)) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int row = row0 + 8 * i + (lane >> 2);
-    const uint4 v = ld_shared_v4(slice + slice_off(8 * i + (lane >> 2), lane & 3));
-    if (row < rows && col < cols) {
-      uint16_t* p = static_cast<uint16_t*>(mat.p) + row * mat.ld + col;
-      if (mat.vec && col + 8 <= cols) {
-        *reinterpret_cast<uint4*>(p) = v;
-      } else {
-        const uint32_t e[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-          if (col + j < cols) p[j] = static_cast<uint16_t>(e[j >> 1] >> (16 * (j & 1)));
-      }
+    for (int i = 0; i < 4; ++i) {
+      const int row = 8 * i + (lane >> 2);
+      const uint4 v = ld_shared_v4(slice + slice_off(row, lane & 3));
+      if (row0 + row < rows) *reinterpret_cast<uint4*>(base + row * mat.ld + 8 * (lane & 3)) = v;
     }
+  } else if (col0 + lane < cols) {
+#pragma unroll 8
+    for (int row = 0; row < 32; ++row)
+      if (row0 + row < rows)
+        base[row * mat.ld + lane] = static_cast<uint16_t>(ld_shared_u16(slice + slice_elem(row, lane)));
   }
   __syncwarp();
 }
@@ -489,7 +512,7 @@ __global__ void __launch_bounds__(kF16Threads, 1)
           }
           act_row(p.act, v);
           if (p.residual.p) {
-            chunk_to_rows(slice1, lane, rres, w);
+            chunk_to_rows(slice1, lane, rres, chunk_whole(p.residual, col, p.n), w);
 #pragma unroll
             for (int j = 0; j < 32; ++j) v[j] += unpack_16<BF16>(w[j >> 1], j & 1);
           }
@@ -557,10 +580,10 @@ __global__ void __launch_bounds__(kF16Threads, 1)
             chunk_fetch(rg, p.z0, lane, row0, p.m, col, p.n);
             chunk_fetch(ru, p.z1, lane, row0, p.m, col, p.n);
             uint32_t w[16];
-            chunk_to_rows(slice0, lane, rg, w);
+            chunk_to_rows(slice0, lane, rg, chunk_whole(p.z0, col, p.n), w);
 #pragma unroll
             for (int j = 0; j < 32; ++j) g[j] = unpack_16<BF16>(w[j >> 1], j & 1);
-            chunk_to_rows(slice1, lane, ru, w);
+            chunk_to_rows(slice1, lane, ru, chunk_whole(p.z1, col, p.n), w);
 #pragma unroll
             for (int j = 0; j < 32; ++j) u[j] = unpack_16<BF16>(w[j >> 1], j & 1);
           }

@@ -34,7 +34,8 @@ constexpr int kStreamThreads = 256;
 constexpr int kStreamMaxTokens = 128;
 constexpr int kStreamMaxStages = 12;
 constexpr int kStreamBarBytes = 256;
-constexpr int kStreamSmem = 112 * 1024;  // two CTAs per SM
+constexpr int kStreamSmem = 112 * 1024;       // two CTAs per SM
+constexpr int kStreamSmemAlone = 200 * 1024;  // one
 static_assert((2 * kStreamMaxStages + 1) * 8 + 8 <= kStreamBarBytes, "barrier area");
 
 // An MMA reads 128 token rows (16 KB) from where a block's tokens begin,

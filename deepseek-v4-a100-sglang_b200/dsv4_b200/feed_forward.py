@@ -454,7 +454,7 @@ class SavedFeedForward:
     x: tuple
     w13: torch.Tensor
     w2: torch.Tensor
-    z: tuple  # (z,) [M, 2I], or 8-bit (codes, scales)
+    z: tuple  # (z,) [M, 2I] (halves padded to 8), or 8-bit (codes, scales)
     h: Optional[torch.Tensor]  # the gated product; formed again from z when kept in 8 bits
     activation: Optional[str]
     clamp_limit: Optional[float]
@@ -503,7 +503,7 @@ def _ffn(x, w13, w2, activation, clamp_limit, residual, m, hidden, inter, n, che
     if keep_x and checkpoint is not None:
         xk = _checkpoint(x)
     if keep_z and checkpoint is None:
-        zk = (_rows_buffer(m, 2 * inter, x),)
+        zk = (x.new_empty((m, 2 * _up(inter, 8))),)
     elif keep_z:
         zk = _empty_codes(m, 2 * _up(inter, _GROUP), x)
     if m == 0:

@@ -417,7 +417,8 @@ DSV4_API int dsv4_b200_dense_gemm(const void* a, int64_t lda, int a_mn, const vo
 
 /* h[m][intermediate] = act(min(g, L)) * clamp(u, -L, L), g and u the products
  * of x with rows [0, intermediate) and [intermediate, 2 intermediate) of w13.
- * z [m][2 intermediate] (or its codes) receives g and u before the clamp.
+ * z (or its codes) receives g and u before the clamp: row r of g at z + r ldz,
+ * of u ceil8(intermediate) elements behind it.
  * w_mn = 1 needs intermediate % 8 == 0. */
 DSV4_API int dsv4_b200_gated_gemm(const void* x, int64_t ldx, int x_mn, const void* w13, int64_t ldw,
                                   int w_mn, int64_t m, int64_t intermediate, int64_t k, int dtype,
