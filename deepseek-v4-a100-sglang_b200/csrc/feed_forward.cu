@@ -97,20 +97,20 @@ int encode_wide_mn(CUtensorMap* map, const char* what, const void* p, int64_t ro
   return DSV4_OK;
 }
 
-// Columns of a pair tile.  A wave of tiles costs its MMA cycles (2 per column
-// and 64 of k) or its operand bytes from L2, whichever is longer; the tile
-// that needs the fewest wave-cycles wins, the wider one on a tie.
-int pick_tn(int64_t m, int64_t n, bool gated) {
-  const int64_t pairs = sm_count() / 2, tiles_m = (m + 255) / 256;
+// Columns of a pair tile, and the microseconds that the pair product takes with
+// them.  64 of k cost a tile 0.11 us and 1.04 ns a column (measured at 64, 128
+// and 256 columns: 173, 229 and 377 ns, the last under the power cap); the tile
+// that needs the least over all waves wins, the wider one on a tie.  3 us are
+// set-up and the last tile's epilogue.
+int pick_tn(int m, int n, int k, bool gated, double* us) {
+  const int pairs = sm_count() / 2, tiles_m = (m + 255) / 256;
   const int step = gated ? 64 : 32;
-  int best = 256;
-  double best_cost = 0;
-  for (int tn = 256; tn >= step; tn -= step) {
-    const int64_t width = gated ? tn / 2 : tn;
-    const int64_t tiles = tiles_m * ((n + width - 1) / width);
-    const double mma = 2.0 * tn, load = (16384.0 + 64.0 * tn) / 64.0;
-    const double cost = static_cast<double>((tiles + pairs - 1) / pairs) * (mma > load ? mma : load);
-    if (tn == 256 || cost < 0.98 * best_cost) best = tn, best_cost = cost;
+  int best = 0;
+  for (int tn = 256; tn >= 64; tn -= step) {
+    const int width = gated ? tn / 2 : tn;
+    const int64_t tiles = static_cast<int64_t>(tiles_m) * ((n + width - 1) / width);
+    const double cost = static_cast<double>((tiles + pairs - 1) / pairs) * ((k + 63) / 64) * (0.11 + 0.00104 * tn) + 3.0;
+    if (best == 0 || cost < 0.99 * *us) best = tn, *us = cost;
   }
   return best;
 }
@@ -120,7 +120,8 @@ int launch_pair_gemm(F16GemmParams& p, const void* a, int64_t lda, int a_mn, con
                      int64_t b_rows, int64_t ldb, int b_mn, bool bf16, cudaStream_t st) {
   p.a_mn = a_mn != 0;
   p.b_mn = b_mn != 0;
-  p.tn = pick_tn(p.m, p.n, EPI == kEpiGated);
+  double us = 0;
+  p.tn = pick_tn(p.m, p.n, p.k, EPI == kEpiGated, &us);
   const int half = p.tn / 2, width = EPI == kEpiGated ? half : p.tn;
   p.b_stage = p.b_mn ? (half + 63) / 64 * 8192 : half * 128;
   const int stage = kF16ABytes + p.b_stage;
@@ -157,10 +158,10 @@ int launch_pair_gemm(F16GemmParams& p, const void* a, int64_t lda, int a_mn, con
 constexpr int kMaxDevices = 64;
 int g_stream_room[kMaxDevices][2][4];
 
-int stream_room(bool two, int log2) {
+const int (*stream_room())[4] {
   int dev = 0;
   cudaGetDevice(&dev);
-  return dev >= 0 && dev < kMaxDevices ? g_stream_room[dev][two][log2] : 1;
+  return g_stream_room[dev >= 0 && dev < kMaxDevices ? dev : 0];
 }
 
 cudaError_t query_stream_room() {
@@ -187,6 +188,12 @@ cudaError_t query_stream_room() {
   return cudaSuccess;
 }
 
+// Tokens of a tile: all of them up to 128, else tiles of equal height.
+int stream_tokens(int64_t m) {
+  const int64_t tiles = (m + kStreamMaxTokens - 1) / kStreamMaxTokens;
+  return static_cast<int>(round_up((m + tiles - 1) / tiles, 16));
+}
+
 // Few tokens: the weight-streaming kernel.  A launch takes as long as its
 // busiest SM, whose work is counted in weight rows x blocks of k: a block of a
 // CTA costs its weight rows and, from L2, a third as much for its tokens; the
@@ -195,39 +202,37 @@ cudaError_t query_stream_room() {
 // at least 8 blocks each.  Doubling the cluster costs 2 %.  The least of all
 // tile heights and cluster sizes is taken.  (Fitted to 6 shapes, 512 x 1024 to
 // 14336 x 1024 and 4096 x 7168, at 1 to 128 tokens: the choice is on average
-// 2 %, at most 10 % slower than the best of all measured.)
-void pick_stream(const F16GemmParams& q, bool gated, F16StreamParams& p, bool* two_per_sm) {
+// 2 %, at most 10 % slower than the best of all measured.)  A unit of this
+// count is 2.35 ns, on top of 3.2 us.
+double pick_stream(const F16GemmParams& q, bool gated, F16StreamParams& p, bool* two_per_sm) {
   const int kblocks = (q.k + 63) / 64, step = gated ? 32 : 16;
-  const int64_t token_tiles = (q.m + p.tn - 1) / p.tn;
+  const int token_tiles = (q.m + p.tn - 1) / p.tn;
+  const int (*room)[4] = stream_room();
   double best = 0;
   p.rows = 0;
   for (int rows = 128; rows >= (p.w_mn ? 128 : 64); rows -= step) {
     const int cols = gated ? rows / 2 : rows;
-    const int64_t tiles = (q.n + cols - 1) / cols * token_tiles;
+    const int tiles = (q.n + cols - 1) / cols * token_tiles;
     for (int log2 = 0; log2 < 4 && (log2 == 0 || kblocks >= 2 << log2); ++log2) {
       const int blocks = (kblocks + (1 << log2) - 1) >> log2;
-      const bool two = tiles > stream_room(false, log2);
+      const bool two = tiles > room[0][log2];
       if (two && log2 > 0 && blocks < 8) continue;
-      const double waves = two ? static_cast<double>((tiles + stream_room(true, log2) - 1) / stream_room(true, log2)) : 1;
-      const double work = (rows + p.tn / 3.0) * blocks + p.tn * rows / 32.0;
-      const double cost = work * (two ? 2 * waves : 1.08) * (1 + 0.02 * log2);
+      const double waves = two ? 2 * ((tiles + room[1][log2] - 1) / room[1][log2]) : 1.08;
+      const double cost = ((rows + p.tn / 3.0) * blocks + p.tn * rows / 32.0) * waves * (1 + 0.02 * log2);
       if (p.rows == 0 || cost < best) best = cost, p.rows = rows, p.cluster = 1 << log2, *two_per_sm = two;
     }
   }
+  return 3.2 + 0.00235 * best;
 }
 
 template <int EPI>
-int launch_stream_gemm(const F16GemmParams& q, const void* x, int64_t ldx, int x_mn, const void* w,
+int launch_stream_gemm(const F16GemmParams& q, F16StreamParams& p, bool two, const void* x, int64_t ldx, int x_mn, const void* w,
                        int64_t w_rows, int64_t ldw, int w_mn, bool bf16, cudaStream_t st) {
   constexpr bool gated = EPI == kEpiGated;
-  F16StreamParams p = {};
   p.m = q.m, p.n = q.n, p.k = q.k;
-  p.tn = static_cast<int>(round_up(q.m < kStreamMaxTokens ? q.m : kStreamMaxTokens, 16));
-  p.w_mn = w_mn != 0, p.x_mn = x_mn != 0;
+  p.x_mn = x_mn != 0;
   p.up_row = q.up_row, p.act = q.act, p.limit = q.limit, p.bias = q.bias;
   p.residual = q.residual, p.out = q.out;
-  bool two = false;
-  pick_stream(q, gated, p, &two);
   const int room = two ? kStreamSmem : kStreamSmemAlone;
   const int kblocks = (p.k + 63) / 64;
   const int width = gated ? p.rows / 2 : p.rows;
@@ -287,9 +292,18 @@ cudaError_t stream_attrs() {
   return cudaSuccess;
 }
 
-// Up to 128 tokens whose values before the activation are not kept.
-bool takes_stream(const F16GemmParams& p) {
-  return p.m <= kStreamMaxTokens && p.z0.p == nullptr && p.zq == nullptr;
+// The faster of the two products by the counts above (values before the
+// activation are kept by the pair product only).  1 to 128 tokens stream nearly
+// always; beyond that it is long contractions of few columns: 256 tokens 4096
+// -> 1024 take 8.0 us streamed and 13.7 in pairs, 512 tokens 7168 -> 4096 37
+// and 27.
+bool takes_stream(const F16GemmParams& q, bool gated, int w_mn, F16StreamParams& p, bool* two) {
+  if (q.zbits != 0 || q.m > 1024) return false;
+  p.tn = stream_tokens(q.m);
+  p.w_mn = w_mn != 0;
+  double pair_us = 0;
+  pick_tn(q.m, q.n, q.k, gated, &pair_us);
+  return pick_stream(q, gated, p, two) < pair_us;
 }
 
 constexpr int64_t kMaxDim = 1ll << 30;
@@ -311,10 +325,12 @@ int check_limit(int has_limit, float limit, float* out) {
   return DSV4_OK;
 }
 
-// 8-bit kept values are moved by 16-byte pieces
-int check_codes(const int8_t* zq, const float* zs) {
-  DSV4_REQUIRE((zq == nullptr) == (zs == nullptr), "codes and scales go together");
-  DSV4_REQUIRE(aligned16(zq), "codes must be 16-byte aligned");
+// kept values are moved by 16-byte pieces
+int check_kept(const void* codes, int bits, const float* scales) {
+  DSV4_REQUIRE(bits == 0 || bits == 8 || bits == 16, "z_bits must be 0, 8 or 16 (got %d)", bits);
+  DSV4_REQUIRE((codes != nullptr) == (bits != 0) && (scales != nullptr) == (bits != 0),
+               "z_codes, z_bits and z_scales go together");
+  DSV4_REQUIRE(aligned16(codes), "codes must be 16-byte aligned");
   return DSV4_OK;
 }
 
@@ -352,15 +368,13 @@ extern "C" {
 int dsv4_b200_dense_gemm(const void* a, int64_t lda, int a_mn, const void* b, int64_t ldb, int b_mn,
                          int64_t m, int64_t n, int64_t k, int dtype, const void* bias,
                          int activation, const void* residual, int64_t ldr, void* out, int64_t ldo,
-                         void* z, int64_t ldz, int8_t* z_codes, float* z_scales, void* stream) {
+                         void* z_codes, int z_bits, float* z_scales, void* stream) {
   if (int r = ensure_init()) return r;
   if (int r = check_common(m, n, k, dtype, activation)) return r;
-  if (int r = check_codes(z_codes, z_scales)) return r;
-  DSV4_REQUIRE(z == nullptr || z_codes == nullptr, "z is kept in 16 or in 8 bits, not both");
+  if (int r = check_kept(z_codes, z_bits, z_scales)) return r;
   if (m == 0) return DSV4_OK;
   DSV4_REQUIRE(a && b && out, "null pointer argument");
-  DSV4_REQUIRE(ldo >= n && (!residual || ldr >= n || ldr == 0) && (!z || ldz >= n),
-               "row stride below n");
+  DSV4_REQUIRE(ldo >= n && (!residual || ldr >= n || ldr == 0), "row stride below n");
   F16GemmParams p = {};
   p.m = static_cast<int>(m), p.n = static_cast<int>(n), p.k = static_cast<int>(k);
   p.act = activation;
@@ -368,10 +382,11 @@ int dsv4_b200_dense_gemm(const void* a, int64_t lda, int a_mn, const void* b, in
   p.bias = bias;
   p.residual = mat16(residual, ldr);
   p.out = mat16(out, ldo);
-  p.z0 = mat16(z, ldz);
-  p.zq = z_codes, p.zs = z_scales, p.n32 = round_up(n, kGroup);
-  if (takes_stream(p))
-    return launch_stream_gemm<kEpiLinear>(p, a, lda, a_mn, b, n, ldb, b_mn, dtype == DSV4_BF16,
+  p.zq = z_codes, p.zbits = z_bits, p.zs = z_scales, p.n32 = round_up(n, kGroup);
+  F16StreamParams few = {};
+  bool two = false;
+  if (takes_stream(p, false, b_mn, few, &two))
+    return launch_stream_gemm<kEpiLinear>(p, few, two, a, lda, a_mn, b, n, ldb, b_mn, dtype == DSV4_BF16,
                                           as_stream(stream));
   return launch_pair_gemm<kEpiLinear>(p, a, lda, a_mn, b, n, ldb, b_mn, dtype == DSV4_BF16,
                                       as_stream(stream));
@@ -379,18 +394,16 @@ int dsv4_b200_dense_gemm(const void* a, int64_t lda, int a_mn, const void* b, in
 
 int dsv4_b200_gated_gemm(const void* x, int64_t ldx, int x_mn, const void* w13, int64_t ldw, int w_mn,
                          int64_t m, int64_t intermediate, int64_t k, int dtype, int activation,
-                         int has_clamp, float clamp_limit, void* h, int64_t ldh, void* z, int64_t ldz,
-                         int8_t* z_codes, float* z_scales, void* stream) {
+                         int has_clamp, float clamp_limit, void* h, int64_t ldh, void* z_codes, int z_bits,
+                         float* z_scales, void* stream) {
   if (int r = ensure_init()) return r;
   if (int r = check_common(m, 2 * intermediate, k, dtype, activation)) return r;
-  if (int r = check_codes(z_codes, z_scales)) return r;
+  if (int r = check_kept(z_codes, z_bits, z_scales)) return r;
   F16GemmParams p = {};
   if (int r = check_limit(has_clamp, clamp_limit, &p.limit)) return r;
-  DSV4_REQUIRE(z == nullptr || z_codes == nullptr, "z is kept in 16 or in 8 bits, not both");
   if (m == 0) return DSV4_OK;
   DSV4_REQUIRE(x && w13 && h, "null pointer argument");
-  DSV4_REQUIRE(ldh >= intermediate && (!z || ldz >= intermediate + round_up(intermediate, 8)),
-               "row stride below the row");
+  DSV4_REQUIRE(ldh >= intermediate, "row stride below the row");
   // a TMA box starts at a multiple of 16 bytes
   DSV4_REQUIRE(!w_mn || intermediate % 8 == 0,
                "w13 stored by columns needs intermediate to be a multiple of 8 (got %lld)",
@@ -399,11 +412,11 @@ int dsv4_b200_gated_gemm(const void* x, int64_t ldx, int x_mn, const void* w13, 
   p.act = activation;
   p.up_row = p.n;
   p.out = mat16(h, ldh);
-  p.z0 = mat16(z, ldz);
-  p.z1 = z ? mat16(static_cast<uint16_t*>(z) + round_up(intermediate, 8), ldz) : mat16(nullptr, 0);
-  p.zq = z_codes, p.zs = z_scales, p.n32 = round_up(intermediate, kGroup);
-  if (takes_stream(p))
-    return launch_stream_gemm<kEpiGated>(p, x, ldx, x_mn, w13, 2 * intermediate, ldw, w_mn,
+  p.zq = z_codes, p.zbits = z_bits, p.zs = z_scales, p.n32 = round_up(intermediate, kGroup);
+  F16StreamParams few = {};
+  bool two = false;
+  if (takes_stream(p, true, w_mn, few, &two))
+    return launch_stream_gemm<kEpiGated>(p, few, two, x, ldx, x_mn, w13, 2 * intermediate, ldw, w_mn,
                                          dtype == DSV4_BF16, as_stream(stream));
   return launch_pair_gemm<kEpiGated>(p, x, ldx, x_mn, w13, 2 * intermediate, ldw, w_mn,
                                      dtype == DSV4_BF16, as_stream(stream));
@@ -414,42 +427,35 @@ int dsv4_b200_gated_feed_forward(const void* x, int64_t ldx, int x_mn, const voi
                                  int64_t hidden, int64_t intermediate, int64_t out_cols, int dtype,
                                  int activation, int has_clamp, float clamp_limit,
                                  const void* residual, int64_t ldr, void* h, int64_t ldh, void* out,
-                                 int64_t ldo, void* z, int64_t ldz, int8_t* z_codes,
-                                 float* z_scales, void* stream) {
+                                 int64_t ldo, void* z_codes, int z_bits, float* z_scales,
+                                 void* stream) {
   if (int r = dsv4_b200_gated_gemm(x, ldx, x_mn, w13, ldw13, w13_mn, m, intermediate, hidden, dtype,
-                                   activation, has_clamp, clamp_limit, h, ldh, z, ldz, z_codes,
+                                   activation, has_clamp, clamp_limit, h, ldh, z_codes, z_bits,
                                    z_scales, stream))
     return r;
   return dsv4_b200_dense_gemm(h, ldh, 0, w2, ldw2, w2_mn, m, out_cols, intermediate, dtype, nullptr,
-                              DSV4_ACT_NONE, residual, ldr, out, ldo, nullptr, 0, nullptr, nullptr,
-                              stream);
+                              DSV4_ACT_NONE, residual, ldr, out, ldo, nullptr, 0, nullptr, stream);
 }
 
 int dsv4_b200_gated_backward_gemm(const void* dy, int64_t lddy, int dy_mn, const void* w2,
                                   int64_t ldw, int w_mn, int64_t m, int64_t intermediate, int64_t k,
                                   int dtype, int activation, int has_clamp, float clamp_limit,
-                                  const void* z, int64_t ldz, const int8_t* z_codes,
-                                  const float* z_scales, void* dz, int64_t lddz, void* h, int64_t ldh,
+                                  const void* z_codes, int z_bits, const float* z_scales, void* dz, int64_t lddz, void* h, int64_t ldh,
                                   void* stream) {
   if (int r = ensure_init()) return r;
   if (int r = check_common(m, 2 * intermediate, k, dtype, activation)) return r;
-  if (int r = check_codes(z_codes, z_scales)) return r;
+  if (int r = check_kept(z_codes, z_bits, z_scales)) return r;
   F16GemmParams p = {};
   if (int r = check_limit(has_clamp, clamp_limit, &p.limit)) return r;
   if (m == 0) return DSV4_OK;
   DSV4_REQUIRE(dy && w2 && dz, "null pointer argument");
-  DSV4_REQUIRE((z == nullptr) != (z_codes == nullptr), "one of z and its codes is needed");
-  DSV4_REQUIRE(lddz >= 2 * intermediate && (!z || ldz >= intermediate + round_up(intermediate, 8)) &&
-                   (!h || ldh >= intermediate), "row stride below the row");
+  DSV4_REQUIRE(z_bits != 0, "the kept g and u are needed");
+  DSV4_REQUIRE(lddz >= 2 * intermediate && (!h || ldh >= intermediate), "row stride below the row");
   p.m = static_cast<int>(m), p.n = static_cast<int>(intermediate), p.k = static_cast<int>(k);
   p.act = activation;
-  const auto half = [&](const void* q, int64_t ld, int64_t at) {
-    return q ? mat16(static_cast<const uint16_t*>(q) + at, ld) : mat16(nullptr, 0);
-  };
   p.out = mat16(h, ldh);
-  p.z0 = mat16(z, ldz), p.z1 = half(z, ldz, round_up(intermediate, 8));
-  p.d0 = mat16(dz, lddz), p.d1 = half(dz, lddz, intermediate);
-  p.zq = const_cast<int8_t*>(z_codes), p.zs = const_cast<float*>(z_scales);
+  p.d0 = mat16(dz, lddz), p.d1 = mat16(static_cast<const uint16_t*>(dz) + intermediate, lddz);
+  p.zq = const_cast<void*>(z_codes), p.zbits = z_bits, p.zs = const_cast<float*>(z_scales);
   p.n32 = round_up(intermediate, kGroup);
   return launch_pair_gemm<kEpiGatedBwd>(p, dy, lddy, dy_mn, w2, intermediate, ldw, w_mn,
                                         dtype == DSV4_BF16, as_stream(stream));
@@ -463,7 +469,7 @@ int dsv4_b200_checkpoint_int8(const void* x, int dtype, int64_t m, int64_t k, in
                "bad shape m=%lld k=%lld ldx=%lld", (long long)m, (long long)k, (long long)ldx);
   if (m == 0) return DSV4_OK;
   DSV4_REQUIRE(x && codes && scales, "null pointer argument");
-  if (int r = check_codes(codes, scales)) return r;
+  DSV4_REQUIRE(aligned16(codes), "codes must be 16-byte aligned");
   const int64_t k32 = round_up(k, kGroup), cb = (k32 + 255) / 256, blocks = (m + 31) / 32 * cb;
   DSV4_REQUIRE(blocks < (1ll << 31), "checkpoint too large");
   const int per = dtype == DSV4_F32 ? 4 : 8;
@@ -487,7 +493,7 @@ int dsv4_b200_restore_int8(const int8_t* codes, const float* scales, int64_t m, 
                "bad shape m=%lld k=%lld ldo=%lld", (long long)m, (long long)k, (long long)ldo);
   if (m == 0) return DSV4_OK;
   DSV4_REQUIRE(out && codes && scales, "null pointer argument");
-  if (int r = check_codes(codes, scales)) return r;
+  DSV4_REQUIRE(aligned16(codes), "codes must be 16-byte aligned");
   const int64_t k32 = round_up(k, kGroup), cb = (k32 + 255) / 256, blocks = (m + 31) / 32 * cb;
   DSV4_REQUIRE(blocks < (1ll << 31), "checkpoint too large");
   const int per = dtype == DSV4_F32 ? 4 : 8;
@@ -515,28 +521,26 @@ int dsv4_b200_act_backward_slabs(int64_t m, int64_t n, int64_t* slabs) {
   return DSV4_OK;
 }
 
-int dsv4_b200_act_backward(const void* dy, int64_t lddy, const void* z, int64_t ldz,
-                           const int8_t* z_codes, const float* z_scales, int64_t m, int64_t n,
+int dsv4_b200_act_backward(const void* dy, int64_t lddy, const void* z_codes, int z_bits,
+                           const float* z_scales, int64_t m, int64_t n,
                            int dtype, int activation, void* dz, int64_t lddz, float* partial,
                            int64_t slabs, void* dbias, void* stream) {
   if (int r = ensure_init()) return r;
   if (int r = check_common(m, n, 1, dtype, activation)) return r;
-  if (int r = check_codes(z_codes, z_scales)) return r;
+  if (int r = check_kept(z_codes, z_bits, z_scales)) return r;
   int64_t need = 0;
   if (int r = dsv4_b200_act_backward_slabs(m, n, &need)) return r;
   DSV4_REQUIRE((dbias == nullptr) == (partial == nullptr), "dbias and its workspace go together");
   DSV4_REQUIRE(!dbias || slabs >= need, "workspace of %lld slabs, %lld needed", (long long)slabs,
                (long long)need);
   DSV4_REQUIRE(activation == kActNone || m == 0 ||
-                   (dz && lddz >= n && (z == nullptr) != (z_codes == nullptr) && (!z || ldz >= n)),
-               "an activation needs dz and one of z and its codes");
+                   (dz && lddz >= n && z_bits != 0), "an activation needs dz and the kept z");
   DSV4_REQUIRE(m == 0 || (dy && (lddy >= n || m == 1)), "bad dy");
   DSV4_REQUIRE(need < 65536, "too many rows");
   cudaStream_t st = as_stream(stream);
   ActBackward p = {};
   p.dy = dy, p.lddy = lddy, p.vec_dy = mat16(dy, lddy).vec;
-  p.z = z, p.ldz = ldz, p.vec_z = mat16(z, ldz).vec;
-  p.zq = z_codes, p.zs = z_scales, p.n32 = round_up(n, kGroup);
+  p.zq = z_codes, p.zbits = z_bits, p.zs = z_scales, p.n32 = round_up(n, kGroup);
   p.dz = dz, p.lddz = lddz, p.vec_dz = mat16(dz, lddz).vec;
   p.partial = partial;
   p.m = m, p.n = n, p.act = activation;

@@ -82,27 +82,6 @@ __device__ __forceinline__ void pack_row(const float (&v)[32], uint32_t (&w)[16]
   for (int j = 0; j < 16; ++j) w[j] = pack_16<BF16>(v[2 * j], v[2 * j + 1]);
 }
 
-// Rounded to 16 bits, but on the same side of the clamp limit as before: the
-// backward pass asks |z| <= limit of the kept value, and a value rounded over
-// the border would lose or gain its whole gradient.  At most one 16-bit step
-// (against half a step) for values next to the limit; limit > 0.
-template <bool BF16>
-__device__ __forceinline__ uint32_t round_sided(float z, float limit) {
-  uint32_t b = pack_16<BF16>(z, 0.f) & 0xffffu;
-  const bool over = fabsf(z) > limit, kept = fabsf(unpack_16<BF16>(b, 0)) > limit;
-  if (over && !kept) ++b;
-  if (!over && kept && z == z) --b;
-  return b;
-}
-
-template <bool BF16>
-__device__ __forceinline__ void pack_row_sided(const float (&v)[32], uint32_t (&w)[16],
-                                               float limit) {
-#pragma unroll
-  for (int j = 0; j < 16; ++j)
-    w[j] = round_sided<BF16>(v[2 * j], limit) | (round_sided<BF16>(v[2 * j + 1], limit) << 16);
-}
-
 // ---- activations: value and slope ----
 // sigmoid(z) = 1 / (1 + exp(-z)) in fast fp32 (a few units of 2^-23, against
 // the 2^-9 and more of the 16-bit results); gelu_tanh is z sigmoid(2a) with
@@ -228,20 +207,23 @@ __device__ __forceinline__ float rcp_approx(float a) {
   return r;
 }
 
-// The scale is rounded toward zero: 127 steps never pass amax, so the largest
-// finite value stays finite.
-__device__ __forceinline__ float group_step(uint32_t amax_bits) {
+// Whole steps up to amax: 127 in 8 bits, 32767 in 16.  The scale is rounded
+// toward zero: that many steps never pass amax, so the largest finite value
+// stays finite.
+constexpr float kSteps8 = 127.f, kSteps16 = 32767.f;
+
+__device__ __forceinline__ float group_step(uint32_t amax_bits, float steps) {
   const float amax = __uint_as_float(amax_bits);
   if (amax_bits >= 0x7f800000u) return CUDART_NAN_F;
-  return amax < kTinyGroup ? 0.f : __fdiv_rz(amax, 127.f);
+  return amax < kTinyGroup ? 0.f : __fdiv_rz(amax, steps);
 }
 
-// 127 / amax to about 2^-22; 0 for a group that holds zeros or decodes to NaN
-__device__ __forceinline__ float group_inverse(uint32_t amax_bits) {
+// steps / amax to about 2^-22; 0 for a group that holds zeros or decodes to NaN
+__device__ __forceinline__ float group_inverse(uint32_t amax_bits, float steps) {
   const float amax = __uint_as_float(amax_bits);
   if (amax_bits >= 0x7f800000u || amax < kTinyGroup) return 0.f;
-  return amax > 1.8446744e19f ? (127.f * 5.4210109e-20f) * rcp_approx(amax * 5.4210109e-20f)
-                              : 127.f * rcp_approx(amax);  // 2^64, 2^-64
+  return amax > 1.8446744e19f ? (steps * 5.4210109e-20f) * rcp_approx(amax * 5.4210109e-20f)
+                              : steps * rcp_approx(amax);  // 2^64, 2^-64
 }
 
 // Correctly rounded 127 v / amax for 16-bit v: p = 127 v is exact, the first
@@ -307,13 +289,22 @@ __device__ __forceinline__ uint32_t quantize4_f32(const float (&v)[4], float inv
   return pack_codes(q[0], q[1], q[2], q[3]);
 }
 
-// A thread's own group of fp32 sums: codes (4 per word) and the scale.  (A sum
-// next to the border of two codes is itself only known to its last bits.)
-__device__ __forceinline__ float quantize_group(const float (&v)[32], uint32_t (&codes)[8]) {
+// What the backward pass needs of a value before its activation is kept as
+// groups too, in 8 bits or in 16: a thread's own 32 fp32 sums -> codes and the
+// scale.  (A sum next to the border of two codes is itself only known to its
+// last bits.)  16 bits hold a group to amax / 65534, where bf16 would be off by
+// 1/512 of every value: gradients are then as exact as their own rounding, at
+// 2.125 bytes a value.
+__device__ __forceinline__ uint32_t group_top(const float (&v)[32]) {
   uint32_t top = 0;
 #pragma unroll
   for (int j = 0; j < 32; ++j) top = max(top, __float_as_uint(v[j]) & 0x7fffffffu);
-  const float inv = group_inverse(top);
+  return top;
+}
+
+__device__ __forceinline__ float keep_group8(const float (&v)[32], uint32_t (&codes)[8]) {
+  const uint32_t top = group_top(v);
+  const float inv = group_inverse(top, kSteps8);
   if (inv == 0.f) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) codes[j] = 0;
@@ -322,7 +313,52 @@ __device__ __forceinline__ float quantize_group(const float (&v)[32], uint32_t (
     for (int j = 0; j < 8; ++j)
       codes[j] = pack_codes(v[4 * j] * inv, v[4 * j + 1] * inv, v[4 * j + 2] * inv, v[4 * j + 3] * inv);
   }
-  return group_step(top);
+  return group_step(top, kSteps8);
+}
+
+// With a clamp limit the code stays on the value's side of it: the backward
+// pass asks |z| <= limit of the kept value, and one kept over the border would
+// lose or gain its whole gradient.  For relu a value other than zero keeps its
+// sign the same way.  That is one step instead of half a step next to the
+// border.
+__device__ __forceinline__ float keep_group16(const float (&v)[32], float limit, bool keep_sign,
+                                              uint32_t (&codes)[16]) {
+  const uint32_t top = group_top(v);
+  const float inv = group_inverse(top, kSteps16), step = group_step(top, kSteps16);
+  if (inv == 0.f) {
+#pragma unroll
+    for (int j = 0; j < 16; ++j) codes[j] = 0;
+    return step;
+  }
+  const bool limited = limit < CUDART_INF_F || keep_sign;
+#pragma unroll
+  for (int j = 0; j < 16; ++j) {
+    float q[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const float x = v[2 * j + i];
+      q[i] = x * inv + 12582912.f;  // 1.5 * 2^23: the nearest whole number in the low bits
+      if (limited) {
+        const float n = q[i] - 12582912.f, toward = x < 0.f ? 1.f : -1.f;  // toward zero
+        const bool over = fabsf(x) > limit, kept = fabsf(n * step) > limit;
+        if (over && !kept) q[i] -= toward;
+        if (!over && kept) q[i] += toward;
+        if (keep_sign && n == 0.f && x != 0.f) q[i] -= toward;
+      }
+    }
+    codes[j] = prmt(__float_as_uint(q[0]), __float_as_uint(q[1]), 0x5410u);
+  }
+  return step;
+}
+
+// Codes back to whole numbers: the code, moved to be positive, as the low bits
+// of a float 2^23 + code.
+__device__ __forceinline__ float code16_value(uint32_t w, int hi) {
+  return __uint_as_float(prmt(w ^ 0x80008000u, 0x4b000000u, hi ? 0x7432u : 0x7410u)) - 8421376.f;
+}
+
+__device__ __forceinline__ float code8_value(uint32_t w, int byte) {
+  return __uint_as_float(prmt(w ^ 0x80808080u, 0x4b000000u, 0x7440u + byte)) - 8388736.f;
 }
 
 // 8 consecutive values of a 16- or 32-bit row; pieces past `cols` read as 0.
@@ -459,8 +495,8 @@ __global__ void __launch_bounds__(256)
   }
   const int sub = lane & 3;
   const uint32_t mine = sub == 0 ? top[0] : sub == 1 ? top[1] : sub == 2 ? top[2] : top[3];
-  s_scale[lane >> 2][warp + 8 * sub] = group_step(mine);
-  float own = group_inverse(mine);
+  s_scale[lane >> 2][warp + 8 * sub] = group_step(mine, kSteps8);
+  float own = group_inverse(mine, kSteps8);
   if (!F32) own = group_special(mine) ? -own : own * kTieBias;
   int8_t* const c = codes + row0 * k32 + col;
 #pragma unroll
@@ -530,7 +566,7 @@ __global__ void __launch_bounds__(256)
     float v[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j)
-      v[j] = s * static_cast<float>(static_cast<int8_t>(w[j >> 2] >> (8 * (j & 3))));
+      v[j] = s * code8_value(w[j >> 2], j & 3);
     if (row < m && col < k) store_piece8<DT>(out, row * ldo + col, col, k, vec, v);
   }
 }
@@ -545,10 +581,8 @@ struct ActBackward {
   const void* dy;
   int64_t lddy;
   int vec_dy;
-  const void* z;  // 16-bit z, or null: 8-bit codes, or none
-  int64_t ldz;
-  int vec_z;
-  const int8_t* zq;
+  const void* zq;  // kept z: codes [m][n32] of zbits and scales [n32 / 32][m]
+  int zbits;
   const float* zs;
   int64_t n32;
   void* dz;       // null: sums only
@@ -578,15 +612,17 @@ __global__ void __launch_bounds__(256) act_backward_kernel(const ActBackward p) 
         load_piece8<DT>(p.dy, row * p.lddy + col, col, p.n, p.vec_dy, d);
         if constexpr (K != kActNone) {
           float z[8];
-          if (p.zq) {
-            const uint2 c = *reinterpret_cast<const uint2*>(p.zq + row * p.n32 + col);
-            const float s = p.zs[(col / kGroup) * p.m + row];
+          const float s = p.zs[(col / kGroup) * p.m + row];
+          if (p.zbits == 8) {
+            const uint2 c = *reinterpret_cast<const uint2*>(static_cast<const int8_t*>(p.zq) + row * p.n32 + col);
             const uint32_t w[2] = {c.x, c.y};
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
-              z[j] = s * static_cast<float>(static_cast<int8_t>(w[j >> 2] >> (8 * (j & 3))));
+            for (int j = 0; j < 8; ++j) z[j] = s * code8_value(w[j >> 2], j & 3);
           } else {
-            load_piece8<DT>(p.z, row * p.ldz + col, col, p.n, p.vec_z, z);
+            const uint4 c = *reinterpret_cast<const uint4*>(static_cast<const int16_t*>(p.zq) + row * p.n32 + col);
+            const uint32_t w[4] = {c.x, c.y, c.z, c.w};
+#pragma unroll
+            for (int j = 0; j < 8; ++j) z[j] = s * code16_value(w[j >> 1], j & 1);
           }
 #pragma unroll
           for (int j = 0; j < 8; ++j) {

@@ -18,7 +18,7 @@
 //
 // Epilogues (all arithmetic in fp32, one rounding when a value is stored):
 //   kEpiLinear    y = act(D + bias) + residual; optionally z = D + bias is
-//                 kept for the backward pass (16 bits, or 8 bits per group)
+//                 kept for the backward pass (groups of 32 in 16 or 8 bits)
 //   kEpiGated     B holds gate rows [0, n) and up rows [n, 2n); the tile takes
 //                 tn/2 of each, so a thread has both factors of
 //                 h = act(min(g, L)) * clamp(u, -L, L) in its registers
@@ -72,9 +72,9 @@ struct F16GemmParams {
   float limit;            // infinity where there is none
   const void* bias;
   F16Mat residual, out;   // out: y, h (kEpiGatedBwd: h, or null)
-  F16Mat z0, z1;          // kept z (kEpiLinear: z0), or g and u; written forward, read backward
   F16Mat d0, d1;          // kEpiGatedBwd: dg and du
-  int8_t* zq;             // 8-bit kept values: codes [m][halves * n32] ...
+  void* zq;               // kept z, or g and u: codes of zbits [m][halves * n32] ...
+  int zbits;              // 0 (none), 8 or 16
   float* zs;              // ... and scales [halves * n32 / 32][m]
   int64_t n32;            // n rounded up to the group
 };
@@ -323,9 +323,43 @@ __device__ __forceinline__ void codes_to_rows(uint32_t slice, int lane, const ui
 #pragma unroll
     for (int j = 0; j < 16; ++j)
       x[16 * half + j] =
-          scale * static_cast<float>(static_cast<int8_t>(w[j >> 2] >> (8 * (j & 3))));
+          scale * code8_value(w[j >> 2], j & 3);
   }
   __syncwarp();
+}
+
+// A warp's 32 rows of one kept group, columns `at`.. of code rows of `ld`.
+__device__ __forceinline__ void keep_rows(const F16GemmParams& p, uint32_t slice, int lane,
+                                          const float (&v)[32], int64_t ld, int row0, int at) {
+  float s;
+  if (p.zbits == 8) {
+    uint32_t q[8];
+    s = keep_group8(v, q);
+    codes_store(slice, lane, q, static_cast<int8_t*>(p.zq), ld, row0, p.m, at);
+  } else {
+    uint32_t q[16];
+    s = keep_group16(v, p.limit, p.act == kActRelu, q);
+    chunk_store(slice, lane, q, F16Mat{p.zq, ld, 1}, row0, p.m, at, static_cast<int>(ld));
+  }
+  if (row0 + lane < p.m) p.zs[static_cast<int64_t>(at >> 5) * p.m + row0 + lane] = s;
+}
+
+__device__ __forceinline__ void kept_rows(const F16GemmParams& p, uint32_t slice, int lane,
+                                          float (&v)[32], int64_t ld, int row0, int at) {
+  float s = 0.f;
+  if (row0 + lane < p.m) s = p.zs[static_cast<int64_t>(at >> 5) * p.m + row0 + lane];
+  if (p.zbits == 8) {
+    uint4 c[2];
+    codes_fetch(c, static_cast<const int8_t*>(p.zq), ld, lane, row0, p.m, at);
+    codes_to_rows(slice, lane, c, s, v);
+  } else {
+    uint4 r[4];
+    uint32_t w[16];
+    chunk_fetch(r, F16Mat{p.zq, ld, 1}, lane, row0, p.m, at, static_cast<int>(ld));
+    chunk_to_rows(slice, lane, r, true, w);
+#pragma unroll
+    for (int j = 0; j < 32; ++j) v[j] = s * code16_value(w[j >> 1], j & 1);
+  }
 }
 
 template <int EPI, bool BF16>
@@ -469,14 +503,12 @@ __global__ void __launch_bounds__(kF16Threads, 1)
     const uint32_t slice0 = epi_smem + (warp - 4) * 2 * kF16StageSlice;
     const uint32_t slice1 = slice0 + kF16StageSlice;
     const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
-    const bool limited = p.limit < CUDART_INF_F;
     uint32_t nt = 0;
     for (int t = pair; t < tiles; t += pairs, ++nt) {
       int tm, tc;
       tile_at(t, tm, tc);
       const uint32_t buf = nt & 1, use = nt >> 1;
       const int row0 = tm * 256 + static_cast<int>(rank) * 128 + quarter * 32;
-      const int row = row0 + lane;
       if (!mbar_wait_cl(acc_full(buf), use & 1, kErrF16WaitAccFull)) break;
       tc_fence_after();
       const uint32_t acc = tmem + buf * 256 + lanes;
@@ -496,19 +528,13 @@ __global__ void __launch_bounds__(kF16Threads, 1)
             for (int j = 0; j < 32; ++j) v[j] += __shfl_sync(0xffffffffu, bl, j);
           }
           uint32_t w[16];
-          if (p.z0.p) {
-            pack_row<BF16>(v, w);
-            chunk_store(slice0, lane, w, p.z0, row0, p.m, col, p.n);
-          } else if (p.zq) {
+          if (p.zbits) {
             if (col + 32 > p.n) {
 #pragma unroll
               for (int j = 0; j < 32; ++j)
                 if (col + j >= p.n) v[j] = 0.f;
             }
-            uint32_t q[8];
-            const float s = quantize_group(v, q);
-            codes_store(slice0, lane, q, p.zq, p.n32, row0, p.m, col);
-            if (row < p.m) p.zs[static_cast<int64_t>(col >> 5) * p.m + row] = s;
+            keep_rows(p, slice0, lane, v, p.n32, row0, col);
           }
           act_row(p.act, v);
           if (p.residual.p) {
@@ -523,34 +549,14 @@ __global__ void __launch_bounds__(kF16Threads, 1)
           tmem_ld_f32x32(acc + c0, g);
           tmem_ld_f32x32(acc + half_n + c0, u);
           uint32_t w[16];
-          if (p.z0.p) {
-            if (limited) {
-              pack_row_sided<BF16>(g, w, p.limit);
-            } else {
-              pack_row<BF16>(g, w);
-            }
-            chunk_store(slice0, lane, w, p.z0, row0, p.m, col, p.n);
-            if (limited) {
-              pack_row_sided<BF16>(u, w, p.limit);
-            } else {
-              pack_row<BF16>(u, w);
-            }
-            chunk_store(slice1, lane, w, p.z1, row0, p.m, col, p.n);
-          } else if (p.zq) {
+          if (p.zbits) {
             if (col + 32 > p.n) {
 #pragma unroll
               for (int j = 0; j < 32; ++j)
                 if (col + j >= p.n) g[j] = u[j] = 0.f;
             }
-            uint32_t q[8];
-            const float sg = quantize_group(g, q);
-            codes_store(slice0, lane, q, p.zq, 2 * p.n32, row0, p.m, col);
-            const float su = quantize_group(u, q);
-            codes_store(slice1, lane, q, p.zq, 2 * p.n32, row0, p.m, p.n32 + col);
-            if (row < p.m) {
-              p.zs[static_cast<int64_t>(col >> 5) * p.m + row] = sg;
-              p.zs[((p.n32 + col) >> 5) * p.m + row] = su;
-            }
+            keep_rows(p, slice0, lane, g, 2 * p.n32, row0, col);
+            keep_rows(p, slice1, lane, u, 2 * p.n32, row0, static_cast<int>(p.n32) + col);
           }
 #pragma unroll
           for (int j = 0; j < 32; ++j) {
@@ -564,29 +570,8 @@ __global__ void __launch_bounds__(kF16Threads, 1)
           chunk_store(slice0, lane, w, p.out, row0, p.m, col, p.n);
         } else {
           float g[32], u[32];
-          if (p.zq) {
-            uint4 cg[2], cu[2];
-            codes_fetch(cg, p.zq, 2 * p.n32, lane, row0, p.m, col);
-            codes_fetch(cu, p.zq, 2 * p.n32, lane, row0, p.m, p.n32 + col);
-            float sg = 0.f, su = 0.f;
-            if (row < p.m) {
-              sg = p.zs[static_cast<int64_t>(col >> 5) * p.m + row];
-              su = p.zs[((p.n32 + col) >> 5) * p.m + row];
-            }
-            codes_to_rows(slice0, lane, cg, sg, g);
-            codes_to_rows(slice1, lane, cu, su, u);
-          } else {
-            uint4 rg[4], ru[4];
-            chunk_fetch(rg, p.z0, lane, row0, p.m, col, p.n);
-            chunk_fetch(ru, p.z1, lane, row0, p.m, col, p.n);
-            uint32_t w[16];
-            chunk_to_rows(slice0, lane, rg, chunk_whole(p.z0, col, p.n), w);
-#pragma unroll
-            for (int j = 0; j < 32; ++j) g[j] = unpack_16<BF16>(w[j >> 1], j & 1);
-            chunk_to_rows(slice1, lane, ru, chunk_whole(p.z1, col, p.n), w);
-#pragma unroll
-            for (int j = 0; j < 32; ++j) u[j] = unpack_16<BF16>(w[j >> 1], j & 1);
-          }
+          kept_rows(p, slice0, lane, g, 2 * p.n32, row0, col);
+          kept_rows(p, slice1, lane, u, 2 * p.n32, row0, static_cast<int>(p.n32) + col);
           float v[32];
           tmem_ld_f32x32(acc + c0, v);
           uint32_t w[16], wu[16], wh[16];

@@ -76,19 +76,17 @@ SIGNATURES: dict[str, list] = {
     "dsv4_b200_mxfp4_int8_dense_gemm_noalloc": [_P, _P, _I64, _I64, _P, _P, _I64, _P, _I64, _P,
                                                 _P],
     "dsv4_b200_dense_gemm": [_P, _I64, _I, _P, _I64, _I, _I64, _I64, _I64, _I, _P, _I, _P, _I64, _P,
-                             _I64, _P, _I64, _P, _P, _P],
+                             _I64, _P, _I, _P, _P],
     "dsv4_b200_gated_gemm": [_P, _I64, _I, _P, _I64, _I, _I64, _I64, _I64, _I, _I, _I, _F, _P, _I64,
-                             _P, _I64, _P, _P, _P],
+                             _P, _I, _P, _P],
     "dsv4_b200_gated_feed_forward": [_P, _I64, _I, _P, _I64, _I, _P, _I64, _I, _I64, _I64, _I64, _I64,
-                                     _I, _I, _I, _F, _P, _I64, _P, _I64, _P, _I64, _P, _I64, _P, _P,
-                                     _P],
+                                     _I, _I, _I, _F, _P, _I64, _P, _I64, _P, _I64, _P, _I, _P, _P],
     "dsv4_b200_gated_backward_gemm": [_P, _I64, _I, _P, _I64, _I, _I64, _I64, _I64, _I, _I, _I, _F,
-                                      _P, _I64, _P, _P, _P, _I64, _P, _I64, _P],
+                                      _P, _I, _P, _P, _I64, _P, _I64, _P],
     "dsv4_b200_checkpoint_int8": [_P, _I, _I64, _I64, _I64, _P, _P, _P],
     "dsv4_b200_restore_int8": [_P, _P, _I64, _I64, _P, _I, _I64, _P],
     "dsv4_b200_act_backward_slabs": [_I64, _I64, _P],
-    "dsv4_b200_act_backward": [_P, _I64, _P, _I64, _P, _P, _I64, _I64, _I, _I, _P, _I64, _P, _I64,
-                               _P, _P],
+    "dsv4_b200_act_backward": [_P, _I64, _P, _I, _P, _I64, _I64, _I, _I, _P, _I64, _P, _I64, _P, _P],
     "dsv4_b200_pack_rows": [_P, _I64, _I64, _I64, _I64, _P, _I64, _P],
 }
 _RESTYPES = {"dsv4_b200_last_error": ctypes.c_char_p}

@@ -7,7 +7,8 @@ projections), forward and backward.
     checkpoint_int8 / restore_int8    activations kept in 8 bits
 
 bf16 and fp16; sums, activations and their slopes in fp32, one rounding where
-a value is stored.  ``dense_forward`` and ``gated_feed_forward`` are
+a value is stored.  The values before an activation are kept for the backward
+pass as groups of 32 with a shared scale, in 16 bits.  ``dense_forward`` and ``gated_feed_forward`` are
 differentiable; their ``*_save`` / ``*_backward`` forms give the same steps
 without autograd (and are the ones to capture into a CUDA graph).  With
 ``checkpoint="int8"`` what the backward pass needs is kept in 8 bits.  Every
@@ -160,7 +161,7 @@ def _row_stride(t: torch.Tensor) -> int:
 def _product(a, a_mn, b, b_mn, m, n, k, dtype, out, stream) -> None:
     """out = a @ b.T of operands; a_mn, b_mn: how this product reads them."""
     _call("dense_gemm", a[1], a[2], a_mn, b[1], b[2], b_mn, m, n, k, dtype, None, 0, None, 0,
-          out.data_ptr(), _row_stride(out), None, 0, None, None, stream)
+          out.data_ptr(), _row_stride(out), None, 0, None, stream)
 
 
 # ---- 8-bit checkpoints ----
@@ -179,9 +180,9 @@ class Int8Checkpoint:
     dtype: torch.dtype
 
 
-def _empty_codes(rows: int, cols: int, like: torch.Tensor):
+def _empty_codes(rows: int, cols: int, like: torch.Tensor, dtype=torch.int8):
     k32 = _up(cols, _GROUP)
-    return (like.new_empty((rows, k32), dtype=torch.int8),
+    return (like.new_empty((rows, k32), dtype=dtype),
             like.new_empty((k32 // _GROUP, rows), dtype=torch.float32))
 
 
@@ -247,14 +248,17 @@ def _kept_operand(kept, m, k, like):
     return _operand(_restore(*kept, _rows_buffer(m, k, like)))
 
 
-# z as the kernels take it: (address, stride, codes' address, scales' address).
+# The values before an activation, kept as groups of 32 in 16 or 8 bits:
+# (codes, scales), or ().  As the kernels take them: codes, bits, scales.
+
+def _empty_kept(rows, cols, like, checkpoint):
+    return _empty_codes(rows, cols, like, torch.int16 if checkpoint is None else torch.int8)
+
 
 def _z_args(kept):
     if not kept:
-        return None, 0, None, None
-    if len(kept) == 1:
-        return kept[0].data_ptr(), kept[0].stride(0), None, None
-    return None, 0, kept[0].data_ptr(), kept[1].data_ptr()
+        return None, 0, None
+    return kept[0].data_ptr(), 8 * kept[0].element_size(), kept[1].data_ptr()
 
 
 # ---- dense product ----
@@ -264,7 +268,7 @@ class SavedDense:
     """What :func:`dense_backward` needs of a :func:`dense_forward_save` call."""
     x: tuple
     weight: torch.Tensor
-    z: tuple  # (z,), (codes, scales), or () without an activation
+    z: tuple  # (codes, scales), or () without an activation
     activation: Optional[str]
     shape: tuple
     has_bias: bool
@@ -308,7 +312,7 @@ def _dense(x, weight, bias, activation, residual, m, n, k, checkpoint=None, keep
     if keep_x and checkpoint is not None:
         xk = _checkpoint(x)
     if keep_z:
-        zk = (_rows_buffer(m, n, x),) if checkpoint is None else _empty_codes(m, n, x)
+        zk = _empty_kept(m, n, x, checkpoint)
     if m == 0:
         return out, xk or (x,), weight, zk
     a, b = _operand(x), _operand(weight)
@@ -454,7 +458,7 @@ class SavedFeedForward:
     x: tuple
     w13: torch.Tensor
     w2: torch.Tensor
-    z: tuple  # (z,) [M, 2I] (halves padded to 8), or 8-bit (codes, scales)
+    z: tuple  # gate and up: (codes, scales)
     h: Optional[torch.Tensor]  # the gated product; formed again from z when kept in 8 bits
     activation: Optional[str]
     clamp_limit: Optional[float]
@@ -502,10 +506,8 @@ def _ffn(x, w13, w2, activation, clamp_limit, residual, m, hidden, inter, n, che
     xk = zk = ()
     if keep_x and checkpoint is not None:
         xk = _checkpoint(x)
-    if keep_z and checkpoint is None:
-        zk = (x.new_empty((m, 2 * _up(inter, 8))),)
-    elif keep_z:
-        zk = _empty_codes(m, 2 * _up(inter, _GROUP), x)
+    if keep_z:
+        zk = _empty_kept(m, 2 * _up(inter, _GROUP), x, checkpoint)
     if m == 0:
         return out, xk or (x,), w13, w2, zk, h
     # w13 stored by columns: its up rows begin `inter` elements into a row

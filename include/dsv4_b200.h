@@ -392,12 +392,12 @@ DSV4_API int dsv4_b200_mxfp4_int8_dense_gemm_noalloc(const int8_t* a_q, const fl
  * means rows of the contraction axis ([rows][k]), 1 the transposed storage
  * ([k][rows]).  dsv4_b200_pack_rows lays out an operand of any strides.
  * Results and `residual` have any alignment.  activation: dsv4_activation.
- * 8-bit kept values: int8 codes [m][ceil32(k)] and fp32 scales
- * [ceil32(k) / 32][m]: groups of 32 values of a row share a scale amax / 127
- * (rounded toward zero);
- * code = 127 v / amax rounded to nearest even; a group with an infinity or a
- * NaN decodes to NaN, one whose amax is below 2^-100 to zeros.  Codes and
- * scales of gate and up lie behind each other (ceil32(intermediate) each). */
+ * Kept values are groups of 32 values of a row that share an fp32 scale
+ * amax / steps (rounded toward zero), steps 127 in 8 bits and 32767 in 16:
+ * codes int8 or int16 [m][ceil32(k)], scales [ceil32(k) / 32][m], codes 16-byte
+ * aligned.  code = steps v / amax to the nearest, ties to even; a group with
+ * an infinity or a NaN decodes to NaN, one whose amax is below 2^-100 to zeros.
+ * z_bits = 0, 8 or 16 (0: z_codes and z_scales NULL). */
 typedef enum dsv4_activation {
   DSV4_ACT_NONE = 0,
   DSV4_ACT_RELU = 1,
@@ -408,23 +408,24 @@ typedef enum dsv4_activation {
 
 /* out[m][n] = act(a b^T + bias) + residual; bias [n] and residual may be NULL;
  * ldr = 0 adds the same row everywhere.
- * z (or z_codes + z_scales) receives a b^T + bias for the backward pass. */
+ * z_codes and z_scales receive a b^T + bias for the backward pass (in 16 bits
+ * and for relu, values other than zero keep their sign). */
 DSV4_API int dsv4_b200_dense_gemm(const void* a, int64_t lda, int a_mn, const void* b, int64_t ldb,
                                   int b_mn, int64_t m, int64_t n, int64_t k, int dtype,
                                   const void* bias, int activation, const void* residual,
-                                  int64_t ldr, void* out, int64_t ldo, void* z, int64_t ldz,
-                                  int8_t* z_codes, float* z_scales, void* stream);
+                                  int64_t ldr, void* out, int64_t ldo, void* z_codes, int z_bits,
+                                  float* z_scales, void* stream);
 
 /* h[m][intermediate] = act(min(g, L)) * clamp(u, -L, L), g and u the products
  * of x with rows [0, intermediate) and [intermediate, 2 intermediate) of w13.
- * z (or its codes) receives g and u before the clamp: row r of g at z + r ldz,
- * of u ceil8(intermediate) elements behind it.
+ * z_codes [m][2 ceil32(intermediate)] and z_scales receive g and then u before
+ * the clamp (in 16 bits on the same side of the limit as the sums).
  * w_mn = 1 needs intermediate % 8 == 0. */
 DSV4_API int dsv4_b200_gated_gemm(const void* x, int64_t ldx, int x_mn, const void* w13, int64_t ldw,
                                   int w_mn, int64_t m, int64_t intermediate, int64_t k, int dtype,
                                   int activation, int has_clamp, float clamp_limit, void* h,
-                                  int64_t ldh, void* z, int64_t ldz, int8_t* z_codes,
-                                  float* z_scales, void* stream);
+                                  int64_t ldh, void* z_codes, int z_bits, float* z_scales,
+                                  void* stream);
 
 /* The whole block, y = h w2^T + residual: dsv4_b200_gated_gemm into h, then
  * dsv4_b200_dense_gemm (w2 [out_cols][intermediate]).  h is a workspace that
@@ -433,8 +434,8 @@ DSV4_API int dsv4_b200_gated_feed_forward(
     const void* x, int64_t ldx, int x_mn, const void* w13, int64_t ldw13, int w13_mn, const void* w2,
     int64_t ldw2, int w2_mn, int64_t m, int64_t hidden, int64_t intermediate, int64_t out_cols,
     int dtype, int activation, int has_clamp, float clamp_limit, const void* residual, int64_t ldr,
-    void* h, int64_t ldh, void* out, int64_t ldo, void* z, int64_t ldz, int8_t* z_codes,
-    float* z_scales, void* stream);
+    void* h, int64_t ldh, void* out, int64_t ldo, void* z_codes, int z_bits, float* z_scales,
+    void* stream);
 
 /* Backward of the gate: dh = dy w2 (w2 [k][intermediate], or with w_mn = 0 its
  * transpose) stays in registers; dz [m][2 intermediate] = the gradients of g
@@ -442,8 +443,8 @@ DSV4_API int dsv4_b200_gated_feed_forward(
 DSV4_API int dsv4_b200_gated_backward_gemm(const void* dy, int64_t lddy, int dy_mn, const void* w2,
                                            int64_t ldw, int w_mn, int64_t m, int64_t intermediate,
                                            int64_t k, int dtype, int activation, int has_clamp,
-                                           float clamp_limit, const void* z, int64_t ldz,
-                                           const int8_t* z_codes, const float* z_scales, void* dz,
+                                           float clamp_limit, const void* z_codes, int z_bits,
+                                           const float* z_scales, void* dz,
                                            int64_t lddz, void* h, int64_t ldh, void* stream);
 
 /* Activations in 8 bits: x [m][k] fp32 / fp16 / bf16 -> codes, scales; and back. */
@@ -456,8 +457,8 @@ DSV4_API int dsv4_b200_restore_int8(const int8_t* codes, const float* scales, in
  * DSV4_ACT_NONE dz = dy is not written).  partial: fp32 [slabs][n], at least
  * the number of slabs that dsv4_b200_act_backward_slabs reports. */
 DSV4_API int dsv4_b200_act_backward_slabs(int64_t m, int64_t n, int64_t* slabs);
-DSV4_API int dsv4_b200_act_backward(const void* dy, int64_t lddy, const void* z, int64_t ldz,
-                                    const int8_t* z_codes, const float* z_scales, int64_t m,
+DSV4_API int dsv4_b200_act_backward(const void* dy, int64_t lddy, const void* z_codes,
+                                    int z_bits, const float* z_scales, int64_t m,
                                     int64_t n, int dtype, int activation, void* dz, int64_t lddz,
                                     float* partial, int64_t slabs, void* dbias, void* stream);
 

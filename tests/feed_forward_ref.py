@@ -88,11 +88,15 @@ def tiny_of(dtype):
     return torch.finfo(dtype).tiny * torch.finfo(dtype).eps / 2
 
 
-def kept(z, mode, h16, tiny, sided=None):
-    """z as the backward pass reads it."""
+def kept(z, mode):
+    """z as the backward pass reads it: groups of 32, off by half a step of
+    amax / 32767, or a whole one to stay on its side of a limit or of zero; or
+    in 8 bits."""
     if mode is None:
-        full = 2 if sided is not None else 1
-        return Bounded(z.v, z.e + full * h16 * (z.v.abs() + z.e) + tiny)
+        k = z.v.shape[1]
+        top = torch.nn.functional.pad(z.v.abs() + z.e, (0, -k % GROUP)).reshape(z.v.shape[0], -1, GROUP)
+        top = top.amax(2, keepdim=True).expand_as(top).reshape(z.v.shape[0], -1)[:, :k]
+        return Bounded(z.v, z.e + 1.001 * top / 32767)
     back, step, edge = eight(z.v)
     # the largest value of a group may be off as well: the step with it
     top_e = torch.nn.functional.pad(z.e, (0, -z.e.shape[1] % GROUP)).reshape(z.e.shape[0], -1, GROUP)
@@ -138,8 +142,11 @@ def dense(x, w, bias, residual, kind, dtype, dy=None, mode=None):
         return out
     dz = Bounded(dy.double())
     if kind is not None:
-        dz = rounded(times(dz, slope_bounded(kind, kept(z, mode, h16, tiny))), h16, tiny)
-        unrounded = times(Bounded(dy.double()), slope_bounded(kind, kept(z, mode, h16, tiny)))
+        zk = kept(z, mode)
+        if kind == "relu" and mode is None:
+            zk = z  # kept with its sign
+        unrounded = times(dz, slope_bounded(kind, zk))
+        dz = rounded(unrounded, h16, tiny)
     else:
         unrounded = dz
     xk = X if mode is None else rounded(Bounded(eight(X.v)[0]), 2 * h16, tiny)
@@ -160,9 +167,10 @@ def ffn(x, w13, w2, residual, kind, limit, dtype, dy=None, mode=None):
     z = product(X, W13)
     g, u = Bounded(z.v[:, :inter], z.e[:, :inter]), Bounded(z.v[:, inter:], z.e[:, inter:])
 
-    def gate(g, u):
+    def gate(g, u, sign_e=None):
         gc, uc = Bounded(g.v.clamp(max=lim), g.e), Bounded(u.v.clamp(-lim, lim), u.e)
-        return act_bounded(kind, gc), slope_bounded(kind, gc), uc
+        gs = gc if sign_e is None else Bounded(gc.v, sign_e)
+        return act_bounded(kind, gc), slope_bounded(kind, gs), uc
 
     a, _, uc = gate(g, u)
     h = rounded(times(a, uc), h16, tiny)
@@ -173,9 +181,9 @@ def ffn(x, w13, w2, residual, kind, limit, dtype, dy=None, mode=None):
     out = {"y": rounded(y, h16, tiny)}
     if dy is None:
         return out
-    sided = None if limit is None else lim
-    gk, uk = kept(g, mode, h16, tiny, sided), kept(u, mode, h16, tiny, sided)
-    a, s, uc = gate(gk, uk)
+    gk, uk = kept(g, mode), kept(u, mode)
+    # relu keeps the sign: its slope is as sure as the sum itself
+    a, s, uc = gate(gk, uk, g.e if kind == "relu" and mode is None else None)
     DY = Bounded(dy.double())
     dh = product(DY, Bounded(W2.v.T))
 
