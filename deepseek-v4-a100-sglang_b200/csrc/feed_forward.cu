@@ -428,7 +428,11 @@ int dsv4_b200_gated_feed_forward(const void* x, int64_t ldx, int x_mn, const voi
                                  int activation, int has_clamp, float clamp_limit,
                                  const void* residual, int64_t ldr, void* h, int64_t ldh, void* out,
                                  int64_t ldo, void* z_codes, int z_bits, float* z_scales,
-                                 void* stream) {
+                                 int8_t* x_codes, float* x_scales, void* stream) {
+  if (x_codes != nullptr) {
+    DSV4_REQUIRE(!x_mn, "x is kept in 8 bits by rows");
+    if (int r = dsv4_b200_checkpoint_int8(x, dtype, m, hidden, ldx, x_codes, x_scales, stream)) return r;
+  }
   if (int r = dsv4_b200_gated_gemm(x, ldx, x_mn, w13, ldw13, w13_mn, m, intermediate, hidden, dtype,
                                    activation, has_clamp, clamp_limit, h, ldh, z_codes, z_bits,
                                    z_scales, stream))
@@ -559,6 +563,79 @@ int dsv4_b200_act_backward(const void* dy, int64_t lddy, const void* z_codes, in
     else launch_pdl(&column_sum_kernel<false>, sum_grid, dim3(128), 0, st, partial, need, n, dbias);
     return check_launch("column_sum_kernel");
   }
+  return DSV4_OK;
+}
+
+// dW = d^T x, with x as it is or restored from its 8-bit codes first.
+static int weight_gradient(const void* d, int64_t ldd, int d_mn, const void* x, int64_t ldx, int x_mn,
+                           const int8_t* x_codes, const float* x_scales, void* x_restored,
+                           int64_t ldxr, int64_t rows, int64_t cols, int64_t m, int dtype, void* dw,
+                           void* stream) {
+  if (x_codes != nullptr) {
+    if (int r = dsv4_b200_restore_int8(x_codes, x_scales, m, cols, x_restored, dtype, ldxr, stream))
+      return r;
+    x = x_restored, ldx = ldxr, x_mn = 0;
+  }
+  return dsv4_b200_dense_gemm(d, ldd, !d_mn, x, ldx, !x_mn, rows, cols, m, dtype, nullptr,
+                              DSV4_ACT_NONE, nullptr, 0, dw, cols, nullptr, 0, nullptr, stream);
+}
+
+int dsv4_b200_gated_feed_forward_backward(
+    const void* dy, int64_t lddy, int dy_mn, const void* x, int64_t ldx, int x_mn,
+    const int8_t* x_codes, const float* x_scales, void* x_restored, int64_t ldxr, const void* w13,
+    int64_t ldw13, int w13_mn, const void* w2, int64_t ldw2, int w2_mn, int64_t m, int64_t hidden,
+    int64_t intermediate, int64_t out_cols, int dtype, int activation, int has_clamp,
+    float clamp_limit, const void* z_codes, int z_bits, const float* z_scales, void* h, int64_t ldh,
+    int form_h, void* dz, int64_t lddz, void* dx, void* dw13, void* dw2, void* stream) {
+  if (m == 0) return DSV4_OK;
+  if (dx != nullptr || dw13 != nullptr || (dw2 != nullptr && form_h)) {
+    if (int r = dsv4_b200_gated_backward_gemm(dy, lddy, dy_mn, w2, ldw2, !w2_mn, m, intermediate,
+                                              out_cols, dtype, activation, has_clamp, clamp_limit,
+                                              z_codes, z_bits, z_scales, dz, lddz,
+                                              form_h ? h : nullptr, ldh, stream))
+      return r;
+  }
+  if (dw2 != nullptr) {
+    if (int r = dsv4_b200_dense_gemm(dy, lddy, !dy_mn, h, ldh, 1, out_cols, intermediate, m, dtype,
+                                     nullptr, DSV4_ACT_NONE, nullptr, 0, dw2, intermediate, nullptr, 0,
+                                     nullptr, stream))
+      return r;
+  }
+  if (dx != nullptr) {
+    if (int r = dsv4_b200_dense_gemm(dz, lddz, 0, w13, ldw13, !w13_mn, m, hidden, 2 * intermediate,
+                                     dtype, nullptr, DSV4_ACT_NONE, nullptr, 0, dx, hidden, nullptr, 0,
+                                     nullptr, stream))
+      return r;
+  }
+  if (dw13 != nullptr)
+    return weight_gradient(dz, lddz, 0, x, ldx, x_mn, x_codes, x_scales, x_restored, ldxr,
+                           2 * intermediate, hidden, m, dtype, dw13, stream);
+  return DSV4_OK;
+}
+
+int dsv4_b200_dense_backward(const void* dy, int64_t lddy, const void* d, int64_t ldd, int d_mn,
+                             const void* x, int64_t ldx, int x_mn, const int8_t* x_codes,
+                             const float* x_scales, void* x_restored, int64_t ldxr, const void* w,
+                             int64_t ldw, int w_mn, int64_t m, int64_t n, int64_t k, int dtype,
+                             int activation, const void* z_codes, int z_bits, const float* z_scales,
+                             float* partial, int64_t slabs, void* dx, void* dw, void* dbias,
+                             void* stream) {
+  if (m == 0) return DSV4_OK;
+  if (activation != DSV4_ACT_NONE || dbias != nullptr) {
+    DSV4_REQUIRE(activation == DSV4_ACT_NONE || !d_mn, "dz is written by rows");
+    if (int r = dsv4_b200_act_backward(dy, lddy, z_codes, z_bits, z_scales, m, n, dtype, activation,
+                                       activation == DSV4_ACT_NONE ? nullptr : const_cast<void*>(d),
+                                       ldd, partial, slabs, dbias, stream))
+      return r;
+  }
+  if (dx != nullptr) {
+    if (int r = dsv4_b200_dense_gemm(d, ldd, d_mn, w, ldw, !w_mn, m, k, n, dtype, nullptr,
+                                     DSV4_ACT_NONE, nullptr, 0, dx, k, nullptr, 0, nullptr, stream))
+      return r;
+  }
+  if (dw != nullptr)
+    return weight_gradient(d, ldd, d_mn, x, ldx, x_mn, x_codes, x_scales, x_restored, ldxr, n, k, m,
+                           dtype, dw, stream);
   return DSV4_OK;
 }
 

@@ -80,7 +80,13 @@ SIGNATURES: dict[str, list] = {
     "dsv4_b200_gated_gemm": [_P, _I64, _I, _P, _I64, _I, _I64, _I64, _I64, _I, _I, _I, _F, _P, _I64,
                              _P, _I, _P, _P],
     "dsv4_b200_gated_feed_forward": [_P, _I64, _I, _P, _I64, _I, _P, _I64, _I, _I64, _I64, _I64, _I64,
-                                     _I, _I, _I, _F, _P, _I64, _P, _I64, _P, _I64, _P, _I, _P, _P],
+                                     _I, _I, _I, _F, _P, _I64, _P, _I64, _P, _I64, _P, _I, _P, _P,
+                                     _P, _P],
+    "dsv4_b200_gated_feed_forward_backward": [
+        _P, _I64, _I, _P, _I64, _I, _P, _P, _P, _I64, _P, _I64, _I, _P, _I64, _I, _I64, _I64, _I64, _I64,
+        _I, _I, _I, _F, _P, _I, _P, _P, _I64, _I, _P, _I64, _P, _P, _P, _P],
+    "dsv4_b200_dense_backward": [_P, _I64, _P, _I64, _I, _P, _I64, _I, _P, _P, _P, _I64, _P, _I64, _I,
+                                 _I64, _I64, _I64, _I, _I, _P, _I, _P, _P, _I64, _P, _P, _P, _P],
     "dsv4_b200_gated_backward_gemm": [_P, _I64, _I, _P, _I64, _I, _I64, _I64, _I64, _I, _I, _I, _F,
                                       _P, _I, _P, _P, _I64, _P, _I64, _P],
     "dsv4_b200_checkpoint_int8": [_P, _I, _I64, _I64, _I64, _P, _P, _P],

@@ -154,14 +154,34 @@ def _plain_rows(t: torch.Tensor) -> torch.Tensor:
     return t.contiguous()
 
 
+def _distinct_rows(t: torch.Tensor) -> torch.Tensor:
+    """:func:`_plain_rows` without a row stride of 0."""
+    t = _plain_rows(t)
+    return t.contiguous() if t.shape[0] > 1 and t.stride(0) == 0 else t
+
+
 def _row_stride(t: torch.Tensor) -> int:
     return t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
 
-def _product(a, a_mn, b, b_mn, m, n, k, dtype, out, stream) -> None:
-    """out = a @ b.T of operands; a_mn, b_mn: how this product reads them."""
-    _call("dense_gemm", a[1], a[2], a_mn, b[1], b[2], b_mn, m, n, k, dtype, None, 0, None, 0,
-          out.data_ptr(), _row_stride(out), None, 0, None, stream)
+# ---- what a training step keeps, and the backward pass's workspace ----
+# One allocation each: parts at multiples of 256 bytes, passed by address.
+
+def _parts(like: torch.Tensor, *sizes):
+    """A buffer of bytes and the addresses of parts of these sizes (None: none)."""
+    total, at = 0, []
+    for size in sizes:
+        at.append(None if size is None else total)
+        total += 0 if size is None else _up(size, 256)
+    buf = like.new_empty(total, dtype=torch.uint8)
+    base = buf.data_ptr()
+    return buf, [None if a is None else base + a for a in at]
+
+
+def _group_bytes(rows: int, cols: int, bits: int):
+    """Bytes of the codes and of the scales of [rows, cols] kept in groups."""
+    k32 = _up(cols, _GROUP)
+    return rows * k32 * bits // 8, rows * (k32 // _GROUP) * 4
 
 
 # ---- 8-bit checkpoints ----
@@ -204,10 +224,8 @@ def checkpoint_int8(x: torch.Tensor) -> Int8Checkpoint:
 
 
 def _checkpoint(x):
-    x = _plain_rows(x.detach())
+    x = _distinct_rows(x.detach())
     m, k = x.shape
-    if m > 1 and x.stride(0) == 0:
-        x = x.contiguous()
     codes, scales = _empty_codes(m, k, x)
     _call("checkpoint_int8", x.data_ptr(), _CHECKPOINT_DTYPES[x.dtype], m, k, _row_stride(x),
           codes.data_ptr(), scales.data_ptr(), _stream(x.get_device()))
@@ -240,38 +258,18 @@ def _restore(codes, scales, out):
     return out
 
 
-# An input as the backward pass gets it back: (x,), or its 8-bit (codes, scales).
-
-def _kept_operand(kept, m, k, like):
-    if len(kept) == 1:
-        return _operand(kept[0])
-    return _operand(_restore(*kept, _rows_buffer(m, k, like)))
-
-
-# The values before an activation, kept as groups of 32 in 16 or 8 bits:
-# (codes, scales), or ().  As the kernels take them: codes, bits, scales.
-
-def _empty_kept(rows, cols, like, checkpoint):
-    return _empty_codes(rows, cols, like, torch.int16 if checkpoint is None else torch.int8)
-
-
-def _z_args(kept):
-    if not kept:
-        return None, 0, None
-    return kept[0].data_ptr(), 8 * kept[0].element_size(), kept[1].data_ptr()
-
-
 # ---- dense product ----
 
 @dataclass
 class SavedDense:
     """What :func:`dense_backward` needs of a :func:`dense_forward_save` call."""
-    x: tuple
+    x: Optional[torch.Tensor]  # None: in 8 bits among `kept`
     weight: torch.Tensor
-    z: tuple  # (codes, scales), or () without an activation
+    kept: torch.Tensor         # the value before the activation, and x in 8 bits
     activation: Optional[str]
     shape: tuple
     has_bias: bool
+    bits: int
 
 
 def _check_dense(x, weight, bias, activation, residual, checkpoint):
@@ -303,28 +301,34 @@ def _check_dense(x, weight, bias, activation, residual, checkpoint):
     raise RuntimeError("unsupported arguments")
 
 
-def _dense(x, weight, bias, activation, residual, m, n, k, checkpoint=None, keep_x=False,
-           keep_z=False):
-    """(y, kept x, weight as laid out, kept z); launches on the current device."""
-    dt, dev = x.dtype, x.get_device()
+def _dense_kept(x, m, n, k, activation, bits, keep_x, keep_z):
+    """(buffer, addresses of z codes, z scales, x codes, x scales)."""
+    z = _group_bytes(m, n, bits) if keep_z and activation is not None else (None, None)
+    xs = _group_bytes(m, k, 8) if keep_x and bits == 8 else (None, None)
+    return _parts(x, *z, *xs)
+
+
+def _dense(x, weight, bias, activation, residual, m, n, k, bits=0, keep_x=False, keep_z=False):
+    """(y, x and weight as laid out, kept buffer); launches on the current device."""
+    dt, st = _DTYPES[x.dtype], _stream(x.get_device())
     out = x.new_empty((m, n))
-    xk = zk = ()
-    if keep_x and checkpoint is not None:
-        xk = _checkpoint(x)
-    if keep_z:
-        zk = _empty_kept(m, n, x, checkpoint)
+    kept, zc, zs = None, None, None
+    if keep_x or keep_z:
+        kept, (zc, zs, xc, xs) = _dense_kept(x, m, n, k, activation, bits, keep_x, keep_z)
     if m == 0:
-        return out, xk or (x,), weight, zk
+        return out, x, weight, kept
     a, b = _operand(x), _operand(weight)
+    if kept is not None and xc is not None:
+        rows = a if a[3] == 0 else _operand(x, False)
+        _call("checkpoint_int8", rows[1], dt, m, k, rows[2], xc, xs, st)
     if bias is not None and bias.stride(0) != 1:
         bias = bias.contiguous()
     r = None if residual is None else _plain_rows(residual)
-    z = _z_args(zk)
-    _call("dense_gemm", a[1], a[2], a[3], b[1], b[2], b[3], m, n, k, _DTYPES[dt],
+    _call("dense_gemm", a[1], a[2], a[3], b[1], b[2], b[3], m, n, k, dt,
           None if bias is None else bias.data_ptr(), ACTIVATIONS[activation],
           None if r is None else r.data_ptr(), 0 if r is None else _row_stride(r), out.data_ptr(), n,
-          *z, _stream(dev))
-    return out, xk or (a[0],), b[0], zk
+          zc, 0 if zc is None else bits, zs, st)
+    return out, a[0], b[0], kept
 
 
 def dense_forward(x, weight, bias=None, *, activation=None, residual=None, checkpoint=None):
@@ -350,10 +354,11 @@ def dense_forward_save(x, weight, bias=None, *, activation=None, residual=None, 
     needs: ``(y, saved)``.  ``saved`` refers to x (unless kept in 8 bits) and
     weight; they must not change before the backward call."""
     m, n, k = _check_dense(x, weight, bias, activation, residual, checkpoint)
+    bits = 16 if checkpoint is None else 8
     with torch.no_grad(), _on(x.get_device()):
-        y, xk, wk, zk = _dense(x, weight, bias, activation, residual, m, n, k, checkpoint, True,
-                               activation is not None)
-    return y, SavedDense(xk, wk, zk, activation, (m, n, k), bias is not None)
+        y, xk, wk, kept = _dense(x, weight, bias, activation, residual, m, n, k, bits, True, True)
+    return y, SavedDense(xk if bits == 16 else None, wk, kept, activation, (m, n, k),
+                         bias is not None, bits)
 
 
 def dense_backward(grad_out, saved: SavedDense, *, need_x=True, need_weight=True, need_bias=True):
@@ -364,39 +369,50 @@ def dense_backward(grad_out, saved: SavedDense, *, need_x=True, need_weight=True
     _explain_matrix(grad_out, "grad_out", m, n, like=saved.weight)
     _explain_device(grad_out, weight=saved.weight)
     with torch.no_grad(), _on(grad_out.get_device()):
-        return _dense_backward(grad_out, saved.x, saved.weight, saved.z, saved.activation, m, n, k,
-                               need_x, need_weight, need_bias and saved.has_bias)
+        return _dense_backward(grad_out, saved.x, saved.weight, saved.kept, True, True,
+                               saved.activation, m, n, k, saved.bits, need_x, need_weight,
+                               need_bias and saved.has_bias)
 
 
-def _dense_backward(dy, xk, weight, zk, activation, m, n, k, need_x, need_weight, need_bias):
+def _addresses(kept, *sizes):
+    """The addresses :func:`_parts` gave for these sizes."""
+    at, out = kept.data_ptr(), []
+    for size in sizes:
+        out.append(None if size is None else at)
+        at += 0 if size is None else _up(size, 256)
+    return out
+
+
+def _dense_backward(dy, x, weight, kept, kept_x, kept_z, activation, m, n, k, bits, need_x, need_weight,
+                    need_bias):
     dt, st = _DTYPES[dy.dtype], _stream(dy.get_device())
     gx = dy.new_empty((m, k)) if need_x else None
     gw = dy.new_empty((n, k)) if need_weight else None
     gb = dy.new_empty((n,)) if need_bias else None
     if m == 0:
         return gx, None if gw is None else gw.zero_(), None if gb is None else gb.zero_()
-    dz = dy
-    if (activation is not None and (need_x or need_weight)) or need_bias:
-        rows = _plain_rows(dy)
-        if m > 1 and rows.stride(0) == 0:
-            rows = rows.contiguous()
-        partial, slabs = None, 0
-        if need_bias:
-            slabs = _slabs(m, n)
-            partial = dy.new_empty((slabs, n), dtype=torch.float32)
-        if activation is not None:
-            dz = _rows_buffer(m, n, dy)
-        _call("act_backward", rows.data_ptr(), _row_stride(rows), *_z_args(zk), m, n, dt,
-              ACTIVATIONS[activation], None if activation is None else dz.data_ptr(),
-              n if activation is None else dz.stride(0), N.ptr(partial), slabs, N.ptr(gb), st)
-    if need_x or need_weight:
-        d = _operand(dz)
-        if need_x:
-            w = _operand(weight)
-            _product(d, d[3], w, 1 - w[3], m, k, n, dt, gx, st)
-        if need_weight:
-            x = _kept_operand(xk, m, k, dy)
-            _product(d, 1 - d[3], x, 1 - x[3], n, k, m, dt, gw, st)
+    if not (need_x or need_weight or need_bias):
+        return None, None, None
+    z = _group_bytes(m, n, bits) if kept_z and activation is not None else (None, None)
+    xs = _group_bytes(m, k, 8) if kept_x and bits == 8 else (None, None)
+    zc, zs, xc, xsc = _addresses(kept, *z, *xs)
+    rows, d = dy, (None, None, 0, 0)
+    if activation is not None or need_bias:
+        rows = _distinct_rows(dy)
+    if activation is None and (need_x or need_weight):
+        d = _operand(dy)
+    slabs = _slabs(m, n) if need_bias else 0
+    ld, ldx = _up(n, 8), _up(k, 8)
+    ws, (dz, partial, xr) = _parts(dy, None if activation is None else m * ld * 2,
+                                   slabs * n * 4 if need_bias else None,
+                                   m * ldx * 2 if need_weight and xc is not None else None)
+    if activation is not None:
+        d = (ws, dz, ld, 0)
+    xo = _operand(x) if need_weight and xc is None else (None, None, 0, 0)
+    w = _operand(weight) if need_x else (None, None, 0, 0)
+    _call("dense_backward", rows.data_ptr(), _row_stride(rows), *d[1:], *xo[1:], xc, xsc, xr, ldx, *w[1:],
+          m, n, k, dt, ACTIVATIONS[activation], zc, 0 if zc is None else bits, zs, partial, slabs,
+          N.ptr(gx), N.ptr(gw), N.ptr(gb), st)
     return gx, gw, gb
 
 
@@ -427,13 +443,12 @@ class _DenseFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, residual, activation, checkpoint, m, n, k):
         need = ctx.needs_input_grad
+        bits = 16 if checkpoint is None else 8
+        keep_z = need[0] or need[1] or need[2]
         with _on(x.get_device()):
-            y, xk, wk, zk = _dense(x, weight, bias, activation, residual, m, n, k, checkpoint,
-                                   need[1], activation is not None and any(need[:3]))
-        if not need[1]:
-            xk = ()
-        ctx.save_for_backward(wk, *xk, *zk)
-        ctx.args = (len(xk), activation, m, n, k)
+            y, xk, wk, kept = _dense(x, weight, bias, activation, residual, m, n, k, bits, need[1], keep_z)
+        ctx.save_for_backward(wk, kept, xk if need[1] and bits == 16 else None)
+        ctx.args = (need[1], keep_z, activation, m, n, k, bits)
         return y
 
     @staticmethod
@@ -441,11 +456,10 @@ class _DenseFunction(torch.autograd.Function):
     def backward(ctx, grad_out):
         need = ctx.needs_input_grad
         gx = gw = gb = None
-        if any(need[:3]):
-            w, *kept = ctx.saved_tensors
-            nx, *args = ctx.args
+        if need[0] or need[1] or need[2]:
+            w, kept, x = ctx.saved_tensors
             with _on(grad_out.get_device()):
-                gx, gw, gb = _dense_backward(grad_out, kept[:nx], w, kept[nx:], *args, *need[:3])
+                gx, gw, gb = _dense_backward(grad_out, x, w, kept, *ctx.args, *need[:3])
         return gx, gw, gb, grad_out if need[3] else None, None, None, None, None, None
 
 
@@ -455,14 +469,14 @@ class _DenseFunction(torch.autograd.Function):
 class SavedFeedForward:
     """What :func:`gated_feed_forward_backward` needs of a
     :func:`gated_feed_forward_save` call."""
-    x: tuple
+    x: Optional[torch.Tensor]  # None: in 8 bits among `kept`
     w13: torch.Tensor
     w2: torch.Tensor
-    z: tuple  # gate and up: (codes, scales)
-    h: Optional[torch.Tensor]  # the gated product; formed again from z when kept in 8 bits
+    kept: torch.Tensor         # gate and up, and their product or x in 8 bits
     activation: Optional[str]
     clamp_limit: Optional[float]
     shape: tuple
+    bits: int
 
 
 def _check_ffn(x, w13, w2, activation, clamp_limit, residual, checkpoint):
@@ -498,26 +512,35 @@ def _limit_args(clamp_limit):
     return (0, 0.0) if clamp_limit is None else (1, float(clamp_limit))
 
 
-def _ffn(x, w13, w2, activation, clamp_limit, residual, m, hidden, inter, n, checkpoint=None,
-         keep_x=False, keep_z=False):
-    """(y, kept x, w13 and w2 as laid out, kept z, h); launches on the current device."""
+def _ffn_kept(m, hidden, inter, bits, keep_x, keep_z, keep_h):
+    """Sizes of the kept parts: z codes, z scales, x codes, x scales, h."""
+    z = _group_bytes(m, 2 * _up(inter, _GROUP), bits) if keep_z else (None, None)
+    xs = _group_bytes(m, hidden, 8) if keep_x and bits == 8 else (None, None)
+    return (*z, *xs, m * _up(inter, 8) * 2 if keep_h else None)
+
+
+def _ffn(x, w13, w2, activation, clamp_limit, residual, m, hidden, inter, n, bits=0, keep_x=False,
+         keep_z=False, keep_h=False):
+    """(y, x, w13 and w2 as laid out, kept buffer); launches on the current device."""
     out = x.new_empty((m, n))
-    h = _rows_buffer(m, inter, x)
-    xk = zk = ()
-    if keep_x and checkpoint is not None:
-        xk = _checkpoint(x)
-    if keep_z:
-        zk = _empty_kept(m, 2 * _up(inter, _GROUP), x, checkpoint)
+    ldh = _up(inter, 8)
+    kept, zc, zs, xc, xs, h = None, None, None, None, None, None
+    if keep_x or keep_z or keep_h:
+        kept, (zc, zs, xc, xs, h) = _parts(x, *_ffn_kept(m, hidden, inter, bits, keep_x, keep_z, keep_h))
+    if h is None:
+        ws = x.new_empty((m, ldh))
+        h = ws.data_ptr()
     if m == 0:
-        return out, xk or (x,), w13, w2, zk, h
-    # w13 stored by columns: its up rows begin `inter` elements into a row
-    a, b, c = _operand(x), _operand(w13, inter & 7 == 0), _operand(w2)
+        return out, x, w13, w2, kept
+    # w13 stored by columns: its up rows begin `inter` elements into a row;
+    # x to be kept in 8 bits is read by rows
+    a, b, c = _operand(x, xc is None), _operand(w13, inter & 7 == 0), _operand(w2)
     r = None if residual is None else _plain_rows(residual)
     _call("gated_feed_forward", a[1], a[2], a[3], b[1], b[2], b[3], c[1], c[2], c[3], m, hidden, inter,
           n, _DTYPES[x.dtype], ACTIVATIONS[activation], *_limit_args(clamp_limit),
-          None if r is None else r.data_ptr(), 0 if r is None else _row_stride(r), h.data_ptr(),
-          _up(inter, 8), out.data_ptr(), n, *_z_args(zk), _stream(x.get_device()))
-    return out, xk or (a[0],), b[0], c[0], zk, h
+          None if r is None else r.data_ptr(), 0 if r is None else _row_stride(r), h, ldh,
+          out.data_ptr(), n, zc, 0 if zc is None else bits, zs, xc, xs, _stream(x.get_device()))
+    return out, a[0], b[0], c[0], kept
 
 
 def gated_feed_forward(x, w13, w2, *, activation="silu", clamp_limit=None, residual=None,
@@ -551,11 +574,12 @@ def gated_feed_forward_save(x, w13, w2, *, activation="silu", clamp_limit=None, 
     refers to x (unless kept in 8 bits), w13 and w2; they must not change
     before the backward call."""
     shape = _check_ffn(x, w13, w2, activation, clamp_limit, residual, checkpoint)
+    bits = 16 if checkpoint is None else 8
     with torch.no_grad(), _on(x.get_device()):
-        y, xk, w13k, w2k, zk, h = _ffn(x, w13, w2, activation, clamp_limit, residual, *shape,
-                                       checkpoint, True, True)
-    return y, SavedFeedForward(xk, w13k, w2k, zk, h if checkpoint is None else None, activation,
-                               clamp_limit, shape)
+        y, xk, w13k, w2k, kept = _ffn(x, w13, w2, activation, clamp_limit, residual, *shape, bits, True,
+                                      True, bits == 16)
+    return y, SavedFeedForward(xk if bits == 16 else None, w13k, w2k, kept, activation, clamp_limit,
+                               shape, bits)
 
 
 def gated_feed_forward_backward(grad_out, saved: SavedFeedForward, *, need_x=True, need_w13=True,
@@ -569,14 +593,13 @@ def gated_feed_forward_backward(grad_out, saved: SavedFeedForward, *, need_x=Tru
     _explain_matrix(grad_out, "grad_out", m, n, like=saved.w2)
     _explain_device(grad_out, w2=saved.w2)
     with torch.no_grad(), _on(grad_out.get_device()):
-        return _ffn_backward(grad_out, saved.x, saved.w13, saved.w2, saved.z, saved.h,
-                             saved.activation, saved.clamp_limit, *saved.shape, need_x, need_w13,
-                             need_w2)
+        return _ffn_backward(grad_out, saved.x, saved.w13, saved.w2, saved.kept, True, True,
+                             saved.bits == 16, saved.activation, saved.clamp_limit, *saved.shape,
+                             saved.bits, need_x, need_w13, need_w2)
 
 
-def _ffn_backward(grad_out, xk, w13, w2, zk, h, activation, clamp_limit, m, hidden, inter, n, need_x,
-                  need_w13, need_w2):
-    dt, st = _DTYPES[grad_out.dtype], _stream(grad_out.get_device())
+def _ffn_backward(grad_out, x, w13, w2, kept, kept_x, kept_z, kept_h, activation, clamp_limit, m,
+                  hidden, inter, n, bits, need_x, need_w13, need_w2):
     gx = grad_out.new_empty((m, hidden)) if need_x else None
     g13 = grad_out.new_empty((2 * inter, hidden)) if need_w13 else None
     g2 = grad_out.new_empty((n, inter)) if need_w2 else None
@@ -584,27 +607,20 @@ def _ffn_backward(grad_out, xk, w13, w2, zk, h, activation, clamp_limit, m, hidd
         return gx, None if g13 is None else g13.zero_(), None if g2 is None else g2.zero_()
     if not (need_x or need_w13 or need_w2):
         return None, None, None
-    dy = _operand(grad_out)
-    form_h = need_w2 and h is None
-    if need_x or need_w13 or form_h:
-        w = _operand(w2)
-        dz = _rows_buffer(m, 2 * inter, grad_out)
-        if form_h:
-            h = _rows_buffer(m, inter, grad_out)
-        _call("gated_backward_gemm", dy[1], dy[2], dy[3], w[1], w[2], 1 - w[3], m, inter, n, dt,
-              ACTIVATIONS[activation], *_limit_args(clamp_limit), *_z_args(zk), dz.data_ptr(),
-              dz.stride(0), h.data_ptr() if form_h else None, _up(inter, 8), st)
-    if need_w2:
-        ho = _operand(h)
-        _product(dy, 1 - dy[3], ho, 1 - ho[3], n, inter, m, dt, g2, st)
-    if need_x or need_w13:
-        d = _operand(dz)
-        if need_x:
-            w = _operand(w13)
-            _product(d, d[3], w, 1 - w[3], m, hidden, 2 * inter, dt, gx, st)
-        if need_w13:
-            x = _kept_operand(xk, m, hidden, grad_out)
-            _product(d, 1 - d[3], x, 1 - x[3], 2 * inter, hidden, m, dt, g13, st)
+    zc, zs, xc, xs, h = _addresses(kept, *_ffn_kept(m, hidden, inter, bits, kept_x, kept_z, kept_h))
+    form_h = need_w2 and not kept_h
+    ldh, lddz, ldx = _up(inter, 8), _up(2 * inter, 8), _up(hidden, 8)
+    ws, (dz, hw, xr) = _parts(grad_out, m * lddz * 2 if need_x or need_w13 or form_h else None,
+                              m * ldh * 2 if form_h else None,
+                              m * ldx * 2 if need_w13 and xc is not None else None)
+    none = (None, None, 0, 0)
+    dy, w = _operand(grad_out), _operand(w2)
+    u = _operand(w13) if need_x else none
+    xo = _operand(x) if need_w13 and xc is None else none
+    _call("gated_feed_forward_backward", *dy[1:], *xo[1:], xc, xs, xr, ldx, *u[1:], *w[1:], m, hidden, inter,
+          n, _DTYPES[grad_out.dtype], ACTIVATIONS[activation], *_limit_args(clamp_limit), zc,
+          0 if zc is None else bits, zs, hw if form_h else h, ldh, int(form_h), dz, lddz, N.ptr(gx),
+          N.ptr(g13), N.ptr(g2), _stream(grad_out.get_device()))
     return gx, g13, g2
 
 
@@ -612,16 +628,15 @@ class _FeedForwardFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w13, w2, residual, activation, clamp_limit, checkpoint, shape):
         need = ctx.needs_input_grad
+        bits = 16 if checkpoint is None else 8
         inner = need[0] or need[1]
-        with _on(x.get_device()):
-            y, xk, w13k, w2k, zk, h = _ffn(x, w13, w2, activation, clamp_limit, residual, *shape,
-                                           checkpoint, need[1], inner)
-        if not need[1]:
-            xk = ()
         # w2's gradient alone needs h only, which is no larger than z in 8 bits
-        hs = (h,) if need[2] and (checkpoint is None or not inner) else ()
-        ctx.save_for_backward(w13k, w2k, *xk, *zk, *hs)
-        ctx.args = (len(xk), len(zk), activation, clamp_limit, *shape)
+        keep_h = need[2] and (bits == 16 or not inner)
+        with _on(x.get_device()):
+            y, xk, w13k, w2k, kept = _ffn(x, w13, w2, activation, clamp_limit, residual, *shape, bits,
+                                          need[1], inner, keep_h)
+        ctx.save_for_backward(w13k, w2k, kept, xk if need[1] and bits == 16 else None)
+        ctx.args = (need[1], inner, keep_h, activation, clamp_limit, *shape, bits)
         return y
 
     @staticmethod
@@ -629,11 +644,8 @@ class _FeedForwardFunction(torch.autograd.Function):
     def backward(ctx, grad_out):
         need = ctx.needs_input_grad
         gx = g13 = g2 = None
-        if any(need[:3]):
-            w13, w2, *kept = ctx.saved_tensors
-            nx, nz, *args = ctx.args
-            h = kept[nx + nz] if len(kept) > nx + nz else None
+        if need[0] or need[1] or need[2]:
+            w13, w2, kept, x = ctx.saved_tensors
             with _on(grad_out.get_device()):
-                gx, g13, g2 = _ffn_backward(grad_out, kept[:nx], w13, w2, kept[nx:nx + nz], h, *args,
-                                            *need[:3])
+                gx, g13, g2 = _ffn_backward(grad_out, x, w13, w2, kept, *ctx.args, *need[:3])
         return gx, g13, g2, grad_out if need[3] else None, None, None, None, None

@@ -429,13 +429,15 @@ DSV4_API int dsv4_b200_gated_gemm(const void* x, int64_t ldx, int x_mn, const vo
 
 /* The whole block, y = h w2^T + residual: dsv4_b200_gated_gemm into h, then
  * dsv4_b200_dense_gemm (w2 [out_cols][intermediate]).  h is a workspace that
- * the backward pass may use; ldh % 8 == 0, 16-byte aligned. */
+ * the backward pass may use; ldh % 8 == 0, 16-byte aligned.  x_codes and
+ * x_scales (NULL, or [m][ceil32(hidden)] and its scales; x_mn = 0) receive x in
+ * 8 bits. */
 DSV4_API int dsv4_b200_gated_feed_forward(
     const void* x, int64_t ldx, int x_mn, const void* w13, int64_t ldw13, int w13_mn, const void* w2,
     int64_t ldw2, int w2_mn, int64_t m, int64_t hidden, int64_t intermediate, int64_t out_cols,
     int dtype, int activation, int has_clamp, float clamp_limit, const void* residual, int64_t ldr,
     void* h, int64_t ldh, void* out, int64_t ldo, void* z_codes, int z_bits, float* z_scales,
-    void* stream);
+    int8_t* x_codes, float* x_scales, void* stream);
 
 /* Backward of the gate: dh = dy w2 (w2 [k][intermediate], or with w_mn = 0 its
  * transpose) stays in registers; dz [m][2 intermediate] = the gradients of g
@@ -446,6 +448,32 @@ DSV4_API int dsv4_b200_gated_backward_gemm(const void* dy, int64_t lddy, int dy_
                                            float clamp_limit, const void* z_codes, int z_bits,
                                            const float* z_scales, void* dz,
                                            int64_t lddz, void* h, int64_t ldh, void* stream);
+
+/* All gradients of the block; dx [m][hidden], dw13 [2 intermediate][hidden] and
+ * dw2 [out_cols][intermediate] are dense, NULL where not needed.  Workspaces: dz
+ * [m][lddz], h [m][ldh] (form_h = 0: the forward call's h; 1: formed again from
+ * the kept z), x_restored [m][ldxr] where x is given by its codes (else NULL);
+ * each 16-byte aligned with a row stride that is a multiple of 8. */
+DSV4_API int dsv4_b200_gated_feed_forward_backward(
+    const void* dy, int64_t lddy, int dy_mn, const void* x, int64_t ldx, int x_mn,
+    const int8_t* x_codes, const float* x_scales, void* x_restored, int64_t ldxr, const void* w13,
+    int64_t ldw13, int w13_mn, const void* w2, int64_t ldw2, int w2_mn, int64_t m, int64_t hidden,
+    int64_t intermediate, int64_t out_cols, int dtype, int activation, int has_clamp,
+    float clamp_limit, const void* z_codes, int z_bits, const float* z_scales, void* h, int64_t ldh,
+    int form_h, void* dz, int64_t lddz, void* dx, void* dw13, void* dw2, void* stream);
+
+/* All gradients of y = act(x w^T + bias): dx [m][k], dw [n][k], dbias [n], NULL
+ * where not needed.  dy: rows of any alignment.  d: without an activation the
+ * operand dy again; with one the workspace of dz (d_mn = 0).  x, x_restored,
+ * partial and slabs as above and in dsv4_b200_act_backward. */
+DSV4_API int dsv4_b200_dense_backward(const void* dy, int64_t lddy, const void* d, int64_t ldd,
+                                      int d_mn, const void* x, int64_t ldx, int x_mn,
+                                      const int8_t* x_codes, const float* x_scales,
+                                      void* x_restored, int64_t ldxr, const void* w, int64_t ldw,
+                                      int w_mn, int64_t m, int64_t n, int64_t k, int dtype,
+                                      int activation, const void* z_codes, int z_bits,
+                                      const float* z_scales, float* partial, int64_t slabs,
+                                      void* dx, void* dw, void* dbias, void* stream);
 
 /* Activations in 8 bits: x [m][k] fp32 / fp16 / bf16 -> codes, scales; and back. */
 DSV4_API int dsv4_b200_checkpoint_int8(const void* x, int dtype, int64_t m, int64_t k, int64_t ldx,
