@@ -125,7 +125,7 @@ int launch_pair_gemm(F16GemmParams& p, const void* a, int64_t lda, int a_mn, con
   const int half = p.tn / 2, width = EPI == kEpiGated ? half : p.tn;
   p.b_stage = p.b_mn ? (half + 63) / 64 * 8192 : half * 128;
   const int stage = kF16ABytes + p.b_stage;
-  const int fixed = 1024 + kF16EpiBytes + kF16BarBytes;
+  const int fixed = 1024 + F16Roles<EPI>::kEpiBytes + kF16BarBytes;
   p.stages = (kF16SmemMax - fixed) / stage;
   if (p.stages > kF16MaxStages) p.stages = kF16MaxStages;
   p.tiles_m = (p.m + 255) / 256;
@@ -146,9 +146,9 @@ int launch_pair_gemm(F16GemmParams& p, const void* a, int64_t lda, int a_mn, con
   const dim3 grid(static_cast<unsigned>(2 * pairs));
   const size_t smem = fixed + static_cast<size_t>(p.stages) * stage;
   if (bf16) {
-    launch_cluster(&f16_pair_gemm_kernel<EPI, true>, grid, dim3(kF16Threads), smem, st, 2, p);
+    launch_cluster(&f16_pair_gemm_kernel<EPI, true>, grid, dim3(F16Roles<EPI>::kThreads), smem, st, 2, p);
   } else {
-    launch_cluster(&f16_pair_gemm_kernel<EPI, false>, grid, dim3(kF16Threads), smem, st, 2, p);
+    launch_cluster(&f16_pair_gemm_kernel<EPI, false>, grid, dim3(F16Roles<EPI>::kThreads), smem, st, 2, p);
   }
   return check_launch("f16_pair_gemm_kernel");
 }
@@ -519,7 +519,7 @@ int dsv4_b200_act_backward_slabs(int64_t m, int64_t n, int64_t* slabs) {
                (long long)n);
   // four blocks per SM, of at least 32 rows
   const int64_t cols = (n + 255) / 256;
-  int64_t s = (4 * 148 + cols - 1) / cols;
+  int64_t s = 4 * 148 / cols;
   if (s > (m + 31) / 32) s = (m + 31) / 32;
   *slabs = s < 1 ? 1 : s;
   return DSV4_OK;
@@ -550,7 +550,7 @@ int dsv4_b200_act_backward(const void* dy, int64_t lddy, const void* z_codes, in
   p.m = m, p.n = n, p.act = activation;
   p.slab_rows = (m + need - 1) / need;
   const dim3 grid(static_cast<unsigned>((n + 255) / 256), static_cast<unsigned>(need));
-  const dim3 sum_grid(static_cast<unsigned>((n + 127) / 128));
+  const dim3 sum_grid(static_cast<unsigned>((n + 31) / 32));
   const bool bf16 = dtype == DSV4_BF16;
   if (activation != kActNone || dbias) {
     if (m == 0 && !dbias) return DSV4_OK;
@@ -559,8 +559,8 @@ int dsv4_b200_act_backward(const void* dy, int64_t lddy, const void* z_codes, in
     if (int r = check_launch("act_backward_kernel")) return r;
   }
   if (dbias) {
-    if (bf16) launch_pdl(&column_sum_kernel<true>, sum_grid, dim3(128), 0, st, partial, need, n, dbias);
-    else launch_pdl(&column_sum_kernel<false>, sum_grid, dim3(128), 0, st, partial, need, n, dbias);
+    if (bf16) launch_pdl(&column_sum_kernel<true>, sum_grid, dim3(256), 0, st, partial, need, n, dbias);
+    else launch_pdl(&column_sum_kernel<false>, sum_grid, dim3(256), 0, st, partial, need, n, dbias);
     return check_launch("column_sum_kernel");
   }
   return DSV4_OK;

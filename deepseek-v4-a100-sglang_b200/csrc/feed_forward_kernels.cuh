@@ -95,11 +95,30 @@ __device__ __forceinline__ float sigmoid_fast(float z) {
 constexpr float kGeluC = 1.5957691216057308f;  // 2 sqrt(2 / pi)
 constexpr float kGeluK = 0.044715f;
 
+// The normal distribution's function and density times sqrt(2 pi), for gelu:
+// erfc(x) = t (a1 + t (a2 + ...)) exp(-x^2), t = 1 / (1 + p x), x >= 0, off by at
+// most 1.5e-7 (Abramowitz and Stegun, 7.1.26).  One exponential serves the
+// value and the slope.
+__device__ __forceinline__ float normal_cdf(float z, float& density) {
+  const float x = fabsf(z) * 0.70710678118654752f;
+  const float t = __fdividef(1.f, 1.f + 0.3275911f * x);
+  density = __expf(-x * x);
+  float q = 1.061405429f * t - 1.453152027f;
+  q = q * t + 1.421413741f;
+  q = q * t - 0.284496736f;
+  q = q * t + 0.254829592f;
+  q *= 0.5f * t * density;
+  return z < 0.f ? q : 1.f - q;
+}
+
 template <int ACT>
 __device__ __forceinline__ float act_value(float z) {
   if constexpr (ACT == kActRelu) return z <= 0.f ? 0.f : z;
   if constexpr (ACT == kActSilu) return z * sigmoid_fast(z);
-  if constexpr (ACT == kActGelu) return 0.5f * z * (1.f + erff(z * 0.70710678118654752f));
+  if constexpr (ACT == kActGelu) {
+    float density;
+    return z * normal_cdf(z, density);
+  }
   if constexpr (ACT == kActGeluTanh)
     return z * sigmoid_fast(kGeluC * (z + kGeluK * z * z * z));
   return z;
@@ -115,9 +134,10 @@ __device__ __forceinline__ void act_both(float z, float& a, float& slope) {
     a = z * s;
     slope = s * (1.f + z * (1.f - s));
   } else if constexpr (ACT == kActGelu) {
-    const float phi = 0.5f * (1.f + erff(z * 0.70710678118654752f));
+    float density;
+    const float phi = normal_cdf(z, density);
     a = z * phi;
-    slope = phi + z * 0.39894228040143268f * __expf(-0.5f * z * z);
+    slope = phi + z * 0.39894228040143268f * density;
   } else if constexpr (ACT == kActGeluTanh) {
     // past |z| = 100 the sigmoid is 0 or 1 and its slope 0: z^2 is held there
     // so that infinity * 0 does not arise
@@ -337,7 +357,7 @@ __device__ __forceinline__ float keep_group16(const float (&v)[32], float limit,
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const float x = v[2 * j + i];
-      q[i] = x * inv + 12582912.f;  // 1.5 * 2^23: the nearest whole number in the low bits
+      q[i] = __fmaf_rn(x, inv, 12582912.f);  // 1.5 * 2^23: the nearest whole number in the low bits
       if (limited) {
         const float n = q[i] - 12582912.f, toward = x < 0.f ? 1.f : -1.f;  // toward zero
         const bool over = fabsf(x) > limit, kept = fabsf(n * step) > limit;
@@ -594,7 +614,7 @@ struct ActBackward {
 };
 
 template <bool BF16>
-__global__ void __launch_bounds__(256) act_backward_kernel(const ActBackward p) {
+__global__ void __launch_bounds__(256, 4) act_backward_kernel(const ActBackward p) {
   pdl_entry();
   constexpr int DT = BF16 ? DSV4_BF16 : DSV4_F16;
   __shared__ float s_sum[8][256];
@@ -606,7 +626,7 @@ __global__ void __launch_bounds__(256) act_backward_kernel(const ActBackward p) 
   if (col < p.n) {
     act_dispatch(p.act, [&](auto kind) {
       constexpr int K = decltype(kind)::value;
-#pragma unroll 4
+#pragma unroll 2
       for (int64_t row = begin + warp; row < end; row += 8) {
         float d[8];
         load_piece8<DT>(p.dy, row * p.lddy + col, col, p.n, p.vec_dy, d);
@@ -650,16 +670,25 @@ __global__ void __launch_bounds__(256) act_backward_kernel(const ActBackward p) 
   }
 }
 
+// A block: 32 columns; its 8 warps take every eighth slab, then add up.
 template <bool BF16>
-__global__ void __launch_bounds__(128)
+__global__ void __launch_bounds__(256)
     column_sum_kernel(const float* __restrict__ partial, int64_t slabs, int64_t n,
                       void* __restrict__ out) {
   pdl_entry();
-  const int64_t c = static_cast<int64_t>(blockIdx.x) * 128 + threadIdx.x;
-  if (c >= n) return;
+  __shared__ float s_sum[8][32];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t c = static_cast<int64_t>(blockIdx.x) * 32 + lane;
   float t = 0.f;
-#pragma unroll 8
-  for (int64_t s = 0; s < slabs; ++s) t += partial[s * n + c];
+  if (c < n) {
+#pragma unroll 4
+    for (int64_t s = warp; s < slabs; s += 8) t += partial[s * n + c];
+  }
+  s_sum[warp][lane] = t;
+  __syncthreads();
+  if (warp != 0 || c >= n) return;
+#pragma unroll
+  for (int w = 1; w < 8; ++w) t += s_sum[w][lane];
   static_cast<uint16_t*>(out)[c] = static_cast<uint16_t>(pack_16<BF16>(t, 0.f) & 0xffffu);
 }
 

@@ -32,8 +32,6 @@
 
 namespace dsv4 {
 
-enum F16Epi : int { kEpiLinear = 0, kEpiGated = 1, kEpiGatedBwd = 2 };
-
 enum F16DeviceErr : int {
   kErrF16WaitEmpty = 0x201,
   kErrF16WaitFull = 0x202,
@@ -41,11 +39,20 @@ enum F16DeviceErr : int {
   kErrF16WaitAccEmpty = 0x204,
 };
 
-constexpr int kF16Threads = 384;
-constexpr int kF16EpiWarps = 8;
+enum F16Epi : int { kEpiLinear = 0, kEpiGated = 1, kEpiGatedBwd = 2 };
+
+// Epilogue warps and their 2-KB shared slices.  The linear epilogue needs 128
+// registers and one slice: 12 warps (2048 x 2048 -> 7168 with everything that a
+// training step asks of it: 79 us with 8).  The gated ones hold two factors.
+template <int EPI>
+struct F16Roles {
+  static constexpr int kEpiWarps = EPI == kEpiLinear ? 12 : 8;
+  static constexpr int kSlices = EPI == kEpiLinear ? 1 : 2;
+  static constexpr int kThreads = 128 + 32 * kEpiWarps;
+  static constexpr int kEpiBytes = kEpiWarps * kSlices * 2048;
+};
 constexpr int kF16ABytes = 128 * 128;          // 128 rows x 64 elements of A per stage
 constexpr int kF16StageSlice = 2048;           // 32 x 32 16-bit values
-constexpr int kF16EpiBytes = kF16EpiWarps * 2 * kF16StageSlice;
 constexpr int kF16MaxStages = 12;
 constexpr int kF16SmemMax = 232448;
 constexpr int kF16BarBytes = 256;
@@ -363,7 +370,7 @@ __device__ __forceinline__ void kept_rows(const F16GemmParams& p, uint32_t slice
 }
 
 template <int EPI, bool BF16>
-__global__ void __launch_bounds__(kF16Threads, 1)
+__global__ void __launch_bounds__(F16Roles<EPI>::kThreads, 1)
     f16_pair_gemm_kernel(const __grid_constant__ F16GemmParams p) {
   extern __shared__ uint8_t smem_raw[];
   const uint32_t smem = (smem_u32(smem_raw) + 1023u) & ~1023u;
@@ -372,7 +379,8 @@ __global__ void __launch_bounds__(kF16Threads, 1)
   const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
   const int stage_bytes = kF16ABytes + p.b_stage;
   const uint32_t epi_smem = smem + p.stages * stage_bytes;
-  const uint32_t bars = epi_smem + kF16EpiBytes;
+  constexpr int kEpiWarps = F16Roles<EPI>::kEpiWarps, kSlices = F16Roles<EPI>::kSlices;
+  const uint32_t bars = epi_smem + F16Roles<EPI>::kEpiBytes;
   const auto full = [&](int s) { return bars + 8u * s; };
   const auto empty = [&](int s) { return bars + 8u * (kF16MaxStages + s); };
   const auto acc_full = [&](int b) { return bars + 8u * (2 * kF16MaxStages + b); };
@@ -386,7 +394,7 @@ __global__ void __launch_bounds__(kF16Threads, 1)
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(acc_full(b), 1);
-      mbar_init(acc_empty(b), 2 * kF16EpiWarps);
+      mbar_init(acc_empty(b), 2 * kEpiWarps);
     }
     mbar_fence_init();
     tma_prefetch_desc(&p.map_a);
@@ -498,10 +506,10 @@ __global__ void __launch_bounds__(kF16Threads, 1)
       if (ok && elect_one()) mma_commit_both(acc_full(buf));
     }
   } else if (warp >= 4) {
-    // ---- epilogue: warp w reads TMEM lanes 32 (w & 3).., every second chunk ----
+    // ---- epilogue: warp w reads TMEM lanes 32 (w & 3).., its share of the chunks ----
     const int quarter = warp & 3, side = (warp - 4) >> 2;
-    const uint32_t slice0 = epi_smem + (warp - 4) * 2 * kF16StageSlice;
-    const uint32_t slice1 = slice0 + kF16StageSlice;
+    const uint32_t slice0 = epi_smem + (warp - 4) * kSlices * kF16StageSlice;
+    const uint32_t slice1 = slice0 + (kSlices - 1) * kF16StageSlice;
     const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
     uint32_t nt = 0;
     for (int t = pair; t < tiles; t += pairs, ++nt) {
@@ -514,7 +522,7 @@ __global__ void __launch_bounds__(kF16Threads, 1)
       const uint32_t acc = tmem + buf * 256 + lanes;
       const int width = EPI == kEpiGated ? half_n : p.tn;
       const int cbase = tc * width;
-      for (int c0 = side * 32; c0 < width; c0 += 64) {
+      for (int c0 = side * 32; c0 < width; c0 += 8 * kEpiWarps) {
         const int col = cbase + c0;
         if (col >= p.n) break;
         if constexpr (EPI == kEpiLinear) {
