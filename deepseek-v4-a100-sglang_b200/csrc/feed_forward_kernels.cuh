@@ -139,12 +139,12 @@ __device__ __forceinline__ void act_both(float z, float& a, float& slope) {
     a = z * phi;
     slope = phi + z * 0.39894228040143268f * density;
   } else if constexpr (ACT == kActGeluTanh) {
-    // past |z| = 100 the sigmoid is 0 or 1 and its slope 0: z^2 is held there
-    // so that infinity * 0 does not arise
-    const float z2 = fminf(z * z, 1e4f);
+    // past |z| = 100 the sigmoid is 0 or 1 and its slope 0: z is held there so
+    // that infinity * 0 does not arise
+    const float c = fminf(fmaxf(z, -100.f), 100.f);
     const float s = sigmoid_fast(kGeluC * (z + kGeluK * z * z * z));
     a = z * s;
-    slope = s + s * (1.f - s) * kGeluC * (z + 3.f * kGeluK * z * z2);
+    slope = s + s * (1.f - s) * kGeluC * (c + 3.f * kGeluK * c * c * c);
   } else {
     a = z;
     slope = 1.f;
@@ -184,8 +184,8 @@ __device__ __forceinline__ void gated_backward(float limit, float dh, float g, f
   const float gc = clamp_top(g, limit), uc = clamp_both(u, limit);
   float a, s;
   act_both<ACT>(gc, a, s);
-  dg = g <= limit ? dh * uc * s : 0.f;
-  du = fabsf(u) <= limit ? dh * a : 0.f;
+  dg = g > limit ? 0.f : dh * uc * s;  // NaN passes: it has to show in the gradient
+  du = fabsf(u) > limit ? 0.f : dh * a;
   h = a * uc;
 }
 
