@@ -18,7 +18,7 @@ COMMON = [HERE / "common.cuh", HERE / "host_common.h", INCLUDE / "dsv4_b200.h"]
 # translation unit -> the files it is built from
 SOURCES = {
     HERE / "dsv4_b200.cu": [HERE / "gemm_tc.cuh", HERE / "small_kernels.cuh", *COMMON],
-    HERE / "feed_forward.cu": [HERE / "gemm_f16.cuh", HERE / "gemm_f16_stream.cuh",
+    HERE / "feed_forward.cu": [HERE / "gemm_f16.cuh", HERE / "gemm_f16_stream.cuh", HERE / "gemm_f16_rows.cuh",
                                  HERE / "feed_forward_kernels.cuh", *COMMON],
 }
 DEPS = [*SOURCES, *(d for deps in SOURCES.values() for d in deps)]

@@ -8,6 +8,7 @@
 
 #include "feed_forward_kernels.cuh"
 #include "gemm_f16.cuh"
+#include "gemm_f16_rows.cuh"
 #include "gemm_f16_stream.cuh"
 
 namespace dsv4 {
@@ -277,6 +278,19 @@ int launch_stream_gemm(const F16GemmParams& q, F16StreamParams& p, bool two, con
   return check_launch("f16_stream_gemm_kernel");
 }
 
+// 32 KB of shared memory for two blocks; the rest of the SM's memory is L1, which
+// holds the loads in flight (all of it shared: 30.7 us for the block above).
+template <int EPI>
+cudaError_t rows_attrs() {
+  void* const fns[2] = {reinterpret_cast<void*>(&f16_rows_gemm_kernel<EPI, true>),
+                        reinterpret_cast<void*>(&f16_rows_gemm_kernel<EPI, false>)};
+  for (void* fn : fns) {
+    const cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributePreferredSharedMemoryCarveout, 14);
+    if (e != cudaSuccess) return e;
+  }
+  return cudaSuccess;
+}
+
 template <int EPI>
 cudaError_t stream_attrs() {
   void* const fns[2] = {reinterpret_cast<void*>(&f16_stream_gemm_kernel<EPI, true>),
@@ -304,6 +318,29 @@ bool takes_stream(const F16GemmParams& q, bool gated, int w_mn, F16StreamParams&
   double pair_us = 0;
   pick_tn(q.m, q.n, q.k, gated, &pair_us);
   return pick_stream(q, gated, p, two) < pair_us;
+}
+
+// Up to 8 tokens, both operands by rows: for one token 2048 x 2048 takes 3.0 us
+// here and 5.0 streamed, 7168 x 2048 7.5 and 8.9, 4096 x 7168 13.2 and 12.8, 256 x
+// 7168 6.1 and 4.9, a block of 7168 -> 2048 -> 7168 back to back 18.9 and 22.0
+// (23.7 with one product of each kind: they split the SM's memory differently).
+bool takes_rows(const F16GemmParams& q, int x_mn, int w_mn) {
+  return q.m <= kRowsMaxTokens && q.zbits == 0 && !x_mn && !w_mn;
+}
+
+template <int EPI>
+int launch_rows_gemm(const F16GemmParams& q, const void* x, int64_t ldx, const void* w, int64_t ldw,
+                     bool bf16, cudaStream_t st) {
+  DSV4_REQUIRE(aligned16(x) && ldx % 8 == 0 && ldx >= q.k && aligned16(w) && ldw % 8 == 0 && ldw >= q.k,
+               "a and b must be 16-byte aligned with a row stride of at least its row and a multiple "
+               "of 8 elements (row strides %lld and %lld, row %d)", (long long)ldx, (long long)ldw, q.k);
+  F16RowsParams p = {static_cast<const uint16_t*>(x), static_cast<const uint16_t*>(w), ldx, ldw, q.m, q.n,
+                     q.k, q.up_row, q.act, q.limit, q.bias, q.residual, q.out};
+  constexpr int kCols = EPI == kEpiGated ? 8 : 16;
+  const dim3 grid(static_cast<unsigned>((q.n + kCols - 1) / kCols));
+  if (bf16) launch_pdl(&f16_rows_gemm_kernel<EPI, true>, grid, dim3(kRowsThreads), 0, st, p);
+  else launch_pdl(&f16_rows_gemm_kernel<EPI, false>, grid, dim3(kRowsThreads), 0, st, p);
+  return check_launch("f16_rows_gemm_kernel");
 }
 
 constexpr int64_t kMaxDim = 1ll << 30;
@@ -343,6 +380,8 @@ int feed_forward_init() {
   if (e == cudaSuccess) e = stream_attrs<kEpiLinear>();
   if (e == cudaSuccess) e = stream_attrs<kEpiGated>();
   if (e == cudaSuccess) e = query_stream_room();
+  if (e == cudaSuccess) e = rows_attrs<kEpiLinear>();
+  if (e == cudaSuccess) e = rows_attrs<kEpiGated>();
   if (e != cudaSuccess)
     return fail(DSV4_ERR_CUDA, "cudaFuncSetAttribute: %s", cudaGetErrorString(e));
   return DSV4_OK;
@@ -383,6 +422,8 @@ int dsv4_b200_dense_gemm(const void* a, int64_t lda, int a_mn, const void* b, in
   p.residual = mat16(residual, ldr);
   p.out = mat16(out, ldo);
   p.zq = z_codes, p.zbits = z_bits, p.zs = z_scales, p.n32 = round_up(n, kGroup);
+  if (takes_rows(p, a_mn, b_mn))
+    return launch_rows_gemm<kEpiLinear>(p, a, lda, b, ldb, dtype == DSV4_BF16, as_stream(stream));
   F16StreamParams few = {};
   bool two = false;
   if (takes_stream(p, false, b_mn, few, &two))
@@ -413,6 +454,8 @@ int dsv4_b200_gated_gemm(const void* x, int64_t ldx, int x_mn, const void* w13, 
   p.up_row = p.n;
   p.out = mat16(h, ldh);
   p.zq = z_codes, p.zbits = z_bits, p.zs = z_scales, p.n32 = round_up(intermediate, kGroup);
+  if (takes_rows(p, x_mn, w_mn))
+    return launch_rows_gemm<kEpiGated>(p, x, ldx, w13, ldw, dtype == DSV4_BF16, as_stream(stream));
   F16StreamParams few = {};
   bool two = false;
   if (takes_stream(p, true, w_mn, few, &two))
