@@ -186,7 +186,7 @@ def _group_bytes(rows: int, cols: int, bits: int):
 
 # ---- 8-bit checkpoints ----
 
-@dataclass
+@dataclass(slots=True)
 class Int8Checkpoint:
     """Rows of activations in 8 bits: ``codes`` int8 [M, K up to 32], ``scales``
     fp32 [groups, M].  32 consecutive values of a row share a scale
@@ -200,36 +200,40 @@ class Int8Checkpoint:
     dtype: torch.dtype
 
 
-def _empty_codes(rows: int, cols: int, like: torch.Tensor, dtype=torch.int8):
-    k32 = _up(cols, _GROUP)
-    return (like.new_empty((rows, k32), dtype=dtype),
-            like.new_empty((k32 // _GROUP, rows), dtype=torch.float32))
+def _empty_codes(rows: int, cols: int, like: torch.Tensor):
+    groups = -(-cols // _GROUP)
+    return (like.new_empty((rows, groups * _GROUP), dtype=torch.int8),
+            like.new_empty((groups, rows), dtype=torch.float32))
 
 
 def checkpoint_int8(x: torch.Tensor) -> Int8Checkpoint:
     """Keep the rows of ``x`` [M, K] (fp32, fp16 or bf16) in 8 bits: 1.125
     bytes per value.  ``restore_int8(checkpoint_int8(x))`` differs from x by at
     most half a step, ``amax / 254`` of its group, and the rounding to x's type."""
-    if x.dim() != 2:
-        raise ValueError(f"x must be 2-D, got shape {tuple(x.shape)}")
-    if x.dtype not in _CHECKPOINT_DTYPES:
-        raise TypeError(f"x must be fp32, fp16 or bf16, got {x.dtype}")
-    if x.shape[1] == 0:
+    shape, dtype = x.shape, x.dtype
+    if len(shape) != 2:
+        raise ValueError(f"x must be 2-D, got shape {tuple(shape)}")
+    if dtype not in _CHECKPOINT_DTYPES:
+        raise TypeError(f"x must be fp32, fp16 or bf16, got {dtype}")
+    m, k = shape
+    if k == 0:
         raise ValueError("x has no columns")
-    if not x.is_cuda:
+    dev = x.get_device()
+    if dev < 0:
         _explain_device(x)
-    with _on(x.get_device()):
-        codes, scales = _checkpoint(x)
-    return Int8Checkpoint(codes, scales, tuple(x.shape), x.dtype)
-
-
-def _checkpoint(x):
-    x = _distinct_rows(x.detach())
-    m, k = x.shape
+    if torch._C._cuda_getDevice() != dev:
+        with torch.cuda.device(dev):
+            return checkpoint_int8(x)
+    ld, s1 = x.stride()
+    if m == 1 and (s1 == 1 or k == 1):
+        ld = k
+    elif (s1 != 1 and k > 1) or ld < k:
+        x = x.detach().contiguous()
+        ld = k
     codes, scales = _empty_codes(m, k, x)
-    _call("checkpoint_int8", x.data_ptr(), _CHECKPOINT_DTYPES[x.dtype], m, k, _row_stride(x),
-          codes.data_ptr(), scales.data_ptr(), _stream(x.get_device()))
-    return codes, scales
+    _call("checkpoint_int8", x.data_ptr(), _CHECKPOINT_DTYPES[dtype], m, k, ld, codes.data_ptr(),
+          scales.data_ptr(), _stream(dev))
+    return Int8Checkpoint(codes, scales, (m, k), dtype)
 
 
 def restore_int8(checkpoint: Int8Checkpoint, dtype: Optional[torch.dtype] = None) -> torch.Tensor:
@@ -245,16 +249,15 @@ def restore_int8(checkpoint: Int8Checkpoint, dtype: Optional[torch.dtype] = None
             or not s.is_contiguous()):
         raise ValueError(f"codes must be contiguous int8 [{m}, {k32}] and scales contiguous fp32 "
                          f"[{k32 // _GROUP}, {m}]")
-    if not c.is_cuda or c.device != s.device:
+    dev = c.get_device()
+    if dev < 0 or s.get_device() != dev:
         _explain_device(c, scales=s)
-    with _on(c.get_device()):
-        return _restore(c, s, c.new_empty((m, k), dtype=dtype))
-
-
-def _restore(codes, scales, out):
-    m, k = out.shape
-    _call("restore_int8", codes.data_ptr(), scales.data_ptr(), m, k, out.data_ptr(),
-          _CHECKPOINT_DTYPES[out.dtype], _row_stride(out), _stream(out.get_device()))
+    if torch._C._cuda_getDevice() != dev:
+        with torch.cuda.device(dev):
+            return restore_int8(checkpoint, dtype)
+    out = c.new_empty((m, k), dtype=dtype)
+    _call("restore_int8", c.data_ptr(), s.data_ptr(), m, k, out.data_ptr(), _CHECKPOINT_DTYPES[dtype], k,
+          _stream(dev))
     return out
 
 
