@@ -373,6 +373,19 @@ int check_kept(const void* codes, int bits, const float* scales) {
 
 }  // namespace
 
+// Loads the kernels that need no attribute, so that a first launch inside a
+// stream capture finds all of them.
+template <typename... Fns>
+cudaError_t load_kernels(Fns... fns) {
+  cudaError_t e = cudaSuccess;
+  cudaFuncAttributes a;
+  const auto one = [&](auto fn) {
+    if (e == cudaSuccess) e = cudaFuncGetAttributes(&a, reinterpret_cast<const void*>(fn));
+  };
+  (one(fns), ...);
+  return e;
+}
+
 int feed_forward_init() {
   cudaError_t e = pair_attrs<kEpiLinear>();
   if (e == cudaSuccess) e = pair_attrs<kEpiGated>();
@@ -382,8 +395,14 @@ int feed_forward_init() {
   if (e == cudaSuccess) e = query_stream_room();
   if (e == cudaSuccess) e = rows_attrs<kEpiLinear>();
   if (e == cudaSuccess) e = rows_attrs<kEpiGated>();
+  if (e == cudaSuccess)
+    e = load_kernels(&checkpoint_kernel<DSV4_F32>, &checkpoint_kernel<DSV4_F16>,
+                     &checkpoint_kernel<DSV4_BF16>, &restore_kernel<DSV4_F32>,
+                     &restore_kernel<DSV4_F16>, &restore_kernel<DSV4_BF16>,
+                     &act_backward_kernel<true>, &act_backward_kernel<false>,
+                     &column_sum_kernel<true>, &column_sum_kernel<false>, &pack_rows_kernel);
   if (e != cudaSuccess)
-    return fail(DSV4_ERR_CUDA, "cudaFuncSetAttribute: %s", cudaGetErrorString(e));
+    return fail(DSV4_ERR_CUDA, "feed-forward kernels: %s", cudaGetErrorString(e));
   return DSV4_OK;
 }
 

@@ -178,6 +178,17 @@ def _parts(like: torch.Tensor, *sizes):
     return buf, [None if a is None else base + a for a in at]
 
 
+def _on_stream(saved, *tensors) -> None:
+    """What a forward call kept is in use on the current stream too: its memory
+    must not go to others while this stream reads it."""
+    dev = saved.kept.get_device()
+    if _stream(dev) != saved.stream:
+        now = torch.cuda.current_stream(dev)
+        for t in (saved.kept, *tensors):
+            if t is not None:
+                t.record_stream(now)
+
+
 def _group_bytes(rows: int, cols: int, bits: int):
     """Bytes of the codes and of the scales of [rows, cols] kept in groups."""
     k32 = _up(cols, _GROUP)
@@ -273,6 +284,7 @@ class SavedDense:
     shape: tuple
     has_bias: bool
     bits: int
+    stream: int
 
 
 def _check_dense(x, weight, bias, activation, residual, checkpoint):
@@ -361,7 +373,7 @@ def dense_forward_save(x, weight, bias=None, *, activation=None, residual=None, 
     with torch.no_grad(), _on(x.get_device()):
         y, xk, wk, kept = _dense(x, weight, bias, activation, residual, m, n, k, bits, True, True)
     return y, SavedDense(xk if bits == 16 else None, wk, kept, activation, (m, n, k),
-                         bias is not None, bits)
+                         bias is not None, bits, _stream(x.get_device()))
 
 
 def dense_backward(grad_out, saved: SavedDense, *, need_x=True, need_weight=True, need_bias=True):
@@ -371,6 +383,7 @@ def dense_backward(grad_out, saved: SavedDense, *, need_x=True, need_weight=True
     m, n, k = saved.shape
     _explain_matrix(grad_out, "grad_out", m, n, like=saved.weight)
     _explain_device(grad_out, weight=saved.weight)
+    _on_stream(saved, saved.x, saved.weight)
     with torch.no_grad(), _on(grad_out.get_device()):
         return _dense_backward(grad_out, saved.x, saved.weight, saved.kept, True, True,
                                saved.activation, m, n, k, saved.bits, need_x, need_weight,
@@ -480,6 +493,7 @@ class SavedFeedForward:
     clamp_limit: Optional[float]
     shape: tuple
     bits: int
+    stream: int
 
 
 def _check_ffn(x, w13, w2, activation, clamp_limit, residual, checkpoint):
@@ -582,7 +596,7 @@ def gated_feed_forward_save(x, w13, w2, *, activation="silu", clamp_limit=None, 
         y, xk, w13k, w2k, kept = _ffn(x, w13, w2, activation, clamp_limit, residual, *shape, bits, True,
                                       True, bits == 16)
     return y, SavedFeedForward(xk if bits == 16 else None, w13k, w2k, kept, activation, clamp_limit,
-                               shape, bits)
+                               shape, bits, _stream(x.get_device()))
 
 
 def gated_feed_forward_backward(grad_out, saved: SavedFeedForward, *, need_x=True, need_w13=True,
@@ -595,6 +609,7 @@ def gated_feed_forward_backward(grad_out, saved: SavedFeedForward, *, need_x=Tru
     m, hidden, inter, n = saved.shape
     _explain_matrix(grad_out, "grad_out", m, n, like=saved.w2)
     _explain_device(grad_out, w2=saved.w2)
+    _on_stream(saved, saved.x, saved.w13, saved.w2)
     with torch.no_grad(), _on(grad_out.get_device()):
         return _ffn_backward(grad_out, saved.x, saved.w13, saved.w2, saved.kept, True, True,
                              saved.bits == 16, saved.activation, saved.clamp_limit, *saved.shape,

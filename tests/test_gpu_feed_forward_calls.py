@@ -304,6 +304,56 @@ def test_cuda_graphs():
             assert all(same(a, b) for a, b in zip(out, step()))
 
 
+def test_first_call_inside_a_capture():
+    """A process whose first call of all is captured."""
+    import subprocess
+    import sys
+    from pathlib import Path
+    root = Path(__file__).resolve().parent.parent
+    code = """
+import torch, dsv4_b200 as D
+x = torch.randn(300, 72, device="cuda").bfloat16()
+w13, w2 = torch.randn(2 * 33, 72, device="cuda").bfloat16(), torch.randn(72, 33, device="cuda").bfloat16()
+b, dy = torch.zeros(66, device="cuda").bfloat16(), torch.randn(300, 72, device="cuda").bfloat16()
+torch.cuda.synchronize()
+def step():
+    y, saved = D.gated_feed_forward_save(x, w13, w2, checkpoint="int8")
+    z, kept = D.dense_forward_save(x, w13, b, activation="gelu")
+    return (y, D.gated_feed_forward(x[:3], w13, w2), D.gated_feed_forward(x[:40], w13, w2),
+            *D.gated_feed_forward_backward(dy, saved), *D.dense_backward(z, kept),
+            D.restore_int8(D.checkpoint_int8(x)))
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    out = step()
+graph.replay()
+assert all(torch.equal(a, c) for a, c in zip(out, step()))
+print("captured")
+"""
+    env = {**__import__("os").environ, "PYTHONPATH": str(root / "deepseek-v4-a100-sglang_b200")}
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, env=env, timeout=300)
+    assert "captured" in r.stdout, r.stderr[-2000:]
+
+
+def test_backward_on_another_stream():
+    import dsv4_b200 as D
+    x, w13, w2, r = ffn_case(300, 512, 256, 512, BF16)
+    dy = rand(300, 512, seed=9)
+    y, saved = D.gated_feed_forward_save(x, w13, w2, residual=r)
+    want = D.gated_feed_forward_backward(dy, saved)
+    torch.cuda.synchronize()
+    for _ in range(5):
+        y, saved = D.gated_feed_forward_save(x, w13, w2, residual=r)
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            got = D.gated_feed_forward_backward(dy, saved)
+        del saved
+        junk = [torch.full((300, 2048), 7.0, device="cuda") for _ in range(4)]  # takes freed memory
+        torch.cuda.synchronize()
+        assert all(same(a, b) for a, b in zip(got, want))
+        del junk
+
+
 def test_autograd_under_capture_is_refused():
     import dsv4_b200 as D
     x, w, _, _ = dense_case(4, 32, 32, BF16, False, False)
