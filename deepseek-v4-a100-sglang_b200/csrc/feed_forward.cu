@@ -282,8 +282,10 @@ int launch_stream_gemm(const F16GemmParams& q, F16StreamParams& p, bool two, con
 // holds the loads in flight (all of it shared: 30.7 us for the block above).
 template <int EPI>
 cudaError_t rows_attrs() {
-  void* const fns[2] = {reinterpret_cast<void*>(&f16_rows_gemm_kernel<EPI, true>),
-                        reinterpret_cast<void*>(&f16_rows_gemm_kernel<EPI, false>)};
+  void* const fns[4] = {reinterpret_cast<void*>(&f16_rows_gemm_kernel<EPI, true, true>),
+                        reinterpret_cast<void*>(&f16_rows_gemm_kernel<EPI, false, true>),
+                        reinterpret_cast<void*>(&f16_rows_gemm_kernel<EPI, true, false>),
+                        reinterpret_cast<void*>(&f16_rows_gemm_kernel<EPI, false, false>)};
   for (void* fn : fns) {
     const cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributePreferredSharedMemoryCarveout, 14);
     if (e != cudaSuccess) return e;
@@ -320,7 +322,7 @@ bool takes_stream(const F16GemmParams& q, bool gated, int w_mn, F16StreamParams&
   return pick_stream(q, gated, p, two) < pair_us;
 }
 
-// Up to 8 tokens, both operands by rows: for one token 2048 x 2048 takes 3.0 us
+// Up to 8 tokens, both operands by rows (at any alignment): for one token 2048 x 2048 takes 3.0 us
 // here and 5.0 streamed, 7168 x 2048 7.5 and 8.9, 4096 x 7168 13.2 and 12.8, 256 x
 // 7168 6.1 and 4.9, a block of 7168 -> 2048 -> 7168 back to back 18.9 and 22.0
 // (23.7 with one product of each kind: they split the SM's memory differently).
@@ -331,15 +333,18 @@ bool takes_rows(const F16GemmParams& q, int x_mn, int w_mn) {
 template <int EPI>
 int launch_rows_gemm(const F16GemmParams& q, const void* x, int64_t ldx, const void* w, int64_t ldw,
                      bool bf16, cudaStream_t st) {
-  DSV4_REQUIRE(aligned16(x) && ldx % 8 == 0 && ldx >= q.k && aligned16(w) && ldw % 8 == 0 && ldw >= q.k,
-               "a and b must be 16-byte aligned with a row stride of at least its row and a multiple "
-               "of 8 elements (row strides %lld and %lld, row %d)", (long long)ldx, (long long)ldw, q.k);
+  DSV4_REQUIRE((reinterpret_cast<uintptr_t>(x) & 1) == 0 && (reinterpret_cast<uintptr_t>(w) & 1) == 0,
+               "a and b must be aligned to their elements");
+  DSV4_REQUIRE(ldx >= q.k && ldw >= q.k, "row stride below k (%lld and %lld, k %d)",
+               (long long)ldx, (long long)ldw, q.k);
   F16RowsParams p = {static_cast<const uint16_t*>(x), static_cast<const uint16_t*>(w), ldx, ldw, q.m, q.n,
                      q.k, q.up_row, q.act, q.limit, q.bias, q.residual, q.out};
   constexpr int kCols = EPI == kEpiGated ? 8 : 16;
   const dim3 grid(static_cast<unsigned>((q.n + kCols - 1) / kCols));
-  if (bf16) launch_pdl(&f16_rows_gemm_kernel<EPI, true>, grid, dim3(kRowsThreads), 0, st, p);
-  else launch_pdl(&f16_rows_gemm_kernel<EPI, false>, grid, dim3(kRowsThreads), 0, st, p);
+  const bool aligned = aligned16(x) && ldx % 8 == 0 && aligned16(w) && ldw % 8 == 0;
+  const auto go = [&](auto kernel) { launch_pdl(kernel, grid, dim3(kRowsThreads), 0, st, p); };
+  if (aligned) bf16 ? go(&f16_rows_gemm_kernel<EPI, true, true>) : go(&f16_rows_gemm_kernel<EPI, false, true>);
+  else bf16 ? go(&f16_rows_gemm_kernel<EPI, true, false>) : go(&f16_rows_gemm_kernel<EPI, false, false>);
   return check_launch("f16_rows_gemm_kernel");
 }
 

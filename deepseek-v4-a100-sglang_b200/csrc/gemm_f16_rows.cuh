@@ -12,6 +12,10 @@
 // between memory and the tensor cores.  The warps' parts meet in shared memory
 // and are added in warp order.  64 registers, so that two blocks fit an SM.
 //
+// Rows at any even address (an odd k, a view): the two aligned 16-byte pieces
+// around 8 values are loaded and shifted together.  That reads a few bytes of
+// the rows beside it, never outside the matrix.
+//
 // kEpiGated: rows 0-7 of the MMA are gate rows, 8-15 the same up rows, so that
 // a thread's sums hold both factors.
 #pragma once
@@ -23,7 +27,6 @@ namespace dsv4 {
 constexpr int kRowsThreads = 512;
 constexpr int kRowsWarps = kRowsThreads / 32;
 constexpr int kRowsMaxTokens = 8;
-constexpr int kRowsAhead = 2;  // blocks of 64 of k in flight
 
 struct F16RowsParams {
   const uint16_t* x;
@@ -63,9 +66,58 @@ __device__ __forceinline__ uint4 load_k8(const uint16_t* p, int left) {
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-template <int EPI, bool BF16>
-__global__ void __launch_bounds__(kRowsThreads, 2)
+// A matrix's first byte and the one behind its last.
+struct Extent {
+  uint64_t lo, hi;
+};
+
+__device__ __forceinline__ Extent extent_of(const uint16_t* p, int64_t rows, int64_t ld, int k) {
+  const uint64_t lo = reinterpret_cast<uint64_t>(p);
+  return {lo, lo + 2 * static_cast<uint64_t>((rows - 1) * ld + k)};
+}
+
+// The same from any even address.
+struct Window {
+  uint4 a, b;
+};
+
+__device__ __forceinline__ Window load_window(const uint16_t* p, int left, const Extent& e) {
+  const uint64_t at = reinterpret_cast<uint64_t>(p) & ~15ull;
+  Window w;
+  if (left >= 8 && at >= e.lo && at + 32 <= e.hi) {
+    w.a = *reinterpret_cast<const uint4*>(at);
+    w.b = *reinterpret_cast<const uint4*>(at + 16);
+  } else {  // at the matrix's ends: the 8 values themselves, put where the shift finds them
+    uint32_t v[8] = {};
+    const int off = static_cast<int>(reinterpret_cast<uint64_t>(p) & 15) >> 1;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const int j = i - off;
+      if (j >= 0 && j < 8 && j < left) v[i >> 1] |= static_cast<uint32_t>(p[j]) << (16 * (i & 1));
+    }
+    w.a = make_uint4(v[0], v[1], v[2], v[3]);
+    w.b = make_uint4(v[4], v[5], v[6], v[7]);
+  }
+  return w;
+}
+
+// 16 bytes of the window from byte `off` (even, below 16)
+__device__ __forceinline__ uint4 shift_window(const Window& w, int off) {
+  const uint32_t v[8] = {w.a.x, w.a.y, w.a.z, w.a.w, w.b.x, w.b.y, w.b.z, w.b.w};
+  uint32_t t[6], u[5];
+#pragma unroll
+  for (int i = 0; i < 6; ++i) t[i] = off & 8 ? v[i + 2] : v[i];
+#pragma unroll
+  for (int i = 0; i < 5; ++i) u[i] = off & 4 ? t[i + 1] : t[i];
+  const int bits = off & 2 ? 16 : 0;
+  return make_uint4(__funnelshift_r(u[0], u[1], bits), __funnelshift_r(u[1], u[2], bits),
+                    __funnelshift_r(u[2], u[3], bits), __funnelshift_r(u[3], u[4], bits));
+}
+
+template <int EPI, bool BF16, bool ALIGNED>
+__global__ void __launch_bounds__(kRowsThreads, ALIGNED ? 2 : 1)
     f16_rows_gemm_kernel(const F16RowsParams p) {
+  constexpr int kRowsAhead = 2;  // blocks of 64 of k in flight
   __shared__ float s_part[kRowsWarps][128];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, q = lane & 3;
@@ -92,7 +144,34 @@ __global__ void __launch_bounds__(kRowsThreads, 2)
   float acc[4] = {};
   const bool live = g < p.m;
   const uint16_t* const token = p.x + (live ? g : 0) * p.ldx;
-  for (int kb = warp; kb < kblocks; kb += kRowsAhead * kRowsWarps) {
+  if constexpr (!ALIGNED) {
+    const Extent we = extent_of(p.w, EPI == kEpiGated ? 2 * p.up_row : p.n, p.ldw, p.k);
+    const Extent xe = extent_of(p.x, p.m, p.ldx, p.k);
+    // rows are apart by any number of elements, k by whole pieces: a row's shift stays
+    const int sa = static_cast<int>(reinterpret_cast<uint64_t>(row_a) & 15);
+    const int sb = static_cast<int>(reinterpret_cast<uint64_t>(row_b) & 15);
+    const int sx = static_cast<int>(reinterpret_cast<uint64_t>(token) & 15);
+    for (int kb = warp; kb < kblocks; kb += kRowsWarps) {
+      Window a[2], b[2], x[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int k0 = kb * 64 + h * 32 + q * 8, left = p.k - k0;
+        a[h].a = a[h].b = b[h].a = b[h].b = x[h].a = x[h].b = make_uint4(0, 0, 0, 0);
+        if (left > 0) {
+          a[h] = load_window(row_a + k0, left, we);
+          b[h] = load_window(row_b + k0, left, we);
+          if (live) x[h] = load_window(token + k0, left, xe);
+        }
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const uint4 va = shift_window(a[h], sa), vb = shift_window(b[h], sb), vx = shift_window(x[h], sx);
+        mma_m16n8k16<BF16>(acc, va.x, vb.x, va.y, vb.y, vx.x, vx.y);
+        mma_m16n8k16<BF16>(acc, va.z, vb.z, va.w, vb.w, vx.z, vx.w);
+      }
+    }
+  }
+  for (int kb = ALIGNED ? warp : kblocks; kb < kblocks; kb += kRowsAhead * kRowsWarps) {
     uint4 a[kRowsAhead][2], b[kRowsAhead][2], x[kRowsAhead][2];
 #pragma unroll
     for (int u = 0; u < kRowsAhead; ++u)

@@ -36,6 +36,7 @@ _CHECKPOINTS = (None, "int8")
 _DTYPES = {torch.float16: N.DTYPE_F16, torch.bfloat16: N.DTYPE_BF16}
 _CHECKPOINT_DTYPES = {torch.float32: N.DTYPE_F32, **_DTYPES}
 _GROUP = 32
+_FEW = 8  # tokens up to which a product without kept values reads rows of any alignment
 
 
 class _Functions(dict):
@@ -143,6 +144,17 @@ def _operand(t: torch.Tensor, columns: bool = True):
     ld = out.stride(0) if rows > 1 else _up(cols, 8)
     _call("pack_rows", ptr, s0, s1, rows, cols, out.data_ptr(), ld, _stream(t.get_device()))
     return out, out.data_ptr(), ld, 0
+
+
+def _row_operands(x: torch.Tensor, w: torch.Tensor, columns: bool = True):
+    """:func:`_operand` of both for a product of few tokens: where both lie by
+    rows, any alignment will do."""
+    if x.shape[0] <= _FEW and w.stride(1) == 1 and x.stride(1) == 1:
+        m, k = x.shape
+        ldx, ldw = x.stride(0) if m > 1 else _up(k, 8), w.stride(0)
+        if ldx >= k and ldw >= k:
+            return (x, x.data_ptr(), ldx, 0), (w, w.data_ptr(), ldw, 0)
+    return _operand(x), _operand(w, columns)
 
 
 def _plain_rows(t: torch.Tensor) -> torch.Tensor:
@@ -332,7 +344,10 @@ def _dense(x, weight, bias, activation, residual, m, n, k, bits=0, keep_x=False,
         kept, (zc, zs, xc, xs) = _dense_kept(x, m, n, k, activation, bits, keep_x, keep_z)
     if m == 0:
         return out, x, weight, kept
-    a, b = _operand(x), _operand(weight)
+    if kept is None:
+        a, b = _row_operands(x, weight)
+    else:
+        a, b = _operand(x), _operand(weight)
     if kept is not None and xc is not None:
         rows = a if a[3] == 0 else _operand(x, False)
         _call("checkpoint_int8", rows[1], dt, m, k, rows[2], xc, xs, st)
@@ -551,7 +566,12 @@ def _ffn(x, w13, w2, activation, clamp_limit, residual, m, hidden, inter, n, bit
         return out, x, w13, w2, kept
     # w13 stored by columns: its up rows begin `inter` elements into a row;
     # x to be kept in 8 bits is read by rows
-    a, b, c = _operand(x, xc is None), _operand(w13, inter & 7 == 0), _operand(w2)
+    if zc is None and xc is None:
+        a, b = _row_operands(x, w13, inter & 7 == 0)
+    else:
+        a, b = _operand(x, xc is None), _operand(w13, inter & 7 == 0)
+    c = (w2, w2.data_ptr(), w2.stride(0), 0) if m <= _FEW and w2.stride(1) == 1 and w2.stride(0) >= inter \
+        else _operand(w2)
     r = None if residual is None else _plain_rows(residual)
     _call("gated_feed_forward", a[1], a[2], a[3], b[1], b[2], b[3], c[1], c[2], c[3], m, hidden, inter,
           n, _DTYPES[x.dtype], ACTIVATIONS[activation], *_limit_args(clamp_limit),

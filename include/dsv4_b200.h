@@ -390,7 +390,9 @@ DSV4_API int dsv4_b200_mxfp4_int8_dense_gemm_noalloc(const int8_t* a_q, const fl
  * with a row stride (ld, elements).  Operands of a product (a, b, x, w, dy)
  * are 16-byte aligned with a row stride that is a multiple of 8; `*_mn` = 0
  * means rows of the contraction axis ([rows][k]), 1 the transposed storage
- * ([k][rows]).  dsv4_b200_pack_rows lays out an operand of any strides.
+ * ([k][rows]).  dsv4_b200_pack_rows lays out an operand of any strides.  (For up
+ * to 8 tokens, operands by rows and nothing kept, dsv4_b200_dense_gemm and
+ * dsv4_b200_gated_gemm take any alignment.)
  * Results and `residual` have any alignment.  activation: dsv4_activation.
  * Kept values are groups of 32 values of a row that share an fp32 scale
  * amax / steps (rounded toward zero), steps 127 in 8 bits and 32767 in 16:

@@ -69,6 +69,46 @@ def test_dense_gradients(kind, mode, m, k, n, dtype):
     assert torch.equal(grads[3], dy)
 
 
+@pytest.mark.parametrize("k", [1, 7, 8, 9, 31, 63, 64, 65, 127, 1001, 2050])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_few_tokens_at_any_alignment(k, dtype):
+    """1 to 9 tokens, rows that begin at every even address of 16 bytes, the
+    matrices inside buffers of NaN: nothing beside them is read into a sum."""
+    import dsv4_b200 as D
+
+    def inside(t, lead, gap):
+        rows, cols = t.shape
+        buf = torch.full((lead + rows * (cols + gap) + 8,), math.nan, dtype=dtype, device="cuda")
+        view = buf[lead:lead + rows * (cols + gap)].view(rows, cols + gap)[:, :cols]
+        view.copy_(t)
+        return view
+
+    for i, (m, n) in enumerate([(1, 1), (1, 40), (2, 17), (3, 8), (5, 33), (8, 16), (8, 100), (9, 24)]):
+        x, w, b, r = dense_case(m, k, n, dtype, seed=k + i)
+        want = R.dense(x, w, b, r, "silu", dtype)["y"]
+        for lead in range(8):
+            xv, wv = inside(x, lead, (i + lead) % 5), inside(w, (3 * lead + i) % 8, lead % 3)
+            R.assert_within(f"y {m} {n} {lead}", D.dense_forward(xv, wv, b, activation="silu", residual=r), want)
+        x, w13, w2, r = ffn_case(m, k, n, 24, dtype, seed=k + i)
+        want = R.ffn(x, w13, w2, r, "gelu", 1.5, dtype)["y"]
+        for lead in range(0, 8, 3):
+            args = inside(x, lead, 1), inside(w13, lead + 1, lead), inside(w2, 7 - lead, 1)
+            y = D.gated_feed_forward(*args, activation="gelu", clamp_limit=1.5, residual=r)
+            R.assert_within(f"block {m} {n} {lead}", y, want)
+
+
+def test_few_tokens_at_the_ends_of_a_buffer():
+    """Matrices that begin and end with their buffers, of one and of few values."""
+    import dsv4_b200 as D
+    for m, k, n in ((1, 1, 1), (1, 3, 1), (2, 5, 3), (1, 17, 2), (8, 23, 5)):
+        x, w, _, _ = dense_case(m, k, n, BF16, False, False)
+        for cut in range(4):
+            xb, wb = torch.empty(m * k + cut, device="cuda", dtype=BF16), torch.empty(n * k + cut, device="cuda", dtype=BF16)
+            xv, wv = xb[cut:].view(m, k), wb[cut:].view(n, k)
+            xv.copy_(x), wv.copy_(w)
+            R.assert_within("y", D.dense_forward(xv, wv), R.dense(x, w, None, None, None, BF16)["y"])
+
+
 FFN = [
     (1, 64, 32, 64), (1, 1024, 512, 1024), (3, 72, 17, 40), (16, 256, 128, 256), (31, 1000, 77, 1000),
     (64, 512, 509, 512), (65, 136, 64, 129), (128, 1024, 512, 1024), (130, 264, 100, 264),
