@@ -22,7 +22,7 @@ formulas say.  All results are the same bits from call to call.
 from __future__ import annotations
 
 import contextlib
-import ctypes
+import functools
 import math
 from dataclasses import dataclass
 from typing import Optional
@@ -114,13 +114,6 @@ def _up(v: int, to: int) -> int:
     return -(-v // to) * to
 
 
-def _rows_buffer(rows: int, cols: int, like: torch.Tensor) -> torch.Tensor:
-    """[rows, cols] with rows at multiples of 16 bytes."""
-    if cols % 8 == 0:
-        return like.new_empty((rows, cols))
-    return like.new_empty((rows, _up(cols, 8)))[:, :cols]
-
-
 def _operand(t: torch.Tensor, columns: bool = True):
     """A 2-D tensor as a product reads it: ``(tensor, address, stride, mn)``
     with rows (mn 0) or columns (mn 1) contiguous and 16-byte aligned.
@@ -140,10 +133,16 @@ def _operand(t: torch.Tensor, columns: bool = True):
                 return t, ptr, _up(rows, 8), 1
             if s1 & 7 == 0 and s1 >= rows:
                 return t, ptr, s1, 1
-    out = _rows_buffer(rows, cols, t)
-    ld = out.stride(0) if rows > 1 else _up(cols, 8)
-    _call("pack_rows", ptr, s0, s1, rows, cols, out.data_ptr(), ld, _stream(t.get_device()))
-    return out, out.data_ptr(), ld, 0
+    ld = _up(cols, 8)
+    out = t.new_empty((rows, ld))
+    ptr2 = out.data_ptr()
+    _call("pack_rows", ptr, s0, s1, rows, cols, ptr2, ld, _stream(t.get_device()))
+    return out, ptr2, ld, 0
+
+
+def _laid_out(operand, t: torch.Tensor) -> torch.Tensor:
+    """t, or the copy of it that a product reads, to be kept for the backward pass."""
+    return t if operand[0] is t else operand[0][:, :t.shape[1]]
 
 
 def _row_operands(x: torch.Tensor, w: torch.Tensor, columns: bool = True):
@@ -177,17 +176,27 @@ def _row_stride(t: torch.Tensor) -> int:
 
 
 # ---- what a training step keeps, and the backward pass's workspace ----
-# One allocation each: parts at multiples of 256 bytes, passed by address.
+# One allocation each, in the inputs' 16-bit type: parts at multiples of 256
+# bytes, passed by address.  The layouts are functions of the sizes alone.
 
-def _parts(like: torch.Tensor, *sizes):
-    """A buffer of bytes and the addresses of parts of these sizes (None: none)."""
+@functools.lru_cache(maxsize=4096)
+def _layout(*sizes):
+    """(elements of 2 bytes, byte offset of each part, None for a size of None)."""
     total, at = 0, []
     for size in sizes:
         at.append(None if size is None else total)
         total += 0 if size is None else _up(size, 256)
-    buf = like.new_empty(total, dtype=torch.uint8)
-    base = buf.data_ptr()
-    return buf, [None if a is None else base + a for a in at]
+    return total // 2, tuple(at)
+
+
+def _group_bytes(rows: int, cols: int, bits: int):
+    """Bytes of the codes and of the scales of [rows, cols] kept in groups."""
+    k32 = _up(cols, _GROUP)
+    return rows * k32 * bits // 8, rows * (k32 // _GROUP) * 4
+
+
+def _at(base: int, offsets):
+    return [None if o is None else base + o for o in offsets]
 
 
 def _on_stream(saved, *tensors) -> None:
@@ -199,12 +208,6 @@ def _on_stream(saved, *tensors) -> None:
         for t in (saved.kept, *tensors):
             if t is not None:
                 t.record_stream(now)
-
-
-def _group_bytes(rows: int, cols: int, bits: int):
-    """Bytes of the codes and of the scales of [rows, cols] kept in groups."""
-    k32 = _up(cols, _GROUP)
-    return rows * k32 * bits // 8, rows * (k32 // _GROUP) * 4
 
 
 # ---- 8-bit checkpoints ----
@@ -328,27 +331,39 @@ def _check_dense(x, weight, bias, activation, residual, checkpoint):
     raise RuntimeError("unsupported arguments")
 
 
-def _dense_kept(x, m, n, k, activation, bits, keep_x, keep_z):
-    """(buffer, addresses of z codes, z scales, x codes, x scales)."""
-    z = _group_bytes(m, n, bits) if keep_z and activation is not None else (None, None)
+@functools.lru_cache(maxsize=4096)
+def _dense_kept(m, n, k, act, bits, keep_x, keep_z):
+    """Layout of z codes, z scales, x codes, x scales."""
+    z = _group_bytes(m, n, bits) if keep_z and act else (None, None)
     xs = _group_bytes(m, k, 8) if keep_x and bits == 8 else (None, None)
-    return _parts(x, *z, *xs)
+    return _layout(*z, *xs)
+
+
+@functools.lru_cache(maxsize=4096)
+def _dense_workspace(m, n, k, act, bias, restore):
+    """Slabs of the bias gradient (those of act_backward_slabs), and the layout
+    of dz, their partial sums and the restored x."""
+    slabs = max(1, min(4 * 148 // -(-n // 256), -(-m // 32))) if bias else 0
+    return slabs, _layout(m * _up(n, 8) * 2 if act else None, slabs * n * 4 if bias else None,
+                          m * _up(k, 8) * 2 if restore else None)
 
 
 def _dense(x, weight, bias, activation, residual, m, n, k, bits=0, keep_x=False, keep_z=False):
     """(y, x and weight as laid out, kept buffer); launches on the current device."""
     dt, st = _DTYPES[x.dtype], _stream(x.get_device())
     out = x.new_empty((m, n))
-    kept, zc, zs = None, None, None
+    kept = zc = zs = xc = None
     if keep_x or keep_z:
-        kept, (zc, zs, xc, xs) = _dense_kept(x, m, n, k, activation, bits, keep_x, keep_z)
+        size, offsets = _dense_kept(m, n, k, activation is not None, bits, keep_x, keep_z)
+        kept = x.new_empty(size)
+        zc, zs, xc, xs = _at(kept.data_ptr(), offsets)
     if m == 0:
         return out, x, weight, kept
     if kept is None:
         a, b = _row_operands(x, weight)
     else:
         a, b = _operand(x), _operand(weight)
-    if kept is not None and xc is not None:
+    if xc is not None:
         rows = a if a[3] == 0 else _operand(x, False)
         _call("checkpoint_int8", rows[1], dt, m, k, rows[2], xc, xs, st)
     if bias is not None and bias.stride(0) != 1:
@@ -358,7 +373,9 @@ def _dense(x, weight, bias, activation, residual, m, n, k, bits=0, keep_x=False,
           None if bias is None else bias.data_ptr(), ACTIVATIONS[activation],
           None if r is None else r.data_ptr(), 0 if r is None else _row_stride(r), out.data_ptr(), n,
           zc, 0 if zc is None else bits, zs, st)
-    return out, a[0], b[0], kept
+    if kept is None:
+        return out, x, weight, None
+    return out, _laid_out(a, x), _laid_out(b, weight), kept
 
 
 def dense_forward(x, weight, bias=None, *, activation=None, residual=None, checkpoint=None):
@@ -405,15 +422,6 @@ def dense_backward(grad_out, saved: SavedDense, *, need_x=True, need_weight=True
                                need_bias and saved.has_bias)
 
 
-def _addresses(kept, *sizes):
-    """The addresses :func:`_parts` gave for these sizes."""
-    at, out = kept.data_ptr(), []
-    for size in sizes:
-        out.append(None if size is None else at)
-        at += 0 if size is None else _up(size, 256)
-    return out
-
-
 def _dense_backward(dy, x, weight, kept, kept_x, kept_z, activation, m, n, k, bits, need_x, need_weight,
                     need_bias):
     dt, st = _DTYPES[dy.dtype], _stream(dy.get_device())
@@ -424,33 +432,24 @@ def _dense_backward(dy, x, weight, kept, kept_x, kept_z, activation, m, n, k, bi
         return gx, None if gw is None else gw.zero_(), None if gb is None else gb.zero_()
     if not (need_x or need_weight or need_bias):
         return None, None, None
-    z = _group_bytes(m, n, bits) if kept_z and activation is not None else (None, None)
-    xs = _group_bytes(m, k, 8) if kept_x and bits == 8 else (None, None)
-    zc, zs, xc, xsc = _addresses(kept, *z, *xs)
-    rows, d = dy, (None, None, 0, 0)
-    if activation is not None or need_bias:
+    act = activation is not None
+    zc, zs, xc, xsc = _at(kept.data_ptr(), _dense_kept(m, n, k, act, bits, kept_x, kept_z)[1])
+    rows, d, ld, ldx = dy, (None, None, 0, 0), _up(n, 8), _up(k, 8)
+    if act or need_bias:
         rows = _distinct_rows(dy)
-    if activation is None and (need_x or need_weight):
-        d = _operand(dy)
-    slabs = _slabs(m, n) if need_bias else 0
-    ld, ldx = _up(n, 8), _up(k, 8)
-    ws, (dz, partial, xr) = _parts(dy, None if activation is None else m * ld * 2,
-                                   slabs * n * 4 if need_bias else None,
-                                   m * ldx * 2 if need_weight and xc is not None else None)
-    if activation is not None:
+    slabs, (size, offsets) = _dense_workspace(m, n, k, act, need_bias, need_weight and xc is not None)
+    ws = dy.new_empty(size)
+    dz, partial, xr = _at(ws.data_ptr(), offsets)
+    if act:
         d = (ws, dz, ld, 0)
+    elif need_x or need_weight:
+        d = _operand(dy)
     xo = _operand(x) if need_weight and xc is None else (None, None, 0, 0)
     w = _operand(weight) if need_x else (None, None, 0, 0)
     _call("dense_backward", rows.data_ptr(), _row_stride(rows), *d[1:], *xo[1:], xc, xsc, xr, ldx, *w[1:],
           m, n, k, dt, ACTIVATIONS[activation], zc, 0 if zc is None else bits, zs, partial, slabs,
           N.ptr(gx), N.ptr(gw), N.ptr(gb), st)
     return gx, gw, gb
-
-
-def _slabs(m: int, n: int) -> int:
-    v = ctypes.c_int64(0)
-    _call("act_backward_slabs", m, n, ctypes.byref(v))
-    return v.value
 
 
 def _recorded(*tensors) -> bool:
@@ -476,8 +475,12 @@ class _DenseFunction(torch.autograd.Function):
         need = ctx.needs_input_grad
         bits = 16 if checkpoint is None else 8
         keep_z = need[0] or need[1] or need[2]
-        with _on(x.get_device()):
-            y, xk, wk, kept = _dense(x, weight, bias, activation, residual, m, n, k, bits, need[1], keep_z)
+        args = (x, weight, bias, activation, residual, m, n, k, bits, need[1], keep_z)
+        if torch._C._cuda_getDevice() == x.get_device():
+            y, xk, wk, kept = _dense(*args)
+        else:
+            with torch.cuda.device(x.device):
+                y, xk, wk, kept = _dense(*args)
         ctx.save_for_backward(wk, kept, xk if need[1] and bits == 16 else None)
         ctx.args = (need[1], keep_z, activation, m, n, k, bits)
         return y
@@ -488,9 +491,8 @@ class _DenseFunction(torch.autograd.Function):
         need = ctx.needs_input_grad
         gx = gw = gb = None
         if need[0] or need[1] or need[2]:
-            w, kept, x = ctx.saved_tensors
-            with _on(grad_out.get_device()):
-                gx, gw, gb = _dense_backward(grad_out, x, w, kept, *ctx.args, *need[:3])
+            w, kept, x = ctx.saved_tensors  # (the engine has made their device current)
+            gx, gw, gb = _dense_backward(grad_out, x, w, kept, *ctx.args, *need[:3])
         return gx, gw, gb, grad_out if need[3] else None, None, None, None, None, None
 
 
@@ -544,11 +546,12 @@ def _limit_args(clamp_limit):
     return (0, 0.0) if clamp_limit is None else (1, float(clamp_limit))
 
 
+@functools.lru_cache(maxsize=4096)
 def _ffn_kept(m, hidden, inter, bits, keep_x, keep_z, keep_h):
-    """Sizes of the kept parts: z codes, z scales, x codes, x scales, h."""
+    """Layout of z codes, z scales, x codes, x scales, h."""
     z = _group_bytes(m, 2 * _up(inter, _GROUP), bits) if keep_z else (None, None)
     xs = _group_bytes(m, hidden, 8) if keep_x and bits == 8 else (None, None)
-    return (*z, *xs, m * _up(inter, 8) * 2 if keep_h else None)
+    return _layout(*z, *xs, m * _up(inter, 8) * 2 if keep_h else None)
 
 
 def _ffn(x, w13, w2, activation, clamp_limit, residual, m, hidden, inter, n, bits=0, keep_x=False,
@@ -556,9 +559,11 @@ def _ffn(x, w13, w2, activation, clamp_limit, residual, m, hidden, inter, n, bit
     """(y, x, w13 and w2 as laid out, kept buffer); launches on the current device."""
     out = x.new_empty((m, n))
     ldh = _up(inter, 8)
-    kept, zc, zs, xc, xs, h = None, None, None, None, None, None
+    kept = zc = zs = xc = xs = h = None
     if keep_x or keep_z or keep_h:
-        kept, (zc, zs, xc, xs, h) = _parts(x, *_ffn_kept(m, hidden, inter, bits, keep_x, keep_z, keep_h))
+        size, offsets = _ffn_kept(m, hidden, inter, bits, keep_x, keep_z, keep_h)
+        kept = x.new_empty(size)
+        zc, zs, xc, xs, h = _at(kept.data_ptr(), offsets)
     if h is None:
         ws = x.new_empty((m, ldh))
         h = ws.data_ptr()
@@ -577,7 +582,9 @@ def _ffn(x, w13, w2, activation, clamp_limit, residual, m, hidden, inter, n, bit
           n, _DTYPES[x.dtype], ACTIVATIONS[activation], *_limit_args(clamp_limit),
           None if r is None else r.data_ptr(), 0 if r is None else _row_stride(r), h, ldh,
           out.data_ptr(), n, zc, 0 if zc is None else bits, zs, xc, xs, _stream(x.get_device()))
-    return out, a[0], b[0], c[0], kept
+    if kept is None:
+        return out, x, w13, w2, None
+    return out, _laid_out(a, x), _laid_out(b, w13), _laid_out(c, w2), kept
 
 
 def gated_feed_forward(x, w13, w2, *, activation="silu", clamp_limit=None, residual=None,
@@ -645,12 +652,15 @@ def _ffn_backward(grad_out, x, w13, w2, kept, kept_x, kept_z, kept_h, activation
         return gx, None if g13 is None else g13.zero_(), None if g2 is None else g2.zero_()
     if not (need_x or need_w13 or need_w2):
         return None, None, None
-    zc, zs, xc, xs, h = _addresses(kept, *_ffn_kept(m, hidden, inter, bits, kept_x, kept_z, kept_h))
+    zc, zs, xc, xs, h = _at(kept.data_ptr(),
+                            _ffn_kept(m, hidden, inter, bits, kept_x, kept_z, kept_h)[1])
     form_h = need_w2 and not kept_h
     ldh, lddz, ldx = _up(inter, 8), _up(2 * inter, 8), _up(hidden, 8)
-    ws, (dz, hw, xr) = _parts(grad_out, m * lddz * 2 if need_x or need_w13 or form_h else None,
-                              m * ldh * 2 if form_h else None,
-                              m * ldx * 2 if need_w13 and xc is not None else None)
+    size, offsets = _layout(m * lddz * 2 if need_x or need_w13 or form_h else None,
+                            m * ldh * 2 if form_h else None,
+                            m * ldx * 2 if need_w13 and xc is not None else None)
+    ws = grad_out.new_empty(size)
+    dz, hw, xr = _at(ws.data_ptr(), offsets)
     none = (None, None, 0, 0)
     dy, w = _operand(grad_out), _operand(w2)
     u = _operand(w13) if need_x else none
@@ -670,9 +680,12 @@ class _FeedForwardFunction(torch.autograd.Function):
         inner = need[0] or need[1]
         # w2's gradient alone needs h only, which is no larger than z in 8 bits
         keep_h = need[2] and (bits == 16 or not inner)
-        with _on(x.get_device()):
-            y, xk, w13k, w2k, kept = _ffn(x, w13, w2, activation, clamp_limit, residual, *shape, bits,
-                                          need[1], inner, keep_h)
+        args = (x, w13, w2, activation, clamp_limit, residual, *shape, bits, need[1], inner, keep_h)
+        if torch._C._cuda_getDevice() == x.get_device():
+            y, xk, w13k, w2k, kept = _ffn(*args)
+        else:
+            with torch.cuda.device(x.device):
+                y, xk, w13k, w2k, kept = _ffn(*args)
         ctx.save_for_backward(w13k, w2k, kept, xk if need[1] and bits == 16 else None)
         ctx.args = (need[1], inner, keep_h, activation, clamp_limit, *shape, bits)
         return y
@@ -683,7 +696,6 @@ class _FeedForwardFunction(torch.autograd.Function):
         need = ctx.needs_input_grad
         gx = g13 = g2 = None
         if need[0] or need[1] or need[2]:
-            w13, w2, kept, x = ctx.saved_tensors
-            with _on(grad_out.get_device()):
-                gx, g13, g2 = _ffn_backward(grad_out, x, w13, w2, kept, *ctx.args, *need[:3])
+            w13, w2, kept, x = ctx.saved_tensors  # (the engine has made their device current)
+            gx, g13, g2 = _ffn_backward(grad_out, x, w13, w2, kept, *ctx.args, *need[:3])
         return gx, g13, g2, grad_out if need[3] else None, None, None, None, None
