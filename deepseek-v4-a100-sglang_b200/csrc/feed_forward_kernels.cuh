@@ -83,13 +83,29 @@ __device__ __forceinline__ void pack_row(const float (&v)[32], uint32_t (&w)[16]
 }
 
 // ---- activations: value and slope ----
-// sigmoid(z) = 1 / (1 + exp(-z)) in fast fp32 (a few units of 2^-23, against
-// the 2^-9 and more of the 16-bit results); gelu_tanh is z sigmoid(2a) with
-// a = sqrt(2/pi) (z + 0.044715 z^3), since (1 + tanh a) / 2 = sigmoid(2a).
+// Fast fp32 (a few units of 2^-22, against the 2^-9 and more of the 16-bit
+// results); powers of two and reciprocals that underflow are 0.  gelu_tanh is
+// z sigmoid(2a) with a = sqrt(2/pi) (z + 0.044715 z^3), since (1 + tanh a) / 2 =
+// sigmoid(2a).
 enum Act : int { kActNone = 0, kActRelu = 1, kActSilu = 2, kActGelu = 3, kActGeluTanh = 4 };
 
+__device__ __forceinline__ float exp2_approx(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+__device__ __forceinline__ float rcp_approx(float a) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(a));
+  return r;
+}
+
+constexpr float kLog2E = 1.4426950408889634f;
+
+// 1 / (1 + exp(-z))
 __device__ __forceinline__ float sigmoid_fast(float z) {
-  return __fdividef(1.f, 1.f + __expf(-z));
+  return rcp_approx(1.f + exp2_approx(-kLog2E * z));
 }
 
 constexpr float kGeluC = 1.5957691216057308f;  // 2 sqrt(2 / pi)
@@ -100,14 +116,14 @@ constexpr float kGeluK = 0.044715f;
 // most 1.5e-7 (Abramowitz and Stegun, 7.1.26).  One exponential serves the
 // value and the slope.
 __device__ __forceinline__ float normal_cdf(float z, float& density) {
-  const float x = fabsf(z) * 0.70710678118654752f;
-  const float t = __fdividef(1.f, 1.f + 0.3275911f * x);
-  density = __expf(-x * x);
-  float q = 1.061405429f * t - 1.453152027f;
-  q = q * t + 1.421413741f;
-  q = q * t - 0.284496736f;
-  q = q * t + 0.254829592f;
-  q *= 0.5f * t * density;
+  // x = |z| / sqrt 2; half of erfc is one tail
+  const float t = rcp_approx(1.f + (0.3275911f * 0.70710678118654752f) * fabsf(z));
+  density = exp2_approx(z * z * (-0.5f * kLog2E));
+  float q = (0.5f * 1.061405429f) * t - 0.5f * 1.453152027f;
+  q = q * t + 0.5f * 1.421413741f;
+  q = q * t - 0.5f * 0.284496736f;
+  q = q * t + 0.5f * 0.254829592f;
+  q *= t * density;
   return z < 0.f ? q : 1.f - q;
 }
 
@@ -219,13 +235,6 @@ __device__ __forceinline__ void gated_backward_row(int act, float limit, const f
 constexpr int kGroup = 32;
 constexpr float kTinyGroup = 7.8886090522101181e-31f;  // 2^-100
 
-
-// 1 / a to about one unit of the last place, a in [2^-100, 2^128)
-__device__ __forceinline__ float rcp_approx(float a) {
-  float r;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(a));
-  return r;
-}
 
 // Whole steps up to amax: 127 in 8 bits, 32767 in 16.  The scale is rounded
 // toward zero: that many steps never pass amax, so the largest finite value
@@ -648,7 +657,7 @@ __global__ void __launch_bounds__(256, 4) act_backward_kernel(const ActBackward 
           for (int j = 0; j < 8; ++j) {
             float a, slope;
             act_both<K>(z[j], a, slope);
-            d[j] = col + j < p.n ? d[j] * slope : 0.f;
+            d[j] *= slope;  // (past the last column dy is 0, and the sum is not stored)
           }
           store_piece8<DT>(p.dz, row * p.lddz + col, col, p.n, p.vec_dz, d);
         }
