@@ -548,7 +548,8 @@ int dsv4_b200_checkpoint_int8(const void* x, int dtype, int64_t m, int64_t k, in
   const dim3 grid(static_cast<unsigned>(blocks));
   cudaStream_t st = as_stream(stream);
   const auto go = [&](auto kernel) {
-    launch_pdl(kernel, grid, dim3(256), 0, st, x, ldx, vec, m, k, k32, cb, codes, scales);
+    launch_pdl(kernel, grid, dim3(256), 0, st, x, ldx, vec, m, k, k32, static_cast<uint32_t>(cb), codes,
+               scales);
   };
   if (dtype == DSV4_F32) go(&checkpoint_kernel<DSV4_F32>);
   else if (dtype == DSV4_F16) go(&checkpoint_kernel<DSV4_F16>);
@@ -572,7 +573,8 @@ int dsv4_b200_restore_int8(const int8_t* codes, const float* scales, int64_t m, 
   const dim3 grid(static_cast<unsigned>(blocks));
   cudaStream_t st = as_stream(stream);
   const auto go = [&](auto kernel) {
-    launch_pdl(kernel, grid, dim3(256), 0, st, codes, scales, m, k, k32, cb, out, ldo, vec);
+    launch_pdl(kernel, grid, dim3(256), 0, st, codes, scales, m, k, k32, static_cast<uint32_t>(cb), out, ldo,
+               vec);
   };
   if (dtype == DSV4_F32) go(&restore_kernel<DSV4_F32>);
   else if (dtype == DSV4_F16) go(&restore_kernel<DSV4_F16>);
@@ -716,7 +718,8 @@ int dsv4_b200_pack_rows(const void* in, int64_t row_stride, int64_t col_stride, 
   const int64_t cb = (cols + 31) / 32, blocks = (rows + 31) / 32 * cb;
   DSV4_REQUIRE(blocks < (1ll << 31), "matrix too large");
   launch_pdl(&pack_rows_kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, as_stream(stream),
-             static_cast<const uint16_t*>(in), row_stride, col_stride, rows, cols, cb,
+             static_cast<const uint16_t*>(in), row_stride, col_stride, rows, cols,
+             static_cast<uint32_t>(cb),
              static_cast<uint16_t*>(out), ldo);
   return check_launch("pack_rows_kernel");
 }

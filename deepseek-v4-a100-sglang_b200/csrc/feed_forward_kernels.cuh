@@ -244,7 +244,15 @@ constexpr float kSteps8 = 127.f, kSteps16 = 32767.f;
 __device__ __forceinline__ float group_step(uint32_t amax_bits, float steps) {
   const float amax = __uint_as_float(amax_bits);
   if (amax_bits >= 0x7f800000u) return CUDART_NAN_F;
-  return amax < kTinyGroup ? 0.f : __fdiv_rz(amax, steps);
+  if (amax < kTinyGroup) return 0.f;
+  // the product is within two units of the last place of the quotient, and the
+  // remainder of a neighbour is exact: the largest with none below zero
+  float y = amax * (1.f / steps);
+  if (__fmaf_rn(-y, steps, amax) < 0.f) y = __uint_as_float(__float_as_uint(y) - 1);
+  if (__fmaf_rn(-y, steps, amax) < 0.f) y = __uint_as_float(__float_as_uint(y) - 1);
+  const float up = __uint_as_float(__float_as_uint(y) + 1);
+  if (__fmaf_rn(-up, steps, amax) >= 0.f) y = up;
+  return y;
 }
 
 // steps / amax to about 2^-22; 0 for a group that holds zeros or decodes to NaN
@@ -291,12 +299,14 @@ __device__ __noinline__ int quantize_code_near(float v, float q, float amax) {
   return q < 0.f ? -r : r;
 }
 
-// Four quotients -> four code bytes: adding 1.5 * 2^23 rounds to the nearest
-// whole number (ties to even) and leaves it in the low bits.
+// Adding 1.5 * 2^23 rounds to the nearest whole number (ties to even) and leaves
+// it in the low bits, so a code is one fused multiply-add of value and inverse.
+constexpr float kWhole = 12582912.f;
+
+// Four such sums -> four code bytes.
 __device__ __forceinline__ uint32_t pack_codes(float a, float b, float c, float d) {
-  constexpr float kMagic = 12582912.f;
-  const uint32_t lo = prmt(__float_as_uint(a + kMagic), __float_as_uint(b + kMagic), 0x0040u);
-  const uint32_t hi = prmt(__float_as_uint(c + kMagic), __float_as_uint(d + kMagic), 0x0040u);
+  const uint32_t lo = prmt(__float_as_uint(a), __float_as_uint(b), 0x0040u);
+  const uint32_t hi = prmt(__float_as_uint(c), __float_as_uint(d), 0x0040u);
   return prmt(lo, hi, 0x5410u);
 }
 
@@ -315,7 +325,7 @@ __device__ __forceinline__ uint32_t quantize4_f32(const float (&v)[4], float inv
       w |= (static_cast<uint32_t>(quantize_code_near(v[i], q[i], amax)) & 0xffu) << (8 * i);
     return w;
   }
-  return pack_codes(q[0], q[1], q[2], q[3]);
+  return pack_codes(q[0] + kWhole, q[1] + kWhole, q[2] + kWhole, q[3] + kWhole);
 }
 
 // What the backward pass needs of a value before its activation is kept as
@@ -340,7 +350,8 @@ __device__ __forceinline__ float keep_group8(const float (&v)[32], uint32_t (&co
   } else {
 #pragma unroll
     for (int j = 0; j < 8; ++j)
-      codes[j] = pack_codes(v[4 * j] * inv, v[4 * j + 1] * inv, v[4 * j + 2] * inv, v[4 * j + 3] * inv);
+      codes[j] = pack_codes(__fmaf_rn(v[4 * j], inv, kWhole), __fmaf_rn(v[4 * j + 1], inv, kWhole),
+                            __fmaf_rn(v[4 * j + 2], inv, kWhole), __fmaf_rn(v[4 * j + 3], inv, kWhole));
   }
   return group_step(top, kSteps8);
 }
@@ -366,9 +377,9 @@ __device__ __forceinline__ float keep_group16(const float (&v)[32], float limit,
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const float x = v[2 * j + i];
-      q[i] = __fmaf_rn(x, inv, 12582912.f);  // 1.5 * 2^23: the nearest whole number in the low bits
+      q[i] = __fmaf_rn(x, inv, kWhole);
       if (limited) {
-        const float n = q[i] - 12582912.f, toward = x < 0.f ? 1.f : -1.f;  // toward zero
+        const float n = q[i] - kWhole, toward = x < 0.f ? 1.f : -1.f;  // toward zero
         const bool over = fabsf(x) > limit, kept = fabsf(n * step) > limit;
         if (over && !kept) q[i] -= toward;
         if (!over && kept) q[i] += toward;
@@ -446,6 +457,12 @@ __device__ __forceinline__ void store_piece8(void* base, int64_t at, int64_t col
   }
 }
 
+__device__ __forceinline__ uint32_t max_u16x2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("max.u16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+
 // ---- activation checkpoint: rows -> 8-bit groups ----
 // A block takes 32 rows x 256 columns.  A lane owns 8 columns (a quarter of a
 // group, 16 bytes of a 16-bit row), so a warp reads 512 contiguous bytes of a
@@ -454,20 +471,21 @@ __device__ __forceinline__ void store_piece8(void* base, int64_t at, int64_t col
 // it.  Scales lie [group][row]; they pass through shared memory so that a warp
 // writes one group's 32 rows together.  Codes rows are padded to the group
 // with zeros.  Bound by issue slots next to memory: 16-bit rows stay packed
-// through the maximum (two values an instruction) and a code costs one product
-// and one addition.
+// through the maximum (two values an instruction) and a code costs one
+// multiply-add.
 template <int DT>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(256, DT == DSV4_F32 ? 4 : 6)
     checkpoint_kernel(const void* __restrict__ x, int64_t ld, int vec, int64_t m, int64_t k,
-                      int64_t k32, int64_t col_blocks, int8_t* __restrict__ codes,
+                      int64_t k32, uint32_t col_blocks, int8_t* __restrict__ codes,
                       float* __restrict__ scales) {
   pdl_entry();
   constexpr bool F32 = DT == DSV4_F32;
   constexpr int kWords = F32 ? 8 : 4;
   __shared__ float s_scale[8][33];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t row0 = (blockIdx.x / col_blocks) * 32 + warp;
-  const int64_t col = (blockIdx.x % col_blocks) * 256 + lane * 8;
+  const uint32_t row_block = blockIdx.x / col_blocks, col_block = blockIdx.x - row_block * col_blocks;
+  const int64_t row0 = static_cast<int64_t>(row_block) * 32 + warp;
+  const int64_t col = static_cast<int64_t>(col_block) * 256 + lane * 8;
   const uint32_t* const p =
       reinterpret_cast<const uint32_t*>(static_cast<const uint8_t*>(x) + (row0 * ld + col) * (F32 ? 4 : 2));
   const int64_t step = 8 * ld * (F32 ? 4 : 2);
@@ -515,9 +533,9 @@ __global__ void __launch_bounds__(256)
     } else {
       uint32_t t = raw[i][0] & 0x7fff7fffu;
 #pragma unroll
-      for (int j = 1; j < 4; ++j) t = __vmaxu2(t, raw[i][j] & 0x7fff7fffu);
-      t = __vmaxu2(t, __shfl_xor_sync(0xffffffffu, t, 1));
-      t = __vmaxu2(t, __shfl_xor_sync(0xffffffffu, t, 2));
+      for (int j = 1; j < 4; ++j) t = max_u16x2(t, raw[i][j] & 0x7fff7fffu);
+      t = max_u16x2(t, __shfl_xor_sync(0xffffffffu, t, 1));
+      t = max_u16x2(t, __shfl_xor_sync(0xffffffffu, t, 2));
       t = max(t & 0xffffu, t >> 16);
       top[i] = __float_as_uint(unpack_16<DT == DSV4_BF16>(t, 0));
     }
@@ -548,13 +566,13 @@ __global__ void __launch_bounds__(256)
       for (int j = 0; j < 8; ++j) q[j] = unpack_16<DT == DSV4_BF16>(raw[i][j >> 1], j & 1);
       if (inv > 0.f) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) q[j] *= inv;
+        for (int j = 0; j < 8; ++j) q[j] = __fmaf_rn(q[j], inv, kWhole);
       } else if (inv < 0.f) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) q[j] = group_quotient(q[j], __uint_as_float(top[i]));
+        for (int j = 0; j < 8; ++j) q[j] = group_quotient(q[j], __uint_as_float(top[i])) + kWhole;
       } else {  // zeros, or a group that holds an infinity or a NaN
 #pragma unroll
-        for (int j = 0; j < 8; ++j) q[j] = 0.f;
+        for (int j = 0; j < 8; ++j) q[j] = kWhole;
       }
       w[0] = pack_codes(q[0], q[1], q[2], q[3]);
       w[1] = pack_codes(q[4], q[5], q[6], q[7]);
@@ -563,20 +581,21 @@ __global__ void __launch_bounds__(256)
       *reinterpret_cast<uint2*>(c + i * 8 * k32) = make_uint2(w[0], w[1]);
   }
   __syncthreads();
-  const int64_t group = (blockIdx.x % col_blocks) * 8 + warp, row = row0 - warp + lane;
+  const int64_t group = static_cast<int64_t>(col_block) * 8 + warp, row = row0 - warp + lane;
   if (group * kGroup < k32 && row < m) scales[group * m + row] = s_scale[warp][lane];
 }
 
 template <int DT>
 __global__ void __launch_bounds__(256)
     restore_kernel(const int8_t* __restrict__ codes, const float* __restrict__ scales, int64_t m,
-                   int64_t k, int64_t k32, int64_t col_blocks, void* __restrict__ out, int64_t ldo,
+                   int64_t k, int64_t k32, uint32_t col_blocks, void* __restrict__ out, int64_t ldo,
                    int vec) {
   pdl_entry();
   __shared__ float s_scale[8][33];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t row0 = (blockIdx.x / col_blocks) * 32;
-  const int64_t col = (blockIdx.x % col_blocks) * 256 + lane * 8;
+  const uint32_t row_block = blockIdx.x / col_blocks, col_block = blockIdx.x - row_block * col_blocks;
+  const int64_t row0 = static_cast<int64_t>(row_block) * 32;
+  const int64_t col = static_cast<int64_t>(col_block) * 256 + lane * 8;
   uint2 c[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -584,7 +603,7 @@ __global__ void __launch_bounds__(256)
     c[i] = make_uint2(0, 0);
     if (row < m && col < k32) c[i] = *reinterpret_cast<const uint2*>(codes + row * k32 + col);
   }
-  const int64_t group = (blockIdx.x % col_blocks) * 8 + warp, srow = row0 + lane;
+  const int64_t group = static_cast<int64_t>(col_block) * 8 + warp, srow = row0 + lane;
   s_scale[warp][lane] = group * kGroup < k32 && srow < m ? scales[group * m + srow] : 0.f;
   __syncthreads();
 #pragma unroll
@@ -705,11 +724,12 @@ __global__ void __launch_bounds__(256)
 // 32 x 32 tiles through shared memory: reads follow the smaller stride.
 __global__ void __launch_bounds__(256)
     pack_rows_kernel(const uint16_t* __restrict__ in, int64_t s0, int64_t s1, int64_t rows,
-                     int64_t cols, int64_t col_blocks, uint16_t* __restrict__ out, int64_t ldo) {
+                     int64_t cols, uint32_t col_blocks, uint16_t* __restrict__ out, int64_t ldo) {
   pdl_entry();
   __shared__ uint16_t tile[32][33];
   const int a = threadIdx.x & 31, b = threadIdx.x >> 5;
-  const int64_t r0 = (blockIdx.x / col_blocks) * 32, c0 = (blockIdx.x % col_blocks) * 32;
+  const uint32_t row_block = blockIdx.x / col_blocks, col_block = blockIdx.x - row_block * col_blocks;
+  const int64_t r0 = static_cast<int64_t>(row_block) * 32, c0 = static_cast<int64_t>(col_block) * 32;
   const bool by_rows = s1 <= s0 || s0 == 0;
 #pragma unroll
   for (int i = 0; i < 32; i += 8) {
