@@ -361,9 +361,66 @@ __device__ __forceinline__ float keep_group8(const float (&v)[32], uint32_t (&co
 // lose or gain its whole gradient.  For relu a value other than zero keeps its
 // sign the same way.  That is one step instead of half a step next to the
 // border.
+//
+// Equal steps serve a group as long as no value stands out: with the largest at
+// most 4 times the root of the mean square (of the `live` columns that there
+// are) they are within 6.2e-5 of that root.  A group with an outlier would lose
+// its small values, and one with an infinity or a NaN all of them: those are
+// kept as fp16 multiples of a power of two, every value within 2^-12 of itself,
+// and say so by a negative scale.
+constexpr float kStandsOut = 16.f;
+
+// acc += a * a, two at a time
+__device__ __forceinline__ void add_squares(float (&acc)[2], float a0, float a1) {
+  asm("{\n\t.reg .b64 a, c;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 c, {%0, %1};\n\t"
+      "fma.rn.f32x2 c, a, a, c;\n\tmov.b64 {%0, %1}, c;\n\t}"
+      : "+f"(acc[0]), "+f"(acc[1])
+      : "f"(a0), "f"(a1));
+}
+
+__device__ __forceinline__ float keep_group16_wide(const float (&v)[32], float limit, bool keep_sign,
+                                                   uint32_t (&codes)[16]) {
+  uint32_t top = 0;  // of the finite values
+#pragma unroll
+  for (int j = 0; j < 32; ++j) {
+    const uint32_t b = __float_as_uint(v[j]) & 0x7fffffffu;
+    if (b < 0x7f800000u) top = max(top, b);
+  }
+  // the largest lands in [2^14, 2^15); scales from 2^-114 to 2^113
+  const uint32_t e = max(top >> 23, 27u) - 14u;
+  const float scale = __uint_as_float(e << 23), inv = __uint_as_float((254u - e) << 23);
+  const bool limited = limit < CUDART_INF_F || keep_sign;
+#pragma unroll
+  for (int j = 0; j < 16; ++j) {
+    uint32_t w = pack_16<false>(v[2 * j] * inv, v[2 * j + 1] * inv);
+    if (limited) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const float x = v[2 * j + i];
+        const uint32_t one = i ? 0x10000u : 1u, n = i ? w >> 16 : w & 0xffffu;
+        const bool over = fabsf(x) > limit, kept = fabsf(unpack_16<false>(w, i) * scale) > limit;
+        if (over && !kept) w += one;  // magnitudes count up away from zero
+        if (!over && kept) w -= one;
+        if (keep_sign && (n & 0x7fffu) == 0 && x != 0.f) w += one;
+      }
+    }
+    codes[j] = w;
+  }
+  return -scale;
+}
+
 __device__ __forceinline__ float keep_group16(const float (&v)[32], float limit, bool keep_sign,
-                                              uint32_t (&codes)[16]) {
-  const uint32_t top = group_top(v);
+                                              int live, uint32_t (&codes)[16]) {
+  float most = 0.f, sum[2] = {};
+#pragma unroll
+  for (int j = 0; j < 16; ++j) {
+    most = fmaxf(most, fmaxf(fabsf(v[2 * j]), fabsf(v[2 * j + 1])));
+    add_squares(sum, v[2 * j], v[2 * j + 1]);
+  }
+  const float squares = sum[0] + sum[1];  // infinite or NaN where a value is
+  if (!(squares < CUDART_INF_F && most * most * live <= kStandsOut * squares))
+    return keep_group16_wide(v, limit, keep_sign, codes);
+  const uint32_t top = __float_as_uint(most);
   const float inv = group_inverse(top, kSteps16), step = group_step(top, kSteps16);
   if (inv == 0.f) {
 #pragma unroll
@@ -395,6 +452,18 @@ __device__ __forceinline__ float keep_group16(const float (&v)[32], float limit,
 // of a float 2^23 + code.
 __device__ __forceinline__ float code16_value(uint32_t w, int hi) {
   return __uint_as_float(prmt(w ^ 0x80008000u, 0x4b000000u, hi ? 0x7432u : 0x7410u)) - 8421376.f;
+}
+
+// N 16-bit codes of a group (scale < 0: fp16 multiples) -> values
+template <int N>
+__device__ __forceinline__ void kept16_values(const uint32_t (&w)[N / 2], float scale, float (&v)[N]) {
+  if (scale < 0.f) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) v[j] = -scale * unpack_16<false>(w[j >> 1], j & 1);
+  } else {
+#pragma unroll
+    for (int j = 0; j < N; ++j) v[j] = scale * code16_value(w[j >> 1], j & 1);
+  }
 }
 
 __device__ __forceinline__ float code8_value(uint32_t w, int byte) {
@@ -669,8 +738,7 @@ __global__ void __launch_bounds__(256, 4) act_backward_kernel(const ActBackward 
           } else {
             const uint4 c = *reinterpret_cast<const uint4*>(static_cast<const int16_t*>(p.zq) + row * p.n32 + col);
             const uint32_t w[4] = {c.x, c.y, c.z, c.w};
-#pragma unroll
-            for (int j = 0; j < 8; ++j) z[j] = s * code16_value(w[j >> 1], j & 1);
+            kept16_values<8>(w, s, z);
           }
 #pragma unroll
           for (int j = 0; j < 8; ++j) {

@@ -335,9 +335,10 @@ __device__ __forceinline__ void codes_to_rows(uint32_t slice, int lane, const ui
   __syncwarp();
 }
 
-// A warp's 32 rows of one kept group, columns `at`.. of code rows of `ld`.
+// A warp's 32 rows of one kept group, columns `at`.. of code rows of `ld`; the
+// first `live` of them are columns of the matrix.
 __device__ __forceinline__ void keep_rows(const F16GemmParams& p, uint32_t slice, int lane,
-                                          const float (&v)[32], int64_t ld, int row0, int at) {
+                                          const float (&v)[32], int64_t ld, int row0, int at, int live) {
   float s;
   if (p.zbits == 8) {
     uint32_t q[8];
@@ -345,7 +346,7 @@ __device__ __forceinline__ void keep_rows(const F16GemmParams& p, uint32_t slice
     codes_store(slice, lane, q, static_cast<int8_t*>(p.zq), ld, row0, p.m, at);
   } else {
     uint32_t q[16];
-    s = keep_group16(v, p.limit, p.act == kActRelu, q);
+    s = keep_group16(v, p.limit, p.act == kActRelu, live, q);
     chunk_store(slice, lane, q, F16Mat{p.zq, ld, 1}, row0, p.m, at, static_cast<int>(ld));
   }
   if (row0 + lane < p.m) p.zs[static_cast<int64_t>(at >> 5) * p.m + row0 + lane] = s;
@@ -364,8 +365,7 @@ __device__ __forceinline__ void kept_rows(const F16GemmParams& p, uint32_t slice
     uint32_t w[16];
     chunk_fetch(r, F16Mat{p.zq, ld, 1}, lane, row0, p.m, at, static_cast<int>(ld));
     chunk_to_rows(slice, lane, r, true, w);
-#pragma unroll
-    for (int j = 0; j < 32; ++j) v[j] = s * code16_value(w[j >> 1], j & 1);
+    kept16_values<32>(w, s, v);
   }
 }
 
@@ -542,7 +542,7 @@ __global__ void __launch_bounds__(F16Roles<EPI>::kThreads, 1)
               for (int j = 0; j < 32; ++j)
                 if (col + j >= p.n) v[j] = 0.f;
             }
-            keep_rows(p, slice0, lane, v, p.n32, row0, col);
+            keep_rows(p, slice0, lane, v, p.n32, row0, col, min(32, p.n - col));
           }
           act_row(p.act, v);
           if (p.residual.p) {
@@ -563,8 +563,8 @@ __global__ void __launch_bounds__(F16Roles<EPI>::kThreads, 1)
               for (int j = 0; j < 32; ++j)
                 if (col + j >= p.n) g[j] = u[j] = 0.f;
             }
-            keep_rows(p, slice0, lane, g, 2 * p.n32, row0, col);
-            keep_rows(p, slice1, lane, u, 2 * p.n32, row0, static_cast<int>(p.n32) + col);
+            keep_rows(p, slice0, lane, g, 2 * p.n32, row0, col, min(32, p.n - col));
+            keep_rows(p, slice1, lane, u, 2 * p.n32, row0, static_cast<int>(p.n32) + col, min(32, p.n - col));
           }
 #pragma unroll
           for (int j = 0; j < 32; ++j) {

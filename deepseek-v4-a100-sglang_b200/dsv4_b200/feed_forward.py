@@ -8,15 +8,17 @@ projections), forward and backward.
 
 bf16 and fp16; sums, activations and their slopes in fp32, one rounding where
 a value is stored.  The values before an activation are kept for the backward
-pass as groups of 32 with a shared scale, in 16 bits.  ``dense_forward`` and ``gated_feed_forward`` are
-differentiable; their ``*_save`` / ``*_backward`` forms give the same steps
-without autograd (and are the ones to capture into a CUDA graph).  With
-``checkpoint="int8"`` what the backward pass needs is kept in 8 bits.  Every
-call is asynchronous on the current stream of the tensors' device; there is
-no CPU path.
+pass as groups of 32 with a shared scale, in 16 bits (as whole steps, or as
+fp16 multiples where a value stands out of its group).  ``dense_forward`` and
+``gated_feed_forward`` are differentiable; their ``*_save`` / ``*_backward``
+forms give the same steps without autograd (and are the ones to capture into a
+CUDA graph).  With ``checkpoint="int8"`` what the backward pass needs is kept
+in 8 bits.  Every call is asynchronous on the current stream of the tensors'
+device; there is no CPU path.
 
 Results follow the inputs' values: NaN and infinities propagate as the
-formulas say.  All results are the same bits from call to call.
+formulas say (kept in 8 bits they make their whole group of 32 NaN in the
+backward pass).  All results are the same bits from call to call.
 """
 
 from __future__ import annotations
@@ -236,6 +238,8 @@ def checkpoint_int8(x: torch.Tensor) -> Int8Checkpoint:
     """Keep the rows of ``x`` [M, K] (fp32, fp16 or bf16) in 8 bits: 1.125
     bytes per value.  ``restore_int8(checkpoint_int8(x))`` differs from x by at
     most half a step, ``amax / 254`` of its group, and the rounding to x's type."""
+    if not isinstance(x, torch.Tensor):
+        raise TypeError(f"x must be a tensor, got {type(x).__name__}")
     shape, dtype = x.shape, x.dtype
     if len(shape) != 2:
         raise ValueError(f"x must be 2-D, got shape {tuple(shape)}")
@@ -264,6 +268,8 @@ def checkpoint_int8(x: torch.Tensor) -> Int8Checkpoint:
 
 def restore_int8(checkpoint: Int8Checkpoint, dtype: Optional[torch.dtype] = None) -> torch.Tensor:
     """The kept rows, in their own type or in ``dtype``."""
+    if not isinstance(checkpoint, Int8Checkpoint):
+        raise TypeError(f"checkpoint must be an Int8Checkpoint, got {type(checkpoint).__name__}")
     dtype = checkpoint.dtype if dtype is None else dtype
     if dtype not in _CHECKPOINT_DTYPES:
         raise TypeError(f"dtype must be fp32, fp16 or bf16, got {dtype}")

@@ -397,8 +397,11 @@ DSV4_API int dsv4_b200_mxfp4_int8_dense_gemm_noalloc(const int8_t* a_q, const fl
  * Kept values are groups of 32 values of a row that share an fp32 scale
  * amax / steps (rounded toward zero), steps 127 in 8 bits and 32767 in 16:
  * codes int8 or int16 [m][ceil32(k)], scales [ceil32(k) / 32][m], codes 16-byte
- * aligned.  code = steps v / amax to the nearest, ties to even; a group with
- * an infinity or a NaN decodes to NaN, one whose amax is below 2^-100 to zeros.
+ * aligned.  code = steps v / amax to the nearest, ties to even; a group of 8
+ * bits with an infinity or a NaN decodes to NaN, a group whose amax is below
+ * 2^-100 to zeros.  A group of 16 bits whose amax is over 4 times its root
+ * mean square, or that holds an infinity or a NaN, has a negative scale -2^e,
+ * and its codes are the fp16 numbers v / 2^e.
  * z_bits = 0, 8 or 16 (0: z_codes and z_scales NULL). */
 typedef enum dsv4_activation {
   DSV4_ACT_NONE = 0,

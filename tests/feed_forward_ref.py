@@ -90,13 +90,18 @@ def tiny_of(dtype):
 
 def kept(z, mode):
     """z as the backward pass reads it: groups of 32, off by half a step of
-    amax / 32767, or a whole one to stay on its side of a limit or of zero; or
-    in 8 bits."""
+    amax / 32767, or a whole one to stay on its side of a limit or of zero (a
+    group whose largest value is over 4 times its root mean square: fp16
+    multiples of a power of two up to amax / 2^14, off by at most a step of those); or in 8 bits."""
     if mode is None:
         k = z.v.shape[1]
-        top = torch.nn.functional.pad(z.v.abs() + z.e, (0, -k % GROUP)).reshape(z.v.shape[0], -1, GROUP)
-        top = top.amax(2, keepdim=True).expand_as(top).reshape(z.v.shape[0], -1)[:, :k]
-        return Bounded(z.v, z.e + 1.001 * top / 32767)
+        g = torch.nn.functional.pad(z.v.abs() + z.e, (0, -k % GROUP)).reshape(z.v.shape[0], -1, GROUP)
+        top = g.amax(2, keepdim=True).expand_as(g)
+        live = (k - GROUP * torch.arange(g.shape[1], device=g.device)).clamp(max=GROUP).view(1, -1, 1)
+        ratio = top.square() * live / g.square().sum(2, keepdim=True).clamp(min=1e-300)
+        even, wide = 1.001 * top / 32767, 2.0 ** -10 * g + 2.0 ** -38 * top
+        e = torch.where(ratio < 15, even, torch.where(ratio > 17, wide, torch.maximum(even, wide)))
+        return Bounded(z.v, z.e + e.reshape(z.v.shape[0], -1)[:, :k])
     back, step, edge = eight(z.v)
     # the largest value of a group may be off as well: the step with it
     top_e = torch.nn.functional.pad(z.e, (0, -z.e.shape[1] % GROUP)).reshape(z.e.shape[0], -1, GROUP)

@@ -86,6 +86,10 @@ def test_checkpoint_refusals():
     with pytest.raises(RuntimeError, match="CUDA"):
         D.checkpoint_int8(z(4, 4))
     good = D.Int8Checkpoint(torch.zeros((4, 32), dtype=torch.int8), torch.zeros((1, 4)), (4, 20), BF16)
+    with pytest.raises(TypeError, match="tensor"):
+        D.checkpoint_int8([[1.0]])
+    with pytest.raises(TypeError, match="Int8Checkpoint"):
+        D.restore_int8(z(4, 4))
     with pytest.raises(RuntimeError, match="CUDA"):
         D.restore_int8(good)
     with pytest.raises(TypeError, match="dtype"):

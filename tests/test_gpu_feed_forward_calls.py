@@ -190,6 +190,78 @@ def test_not_finite_gradients(mode):
     assert torch.isnan(g13).all() and torch.isnan(g2).all()
 
 
+@pytest.mark.parametrize("kind", ["relu", "silu", "gelu", "gelu_tanh"])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_values_beside_an_outlier(kind, dtype):
+    """One column in 32 far above the rest: its neighbours' gradients are as
+    exact as elsewhere."""
+    import dsv4_b200 as D
+    m, k, n = 70, 64, 200
+    x, w, b, _ = dense_case(m, k, n, dtype)
+    w, b = w / 16, b / 16
+    b[5::32] = 4000
+    dy = rand(m, n, dtype=dtype, std=0.1, seed=3)
+    want = R.dense(x, w, b, None, kind, dtype, dy)
+    y, saved = D.dense_forward_save(x, w, b, activation=kind)
+    R.assert_within("y", y, want["y"])
+    for g, key in zip(D.dense_backward(dy, saved), ("grad_x", "grad_weight", "grad_bias")):
+        R.assert_within(key, g, want[key])
+    # the block: gates far above in one column of each group (every token), limits inside the others
+    x, w13, w2, _ = ffn_case(m, k, 96, 72, dtype, residual=False)
+    x[:, 0], w13[5:96:32, 0] = 8, 128
+    dy = rand(m, 72, dtype=dtype, std=0.1, seed=4)
+    for limit in (None, 0.37):
+        want = R.ffn(x, w13, w2, None, kind, limit, dtype, dy)
+        y, saved = D.gated_feed_forward_save(x, w13, w2, activation=kind, clamp_limit=limit)
+        R.assert_within("y", y, want["y"])
+        for g, key in zip(D.gated_feed_forward_backward(dy, saved), ("grad_x", "grad_w13", "grad_w2")):
+            R.assert_within(key, g, want[key])
+
+
+def test_infinities_that_the_formula_masks():
+    """A value before the activation that is infinite, with a slope of zero
+    there: its neighbours' gradients are those of a large finite value."""
+    import dsv4_b200 as D
+    m, k, n = 70, 64, 80
+    x, w, b, _ = dense_case(m, k, n, BF16)
+    dy = rand(m, n, std=0.1, seed=3)
+    b[7] = -1000
+    want = R.dense(x, w, b, None, "relu", BF16, dy)
+    b[7] = -math.inf
+    y, saved = D.dense_forward_save(x, w, b, activation="relu")
+    R.assert_within("y", y, want["y"])
+    for g, key in zip(D.dense_backward(dy, saved), ("grad_x", "grad_weight", "grad_bias")):
+        R.assert_within(key, g, want[key])
+    # gate and up past the limit by an infinite weight (column 0 of dx is 0 times infinity)
+    x, w13, w2, _ = ffn_case(m, k, 48, 72, BF16, residual=False)
+    x[:, 0] = 1
+    dy = rand(m, 72, std=0.1, seed=4)
+    w13[9, 0], w13[48 + 20, 0] = 1000, -1000
+    want = R.ffn(x, w13, w2, None, "silu", 1.5, BF16, dy)
+    w13[9, 0], w13[48 + 20, 0] = math.inf, -math.inf
+    y, saved = D.gated_feed_forward_save(x, w13, w2, clamp_limit=1.5)
+    R.assert_within("y", y, want["y"])
+    gx, g13, g2 = D.gated_feed_forward_backward(dy, saved)
+    R.assert_within("grad_w13", g13, want["grad_w13"])
+    R.assert_within("grad_w2", g2, want["grad_w2"])
+    assert torch.isnan(gx[:, 0]).all()
+    R.assert_within("grad_x", gx[:, 1:], R.Bounded(want["grad_x"].v[:, 1:], want["grad_x"].e[:, 1:]))
+    # NaN in one column stays there
+    x, w, b, _ = dense_case(m, k, n, BF16)
+    dy = rand(m, n, std=0.1, seed=5)
+    b[7] = 1000
+    want = R.dense(x, w, b, None, "silu", BF16, dy)
+    b[7] = math.nan
+    y, saved = D.dense_forward_save(x, w, b, activation="silu")
+    gx, gw, gb = D.dense_backward(dy, saved)
+    keep = torch.arange(n, device="cuda") != 7
+    for key in ("grad_weight", "grad_bias"):
+        got = {"grad_weight": gw, "grad_bias": gb}[key]
+        R.assert_within(key, got[keep], R.Bounded(want[key].v[keep], want[key].e[keep]))
+        assert torch.isnan(got[7]).all()
+    assert torch.isnan(gx).all()
+
+
 def test_extreme_activation_arguments():
     """Values far out: no activation or slope makes NaN of a finite number."""
     import dsv4_b200 as D
