@@ -470,32 +470,16 @@ __device__ __forceinline__ float code8_value(uint32_t w, int byte) {
   return __uint_as_float(prmt(w ^ 0x80808080u, 0x4b000000u, 0x7440u + byte)) - 8388736.f;
 }
 
-// 8 consecutive values of a 16- or 32-bit row; pieces past `cols` read as 0.
-template <int DT>
-__device__ __forceinline__ void load_piece8(const void* base, int64_t at, int64_t col,
-                                            int64_t cols, bool vec, float (&v)[8]) {
-  if constexpr (DT == DSV4_F32) {
-    const float* p = static_cast<const float*>(base) + at;
-    if (vec && col + 8 <= cols) {
-      const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
-      v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
-    } else {
+// 8 consecutive 16-bit values of a row, packed; those past `cols` read as 0.
+__device__ __forceinline__ uint4 load_words8(const void* base, int64_t at, int64_t col, int64_t cols,
+                                             bool vec) {
+  const uint16_t* p = static_cast<const uint16_t*>(base) + at;
+  if (vec && col + 8 <= cols) return *reinterpret_cast<const uint4*>(p);
+  uint32_t w[4] = {};
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = col + j < cols ? p[j] : 0.f;
-    }
-  } else {
-    constexpr bool BF16 = DT == DSV4_BF16;
-    const uint16_t* p = static_cast<const uint16_t*>(base) + at;
-    if (vec && col + 8 <= cols) {
-      const uint4 a = *reinterpret_cast<const uint4*>(p);
-      const uint32_t w[4] = {a.x, a.y, a.z, a.w};
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = unpack_16<BF16>(w[j >> 1], j & 1);
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = col + j < cols ? unpack_16<BF16>(p[j], 0) : 0.f;
-    }
-  }
+  for (int j = 0; j < 8; ++j)
+    if (col + j < cols) w[j >> 1] |= static_cast<uint32_t>(p[j]) << (16 * (j & 1));
+  return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
 template <int DT>
@@ -723,22 +707,38 @@ __global__ void __launch_bounds__(256, 4) act_backward_kernel(const ActBackward 
   if (col < p.n) {
     act_dispatch(p.act, [&](auto kind) {
       constexpr int K = decltype(kind)::value;
-#pragma unroll 2
+      const float* const zs = p.zs + col / kGroup * p.m;
+      // the next row's loads are in flight while a row is worked on
+      const auto fetch = [&](int64_t row, uint4& d, uint4& c, float& s) {
+        d = load_words8(p.dy, row * p.lddy + col, col, p.n, p.vec_dy);
+        if constexpr (K != kActNone) {
+          s = zs[row];
+          if (p.zbits == 8) {
+            const uint2 q = *reinterpret_cast<const uint2*>(static_cast<const int8_t*>(p.zq) + row * p.n32 + col);
+            c.x = q.x, c.y = q.y;
+          } else {
+            c = *reinterpret_cast<const uint4*>(static_cast<const int16_t*>(p.zq) + row * p.n32 + col);
+          }
+        }
+      };
+      uint4 nd = {}, nc = {};
+      float ns = 0.f;
+      if (begin + warp < end) fetch(begin + warp, nd, nc, ns);
+#pragma unroll 1
       for (int64_t row = begin + warp; row < end; row += 8) {
+        const uint32_t dw[4] = {nd.x, nd.y, nd.z, nd.w}, c[4] = {nc.x, nc.y, nc.z, nc.w};
+        const float s = ns;
+        if (row + 8 < end) fetch(row + 8, nd, nc, ns);
         float d[8];
-        load_piece8<DT>(p.dy, row * p.lddy + col, col, p.n, p.vec_dy, d);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) d[j] = unpack_16<BF16>(dw[j >> 1], j & 1);
         if constexpr (K != kActNone) {
           float z[8];
-          const float s = p.zs[(col / kGroup) * p.m + row];
           if (p.zbits == 8) {
-            const uint2 c = *reinterpret_cast<const uint2*>(static_cast<const int8_t*>(p.zq) + row * p.n32 + col);
-            const uint32_t w[2] = {c.x, c.y};
 #pragma unroll
-            for (int j = 0; j < 8; ++j) z[j] = s * code8_value(w[j >> 2], j & 3);
+            for (int j = 0; j < 8; ++j) z[j] = s * code8_value(c[j >> 2], j & 3);
           } else {
-            const uint4 c = *reinterpret_cast<const uint4*>(static_cast<const int16_t*>(p.zq) + row * p.n32 + col);
-            const uint32_t w[4] = {c.x, c.y, c.z, c.w};
-            kept16_values<8>(w, s, z);
+            kept16_values<8>(c, s, z);
           }
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
