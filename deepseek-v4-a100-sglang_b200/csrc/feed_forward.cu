@@ -309,10 +309,10 @@ cudaError_t stream_attrs() {
 }
 
 // The faster of the two products by the counts above (values before the
-// activation are kept by the pair product only).  1 to 128 tokens stream nearly
+// activation are kept by the pair product only).  Up to 128 tokens stream nearly
 // always; beyond that it is long contractions of few columns: 256 tokens 4096
 // -> 1024 take 8.0 us streamed and 13.7 in pairs, 512 tokens 7168 -> 4096 37
-// and 27.
+// and 27.  (Fewest tokens: takes_rows.)
 bool takes_stream(const F16GemmParams& q, bool gated, int w_mn, F16StreamParams& p, bool* two) {
   if (q.zbits != 0 || q.m > 1024) return false;
   p.tn = stream_tokens(q.m);
