@@ -94,6 +94,15 @@ int ensure_init() {
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return fail(DSV4_ERR_CUDA, "cudaGetDevice: %s", cudaGetErrorString(e));
   if (dev < 0 || dev >= kMaxDevices) return fail(DSV4_ERR_CUDA, "device index %d out of range", dev);
+  // tensor maps are encoded by the driver, which wants the device's context
+  // current on this thread; a thread that has made no binding runtime call yet
+  // (an autograd engine's, say) has none
+  thread_local int bound = -1;
+  if (bound != dev) {
+    e = cudaSetDevice(dev);
+    if (e != cudaSuccess) return fail(DSV4_ERR_CUDA, "cudaSetDevice: %s", cudaGetErrorString(e));
+    bound = dev;
+  }
   std::lock_guard<std::mutex> lk(g_init_mu);
   if (g_inited[dev]) return DSV4_OK;
   int major = 0, minor = 0;

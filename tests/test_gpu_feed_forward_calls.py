@@ -341,6 +341,48 @@ def test_side_streams():
         assert all(same(x, y) for a, b in zip(got_t, trained) for x, y in zip(a, b))
 
 
+@pytest.mark.parametrize("m", [1, 64, 300])
+def test_a_thread_that_has_used_no_cuda_yet(m):
+    """Calls from a new thread whose memory all comes from the allocator's
+    cache, so that no other call has set the thread up: both directions."""
+    import threading
+
+    import dsv4_b200 as D
+    x, w13, w2, r = ffn_case(m, 512, 256, 512, BF16)
+    dy = rand(m, 512, seed=2)
+
+    def step():
+        y, saved = D.gated_feed_forward_save(x, w13, w2, residual=r)
+        return (y, D.gated_feed_forward(x, w13, w2), D.dense_forward(x, w13),
+                *D.gated_feed_forward_backward(dy, saved))
+
+    def forget(f):  # leaves its memory in the cache
+        f()
+        torch.cuda.synchronize()
+
+    want = step()
+    forget(step)
+    got, failed = [], []
+
+    def run(f):
+        try:
+            got.append(f())
+        except Exception as e:  # noqa: BLE001 - reported below
+            failed.append(e)
+
+    for f in (lambda: D.gated_feed_forward_backward(dy, saved), lambda: D.dense_forward(x, w13),
+              lambda: D.gated_feed_forward(x, w13, w2), step):
+        y, saved = D.gated_feed_forward_save(x, w13, w2, residual=r)
+        t = threading.Thread(target=run, args=(f,))
+        t.start()
+        t.join()
+    torch.cuda.synchronize()
+    assert not failed, failed
+    g, d, y, all_of_it = got
+    assert all(same(a, b) for a, b in zip(g, want[3:])) and same(d, want[2]) and same(y, want[1])
+    assert all(same(a, b) for a, b in zip(all_of_it, want))
+
+
 def test_cuda_graphs():
     """Captured forward and training steps, replayed with other inputs, two
     graphs in turn: the results of eager calls."""
