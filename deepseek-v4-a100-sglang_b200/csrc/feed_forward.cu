@@ -279,7 +279,8 @@ int launch_stream_gemm(const F16GemmParams& q, F16StreamParams& p, bool two, con
 }
 
 // 32 KB of shared memory for two blocks; the rest of the SM's memory is L1, which
-// holds the loads in flight (all of it shared: 30.7 us for the block above).
+// holds the loads in flight (a block of 7168 -> 2048 -> 7168: 18.4 us, with all of it
+// shared 30.7).
 template <int EPI>
 cudaError_t rows_attrs() {
   void* const fns[4] = {reinterpret_cast<void*>(&f16_rows_gemm_kernel<EPI, true, true>),
@@ -322,12 +323,20 @@ bool takes_stream(const F16GemmParams& q, bool gated, int w_mn, F16StreamParams&
   return pick_stream(q, gated, p, two) < pair_us;
 }
 
-// Up to 8 tokens, both operands by rows (at any alignment): for one token 2048 x 2048 takes 3.0 us
-// here and 5.0 streamed, 7168 x 2048 7.5 and 8.9, 4096 x 7168 13.2 and 12.8, 256 x
-// 7168 6.1 and 4.9, a block of 7168 -> 2048 -> 7168 back to back 18.9 and 22.0
-// (23.7 with one product of each kind: they split the SM's memory differently).
-bool takes_rows(const F16GemmParams& q, int x_mn, int w_mn) {
-  return q.m <= kRowsMaxTokens && q.zbits == 0 && !x_mn && !w_mn;
+bool aligned_rows(const void* x, int64_t ldx, const void* w, int64_t ldw) {
+  return aligned16(x) && ldx % 8 == 0 && aligned16(w) && ldw % 8 == 0;
+}
+
+// Up to 8 tokens, both operands by rows: for one token 2048 x 2048 takes 3.3 us
+// here and 5.1 streamed, 7168 x 2048 7.4 and 9.1, 4096 x 7168 11.7 and 12.8, a
+// block of 7168 -> 2048 -> 7168 back to back 18.4 and 22.1.  Long rows of few
+// columns leave most SMs without a block, so those are streamed (1000 x 4096,
+// 63 blocks: 5.5 and 5.2; 256 x 7168, 16 blocks: 8.1 and 5.1) unless their
+// alignment needs this product.
+bool takes_rows(const F16GemmParams& q, bool gated, int x_mn, int w_mn, bool aligned) {
+  if (q.m > kRowsMaxTokens || q.zbits != 0 || x_mn || w_mn) return false;
+  const int64_t blocks = (static_cast<int64_t>(q.n) + (gated ? 7 : 15)) / (gated ? 8 : 16);
+  return !aligned || q.k <= 2048 || 2 * blocks >= sm_count();
 }
 
 template <int EPI>
@@ -341,7 +350,7 @@ int launch_rows_gemm(const F16GemmParams& q, const void* x, int64_t ldx, const v
                      q.k, q.up_row, q.act, q.limit, q.bias, q.residual, q.out};
   constexpr int kCols = EPI == kEpiGated ? 8 : 16;
   const dim3 grid(static_cast<unsigned>((q.n + kCols - 1) / kCols));
-  const bool aligned = aligned16(x) && ldx % 8 == 0 && aligned16(w) && ldw % 8 == 0;
+  const bool aligned = aligned_rows(x, ldx, w, ldw);
   const auto go = [&](auto kernel) { launch_pdl(kernel, grid, dim3(kRowsThreads), 0, st, p); };
   if (aligned) bf16 ? go(&f16_rows_gemm_kernel<EPI, true, true>) : go(&f16_rows_gemm_kernel<EPI, false, true>);
   else bf16 ? go(&f16_rows_gemm_kernel<EPI, true, false>) : go(&f16_rows_gemm_kernel<EPI, false, false>);
@@ -446,7 +455,7 @@ int dsv4_b200_dense_gemm(const void* a, int64_t lda, int a_mn, const void* b, in
   p.residual = mat16(residual, ldr);
   p.out = mat16(out, ldo);
   p.zq = z_codes, p.zbits = z_bits, p.zs = z_scales, p.n32 = round_up(n, kGroup);
-  if (takes_rows(p, a_mn, b_mn))
+  if (takes_rows(p, false, a_mn, b_mn, aligned_rows(a, lda, b, ldb)))
     return launch_rows_gemm<kEpiLinear>(p, a, lda, b, ldb, dtype == DSV4_BF16, as_stream(stream));
   F16StreamParams few = {};
   bool two = false;
@@ -478,7 +487,7 @@ int dsv4_b200_gated_gemm(const void* x, int64_t ldx, int x_mn, const void* w13, 
   p.up_row = p.n;
   p.out = mat16(h, ldh);
   p.zq = z_codes, p.zbits = z_bits, p.zs = z_scales, p.n32 = round_up(intermediate, kGroup);
-  if (takes_rows(p, x_mn, w_mn))
+  if (takes_rows(p, true, x_mn, w_mn, aligned_rows(x, ldx, w13, ldw)))
     return launch_rows_gemm<kEpiGated>(p, x, ldx, w13, ldw, dtype == DSV4_BF16, as_stream(stream));
   F16StreamParams few = {};
   bool two = false;
@@ -635,7 +644,8 @@ int dsv4_b200_act_backward(const void* dy, int64_t lddy, const void* z_codes, in
   return DSV4_OK;
 }
 
-// dW = d^T x, with x as it is or restored from its 8-bit codes first.
+// dW = d^T x, with x as it is or restored from its 8-bit codes first: rounded to
+// 16 bits, 2^-9 (fp16 2^-12) of a value that the codes hold to amax / 254.
 static int weight_gradient(const void* d, int64_t ldd, int d_mn, const void* x, int64_t ldx, int x_mn,
                            const int8_t* x_codes, const float* x_scales, void* x_restored,
                            int64_t ldxr, int64_t rows, int64_t cols, int64_t m, int dtype, void* dw,
