@@ -50,6 +50,14 @@ __device__ __forceinline__ void tmem_ld_f32x32(uint32_t taddr, float (&f)[32]) {
   for (int j = 0; j < 32; ++j) f[j] = __int_as_float(v[j]);
 }
 
+__device__ __forceinline__ void tmem_ld_f32x16(uint32_t taddr, float (&f)[16]) {
+  int32_t v[16];
+  tmem_ld_x16(taddr, v);
+  tmem_ld_wait_regs(v);
+#pragma unroll
+  for (int j = 0; j < 16; ++j) f[j] = __int_as_float(v[j]);
+}
+
 // ---- 16-bit values ----
 template <bool BF16>
 __device__ __forceinline__ uint32_t pack_16(float lo, float hi) {
@@ -205,15 +213,16 @@ __device__ __forceinline__ void gated_backward(float limit, float dh, float g, f
   h = a * uc;
 }
 
+// 16 columns of a row
 template <bool BF16>
-__device__ __forceinline__ void gated_backward_row(int act, float limit, const float (&dh)[32],
-                                                   const float (&g)[32], const float (&u)[32],
-                                                   uint32_t (&wg)[16], uint32_t (&wu)[16],
-                                                   uint32_t (&wh)[16]) {
+__device__ __forceinline__ void gated_backward_row(int act, float limit, const float (&dh)[16],
+                                                   const float (&g)[16], const float (&u)[16],
+                                                   uint32_t (&wg)[8], uint32_t (&wu)[8],
+                                                   uint32_t (&wh)[8]) {
   act_dispatch(act, [&](auto kind) {
     constexpr int K = decltype(kind)::value;
 #pragma unroll
-    for (int j = 0; j < 16; ++j) {
+    for (int j = 0; j < 8; ++j) {
       float dg[2], du[2], h[2];
 #pragma unroll
       for (int i = 0; i < 2; ++i)
@@ -427,7 +436,14 @@ __device__ __forceinline__ float keep_group16(const float (&v)[32], float limit,
     for (int j = 0; j < 16; ++j) codes[j] = 0;
     return step;
   }
-  const bool limited = limit < CUDART_INF_F || keep_sign;
+  // (a kept value is at most `most`: below the limit there is no side to keep)
+  if (!(most > limit) && !keep_sign) {
+#pragma unroll
+    for (int j = 0; j < 16; ++j)
+      codes[j] = prmt(__float_as_uint(__fmaf_rn(v[2 * j], inv, kWhole)),
+                      __float_as_uint(__fmaf_rn(v[2 * j + 1], inv, kWhole)), 0x5410u);
+    return step;
+  }
 #pragma unroll
   for (int j = 0; j < 16; ++j) {
     float q[2];
@@ -435,13 +451,11 @@ __device__ __forceinline__ float keep_group16(const float (&v)[32], float limit,
     for (int i = 0; i < 2; ++i) {
       const float x = v[2 * j + i];
       q[i] = __fmaf_rn(x, inv, kWhole);
-      if (limited) {
-        const float n = q[i] - kWhole, toward = x < 0.f ? 1.f : -1.f;  // toward zero
-        const bool over = fabsf(x) > limit, kept = fabsf(n * step) > limit;
-        if (over && !kept) q[i] -= toward;
-        if (!over && kept) q[i] += toward;
-        if (keep_sign && n == 0.f && x != 0.f) q[i] -= toward;
-      }
+      const float n = q[i] - kWhole, toward = x < 0.f ? 1.f : -1.f;  // toward zero
+      const bool over = fabsf(x) > limit, kept = fabsf(n * step) > limit;
+      if (over && !kept) q[i] -= toward;
+      if (!over && kept) q[i] += toward;
+      if (keep_sign && n == 0.f && x != 0.f) q[i] -= toward;
     }
     codes[j] = prmt(__float_as_uint(q[0]), __float_as_uint(q[1]), 0x5410u);
   }

@@ -41,14 +41,16 @@ enum F16DeviceErr : int {
 
 enum F16Epi : int { kEpiLinear = 0, kEpiGated = 1, kEpiGatedBwd = 2 };
 
-// Epilogue warps and their 2-KB shared slices.  The linear epilogue fits 96
+// Epilogue warps and their 2-KB shared slices.  The forward epilogues fit 96
 // registers and one slice: 16 warps (2048 x 2048 -> 7168 with bias, gelu,
-// residual and z kept: 61 us, 65 with 12, 71 with 8).  The gated ones hold two
-// factors.
+// residual and z kept: 61 us, 65 with 12, 71 with 8; gated 4096 x 1024 -> 2 x
+// 2048 kept: 33, 38 with 8).  The gate's backward pass turns two matrices over
+// in place and is best with few warps and all of their registers (4096 x 1024
+// -> 2048: 40 us, 46 with 12).
 template <int EPI>
 struct F16Roles {
-  static constexpr int kEpiWarps = EPI == kEpiLinear ? 16 : 8;
-  static constexpr int kSlices = EPI == kEpiLinear ? 1 : 2;
+  static constexpr int kEpiWarps = EPI == kEpiGatedBwd ? 8 : 16;
+  static constexpr int kSlices = EPI == kEpiGatedBwd ? 2 : 1;
   static constexpr int kThreads = 128 + 32 * kEpiWarps;
   static constexpr int kEpiBytes = kEpiWarps * kSlices * 2048;
 };
@@ -209,17 +211,22 @@ __device__ __forceinline__ bool chunk_whole(const F16Mat& mat, int col0, int col
   return mat.vec && col0 + 32 <= cols;
 }
 
+__device__ __forceinline__ void whole_chunk_fetch(uint4 (&r)[4], const uint16_t* base, int64_t ld,
+                                                  int lane, int row0, int rows) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int row = 8 * i + (lane >> 2);
+    r[i] = make_uint4(0, 0, 0, 0);
+    if (row0 + row < rows) r[i] = *reinterpret_cast<const uint4*>(base + row * ld + 8 * (lane & 3));
+  }
+}
+
 // In the second form register word i holds rows 2i and 2i + 1 of the column.
 __device__ __forceinline__ void chunk_fetch(uint4 (&r)[4], const F16Mat& mat, int lane, int row0,
                                             int rows, int col0, int cols) {
   const uint16_t* base = static_cast<const uint16_t*>(mat.p) + row0 * mat.ld + col0;
   if (chunk_whole(mat, col0, cols)) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int row = 8 * i + (lane >> 2);
-      r[i] = make_uint4(0, 0, 0, 0);
-      if (row0 + row < rows) r[i] = *reinterpret_cast<const uint4*>(base + row * mat.ld + 8 * (lane & 3));
-    }
+    whole_chunk_fetch(r, base, mat.ld, lane, row0, rows);
   } else {
     uint32_t w[16];
 #pragma unroll
@@ -235,12 +242,16 @@ __device__ __forceinline__ void chunk_fetch(uint4 (&r)[4], const F16Mat& mat, in
   }
 }
 
+__device__ __forceinline__ void whole_chunk_to_slice(uint32_t slice, int lane, const uint4 (&r)[4]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    st_shared_v4(slice + slice_off(8 * i + (lane >> 2), lane & 3), r[i]);
+}
+
 __device__ __forceinline__ void chunk_to_rows(uint32_t slice, int lane, const uint4 (&r)[4],
                                               bool whole, uint32_t (&w)[16]) {
   if (whole) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      st_shared_v4(slice + slice_off(8 * i + (lane >> 2), lane & 3), r[i]);
+    whole_chunk_to_slice(slice, lane, r);
   } else {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -261,13 +272,17 @@ __device__ __forceinline__ void chunk_to_rows(uint32_t slice, int lane, const ui
   __syncwarp();
 }
 
-__device__ __forceinline__ void chunk_store(uint32_t slice, int lane, const uint32_t (&w)[16],
-                                            const F16Mat& mat, int row0, int rows, int col0,
-                                            int cols) {
+// A lane's row in the slice, from piece `c` on.
+template <int N>
+__device__ __forceinline__ void row_to_slice(uint32_t slice, int lane, int c, const uint32_t (&w)[N]) {
 #pragma unroll
-  for (int c = 0; c < 4; ++c)
-    st_shared_v4(slice + slice_off(lane, c),
-                 make_uint4(w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]));
+  for (int i = 0; i < N / 4; ++i)
+    st_shared_v4(slice + slice_off(lane, c + i),
+                 make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]));
+}
+
+__device__ __forceinline__ void slice_store(uint32_t slice, int lane, const F16Mat& mat, int row0,
+                                            int rows, int col0, int cols) {
   __syncwarp();
   uint16_t* base = static_cast<uint16_t*>(mat.p) + row0 * mat.ld + col0;
   if (chunk_whole(mat, col0, cols)) {
@@ -284,6 +299,13 @@ __device__ __forceinline__ void chunk_store(uint32_t slice, int lane, const uint
         base[row * mat.ld + lane] = static_cast<uint16_t>(ld_shared_u16(slice + slice_elem(row, lane)));
   }
   __syncwarp();
+}
+
+__device__ __forceinline__ void chunk_store(uint32_t slice, int lane, const uint32_t (&w)[16],
+                                            const F16Mat& mat, int row0, int rows, int col0,
+                                            int cols) {
+  row_to_slice(slice, lane, 0, w);
+  slice_store(slice, lane, mat, row0, rows, col0, cols);
 }
 
 // 8-bit codes of a 32 x 32 chunk (rows of 32 bytes, always whole: the code
@@ -305,7 +327,7 @@ __device__ __forceinline__ void codes_store(uint32_t slice, int lane, const uint
   __syncwarp();
 }
 
-__device__ __forceinline__ void codes_fetch(uint4 (&v)[2], const int8_t* base, int64_t ld,
+__device__ __forceinline__ void codes_fetch(uint4 (&v)[4], const int8_t* base, int64_t ld,
                                             int lane, int row0, int rows, int64_t col0) {
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
@@ -316,22 +338,18 @@ __device__ __forceinline__ void codes_fetch(uint4 (&v)[2], const int8_t* base, i
   }
 }
 
-__device__ __forceinline__ void codes_to_rows(uint32_t slice, int lane, const uint4 (&v)[2],
-                                              float scale, float (&x)[32]) {
+__device__ __forceinline__ void codes_to_rows(uint32_t slice, int lane, const uint4& v0, const uint4& v1,
+                                              uint32_t (&q)[8]) {
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     const int r = 16 * i + (lane >> 1);
-    st_shared_v4(slice + r * 32 + (((lane & 1) ^ ((r >> 2) & 1)) << 4), v[i]);
+    st_shared_v4(slice + r * 32 + (((lane & 1) ^ ((r >> 2) & 1)) << 4), i ? v1 : v0);
   }
   __syncwarp();
 #pragma unroll
   for (int half = 0; half < 2; ++half) {
     const uint4 c = ld_shared_v4(slice + lane * 32 + ((half ^ ((lane >> 2) & 1)) << 4));
-    const uint32_t w[4] = {c.x, c.y, c.z, c.w};
-#pragma unroll
-    for (int j = 0; j < 16; ++j)
-      x[16 * half + j] =
-          scale * code8_value(w[j >> 2], j & 3);
+    q[4 * half] = c.x, q[4 * half + 1] = c.y, q[4 * half + 2] = c.z, q[4 * half + 3] = c.w;
   }
   __syncwarp();
 }
@@ -353,20 +371,29 @@ __device__ __forceinline__ void keep_rows(const F16GemmParams& p, uint32_t slice
   if (row0 + lane < p.m) p.zs[static_cast<int64_t>(at >> 5) * p.m + row0 + lane] = s;
 }
 
-__device__ __forceinline__ void kept_rows(const F16GemmParams& p, uint32_t slice, int lane,
-                                          float (&v)[32], int64_t ld, int row0, int at) {
-  float s = 0.f;
-  if (row0 + lane < p.m) s = p.zs[static_cast<int64_t>(at >> 5) * p.m + row0 + lane];
+// The way back: a warp's 32 rows of a kept group as they lie in memory, and
+// each row's scale.
+__device__ __forceinline__ float kept_fetch(const F16GemmParams& p, uint4 (&r)[4], int lane, int64_t ld,
+                                            int row0, int at) {
   if (p.zbits == 8) {
-    uint4 c[2];
-    codes_fetch(c, static_cast<const int8_t*>(p.zq), ld, lane, row0, p.m, at);
-    codes_to_rows(slice, lane, c, s, v);
+    codes_fetch(r, static_cast<const int8_t*>(p.zq), ld, lane, row0, p.m, at);
   } else {
-    uint4 r[4];
-    uint32_t w[16];
-    chunk_fetch(r, F16Mat{p.zq, ld, 1}, lane, row0, p.m, at, static_cast<int>(ld));
-    chunk_to_rows(slice, lane, r, true, w);
-    kept16_values<32>(w, s, v);
+    whole_chunk_fetch(r, static_cast<const uint16_t*>(p.zq) + row0 * ld + at, ld, lane, row0, p.m);
+  }
+  return row0 + lane < p.m ? p.zs[static_cast<int64_t>(at >> 5) * p.m + row0 + lane] : 0.f;
+}
+
+// 16 values of a lane's row: codes in the slice (16 bits) or in its registers.
+__device__ __forceinline__ void kept_half(const F16GemmParams& p, uint32_t slice, int lane, int half,
+                                          const uint32_t (&q)[8], float scale, float (&v)[16]) {
+  if (p.zbits == 8) {
+#pragma unroll
+    for (int j = 0; j < 16; ++j) v[j] = scale * code8_value(q[4 * half + (j >> 2)], j & 3);
+  } else {
+    const uint4 a = ld_shared_v4(slice + slice_off(lane, 2 * half));
+    const uint4 b = ld_shared_v4(slice + slice_off(lane, 2 * half + 1));
+    const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+    kept16_values<16>(w, scale, v);
   }
 }
 
@@ -518,11 +545,19 @@ __global__ void __launch_bounds__(F16Roles<EPI>::kThreads, 1)
       tile_at(t, tm, tc);
       const uint32_t buf = nt & 1, use = nt >> 1;
       const int row0 = tm * 256 + static_cast<int>(rank) * 128 + quarter * 32;
+      const int width = EPI == kEpiGated ? half_n : p.tn;
+      const int cbase = tc * width;
+      // kEpiGatedBwd: the kept groups of the next chunk, on their way
+      uint4 rg[4], ru[4];
+      float next_sg = 0.f, next_su = 0.f;
+      const auto fetch = [&](int col) {
+        next_sg = kept_fetch(p, rg, lane, 2 * p.n32, row0, col);
+        next_su = kept_fetch(p, ru, lane, 2 * p.n32, row0, static_cast<int>(p.n32) + col);
+      };
+      if (EPI == kEpiGatedBwd && cbase + side * 32 < p.n) fetch(cbase + side * 32);
       if (!mbar_wait_cl(acc_full(buf), use & 1, kErrF16WaitAccFull)) break;
       tc_fence_after();
       const uint32_t acc = tmem + buf * 256 + lanes;
-      const int width = EPI == kEpiGated ? half_n : p.tn;
-      const int cbase = tc * width;
       for (int c0 = side * 32; c0 < width; c0 += 8 * kEpiWarps) {
         const int col = cbase + c0;
         if (col >= p.n) break;
@@ -578,15 +613,33 @@ __global__ void __launch_bounds__(F16Roles<EPI>::kThreads, 1)
           pack_row<BF16>(g, w);
           chunk_store(slice0, lane, w, p.out, row0, p.m, col, p.n);
         } else {
-          float g[32], u[32];
-          kept_rows(p, slice0, lane, g, 2 * p.n32, row0, col);
-          kept_rows(p, slice1, lane, u, 2 * p.n32, row0, static_cast<int>(p.n32) + col);
-          float v[32];
-          tmem_ld_f32x32(acc + c0, v);
-          uint32_t w[16], wu[16], wh[16];
-          gated_backward_row<BF16>(p.act, p.limit, v, g, u, w, wu, wh);
-          chunk_store(slice0, lane, w, p.d0, row0, p.m, col, p.n);
-          chunk_store(slice1, lane, wu, p.d1, row0, p.m, col, p.n);
+          const float sg = next_sg, su = next_su;
+          uint32_t qg[8] = {}, qu[8] = {}, wh[16];
+          if (p.zbits == 8) {
+            codes_to_rows(slice0, lane, rg[0], rg[1], qg);
+            codes_to_rows(slice1, lane, ru[0], ru[1], qu);
+          } else {
+            whole_chunk_to_slice(slice0, lane, rg);
+            whole_chunk_to_slice(slice1, lane, ru);
+            __syncwarp();
+          }
+          if (c0 + 8 * kEpiWarps < width && col + 8 * kEpiWarps < p.n) fetch(col + 8 * kEpiWarps);
+          // half a group at a time: its results take its codes' place in the slices
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            float v[16], g[16], u[16];
+            tmem_ld_f32x16(acc + c0 + 16 * half, v);
+            kept_half(p, slice0, lane, half, qg, sg, g);
+            kept_half(p, slice1, lane, half, qu, su, u);
+            uint32_t wg[8], wu[8], w[8];
+            gated_backward_row<BF16>(p.act, p.limit, v, g, u, wg, wu, w);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) wh[8 * half + j] = w[j];
+            row_to_slice(slice0, lane, 2 * half, wg);
+            row_to_slice(slice1, lane, 2 * half, wu);
+          }
+          slice_store(slice0, lane, p.d0, row0, p.m, col, p.n);
+          slice_store(slice1, lane, p.d1, row0, p.m, col, p.n);
           if (p.out.p) chunk_store(slice0, lane, wh, p.out, row0, p.m, col, p.n);
         }
       }
