@@ -410,9 +410,12 @@ int feed_forward_init() {
   if (e == cudaSuccess) e = rows_attrs<kEpiLinear>();
   if (e == cudaSuccess) e = rows_attrs<kEpiGated>();
   if (e == cudaSuccess)
-    e = load_kernels(&checkpoint_kernel<DSV4_F32>, &checkpoint_kernel<DSV4_F16>,
-                     &checkpoint_kernel<DSV4_BF16>, &restore_kernel<DSV4_F32>,
-                     &restore_kernel<DSV4_F16>, &restore_kernel<DSV4_BF16>,
+    e = load_kernels(&checkpoint_kernel<DSV4_F32, true>, &checkpoint_kernel<DSV4_F32, false>,
+                     &checkpoint_kernel<DSV4_F16, true>, &checkpoint_kernel<DSV4_F16, false>,
+                     &checkpoint_kernel<DSV4_BF16, true>, &checkpoint_kernel<DSV4_BF16, false>,
+                     &restore_kernel<DSV4_F32, true>, &restore_kernel<DSV4_F32, false>,
+                     &restore_kernel<DSV4_F16, true>, &restore_kernel<DSV4_F16, false>,
+                     &restore_kernel<DSV4_BF16, true>, &restore_kernel<DSV4_BF16, false>,
                      &act_backward_kernel<true>, &act_backward_kernel<false>,
                      &column_sum_kernel<true>, &column_sum_kernel<false>, &pack_rows_kernel);
   if (e != cudaSuccess)
@@ -553,16 +556,16 @@ int dsv4_b200_checkpoint_int8(const void* x, int dtype, int64_t m, int64_t k, in
   const int64_t k32 = round_up(k, kGroup), cb = (k32 + 255) / 256, blocks = (m + 31) / 32 * cb;
   DSV4_REQUIRE(blocks < (1ll << 31), "checkpoint too large");
   const int per = dtype == DSV4_F32 ? 4 : 8;
-  const int vec = aligned16(x) && ldx % per == 0;
+  const bool vec = aligned16(x) && ldx % per == 0;
   const dim3 grid(static_cast<unsigned>(blocks));
   cudaStream_t st = as_stream(stream);
   const auto go = [&](auto kernel) {
-    launch_pdl(kernel, grid, dim3(256), 0, st, x, ldx, vec, m, k, k32, static_cast<uint32_t>(cb), codes,
+    launch_pdl(kernel, grid, dim3(256), 0, st, x, ldx, m, k, k32, static_cast<uint32_t>(cb), codes,
                scales);
   };
-  if (dtype == DSV4_F32) go(&checkpoint_kernel<DSV4_F32>);
-  else if (dtype == DSV4_F16) go(&checkpoint_kernel<DSV4_F16>);
-  else go(&checkpoint_kernel<DSV4_BF16>);
+  if (dtype == DSV4_F32) vec ? go(&checkpoint_kernel<DSV4_F32, true>) : go(&checkpoint_kernel<DSV4_F32, false>);
+  else if (dtype == DSV4_F16) vec ? go(&checkpoint_kernel<DSV4_F16, true>) : go(&checkpoint_kernel<DSV4_F16, false>);
+  else vec ? go(&checkpoint_kernel<DSV4_BF16, true>) : go(&checkpoint_kernel<DSV4_BF16, false>);
   return check_launch("checkpoint_kernel");
 }
 
@@ -578,16 +581,15 @@ int dsv4_b200_restore_int8(const int8_t* codes, const float* scales, int64_t m, 
   const int64_t k32 = round_up(k, kGroup), cb = (k32 + 255) / 256, blocks = (m + 31) / 32 * cb;
   DSV4_REQUIRE(blocks < (1ll << 31), "checkpoint too large");
   const int per = dtype == DSV4_F32 ? 4 : 8;
-  const int vec = aligned16(out) && ldo % per == 0;
+  const bool vec = aligned16(out) && ldo % per == 0;
   const dim3 grid(static_cast<unsigned>(blocks));
   cudaStream_t st = as_stream(stream);
   const auto go = [&](auto kernel) {
-    launch_pdl(kernel, grid, dim3(256), 0, st, codes, scales, m, k, k32, static_cast<uint32_t>(cb), out, ldo,
-               vec);
+    launch_pdl(kernel, grid, dim3(256), 0, st, codes, scales, m, k, k32, static_cast<uint32_t>(cb), out, ldo);
   };
-  if (dtype == DSV4_F32) go(&restore_kernel<DSV4_F32>);
-  else if (dtype == DSV4_F16) go(&restore_kernel<DSV4_F16>);
-  else go(&restore_kernel<DSV4_BF16>);
+  if (dtype == DSV4_F32) vec ? go(&restore_kernel<DSV4_F32, true>) : go(&restore_kernel<DSV4_F32, false>);
+  else if (dtype == DSV4_F16) vec ? go(&restore_kernel<DSV4_F16, true>) : go(&restore_kernel<DSV4_F16, false>);
+  else vec ? go(&restore_kernel<DSV4_BF16, true>) : go(&restore_kernel<DSV4_BF16, false>);
   return check_launch("restore_kernel");
 }
 

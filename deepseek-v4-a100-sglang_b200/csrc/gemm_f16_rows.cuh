@@ -69,54 +69,6 @@ __device__ __forceinline__ uint4 load_k8(const uint16_t* p, int left) {
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// A matrix's first byte and the one behind its last.
-struct Extent {
-  uint64_t lo, hi;
-};
-
-__device__ __forceinline__ Extent extent_of(const uint16_t* p, int64_t rows, int64_t ld, int k) {
-  const uint64_t lo = reinterpret_cast<uint64_t>(p);
-  return {lo, lo + 2 * static_cast<uint64_t>((rows - 1) * ld + k)};
-}
-
-// The same from any even address.
-struct Window {
-  uint4 a, b;
-};
-
-__device__ __forceinline__ Window load_window(const uint16_t* p, int left, const Extent& e) {
-  const uint64_t at = reinterpret_cast<uint64_t>(p) & ~15ull;
-  Window w;
-  if (left >= 8 && at >= e.lo && at + 32 <= e.hi) {
-    w.a = *reinterpret_cast<const uint4*>(at);
-    w.b = *reinterpret_cast<const uint4*>(at + 16);
-  } else {  // at the matrix's ends: the 8 values themselves, put where the shift finds them
-    uint32_t v[8] = {};
-    const int off = static_cast<int>(reinterpret_cast<uint64_t>(p) & 15) >> 1;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const int j = i - off;
-      if (j >= 0 && j < 8 && j < left) v[i >> 1] |= static_cast<uint32_t>(p[j]) << (16 * (i & 1));
-    }
-    w.a = make_uint4(v[0], v[1], v[2], v[3]);
-    w.b = make_uint4(v[4], v[5], v[6], v[7]);
-  }
-  return w;
-}
-
-// 16 bytes of the window from byte `off` (even, below 16)
-__device__ __forceinline__ uint4 shift_window(const Window& w, int off) {
-  const uint32_t v[8] = {w.a.x, w.a.y, w.a.z, w.a.w, w.b.x, w.b.y, w.b.z, w.b.w};
-  uint32_t t[6], u[5];
-#pragma unroll
-  for (int i = 0; i < 6; ++i) t[i] = off & 8 ? v[i + 2] : v[i];
-#pragma unroll
-  for (int i = 0; i < 5; ++i) u[i] = off & 4 ? t[i + 1] : t[i];
-  const int bits = off & 2 ? 16 : 0;
-  return make_uint4(__funnelshift_r(u[0], u[1], bits), __funnelshift_r(u[1], u[2], bits),
-                    __funnelshift_r(u[2], u[3], bits), __funnelshift_r(u[3], u[4], bits));
-}
-
 template <int EPI, bool BF16, bool ALIGNED>
 __global__ void __launch_bounds__(kRowsThreads, ALIGNED ? 2 : 1)
     f16_rows_gemm_kernel(const F16RowsParams p) {

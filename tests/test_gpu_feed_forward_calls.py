@@ -147,6 +147,34 @@ def test_results_stay_inside_their_rows(m):
     assert (big[m:] == 7).all() and (big[:, n:] == 7).all()
 
 
+@pytest.mark.parametrize("dtype", [BF16, F16, torch.float32])
+def test_checkpoints_at_any_alignment(dtype):
+    """Rows that begin at every element of 16 bytes, inside a buffer: the codes
+    and values of aligned rows, and nothing beside them read or written."""
+    import dsv4_b200 as D
+    from dsv4_b200 import _native as N
+    st = torch.cuda.current_stream().cuda_stream
+    dt = {BF16: N.DTYPE_BF16, F16: N.DTYPE_F16, torch.float32: N.DTYPE_F32}[dtype]
+    m = 37
+    for k in (1, 5, 7, 8, 9, 31, 250, 255, 256, 257, 263, 264, 520, 1001):
+        x = rand(m, k, dtype=dtype, seed=k)
+        want = D.checkpoint_int8(x)
+        back = D.restore_int8(want)
+        for lead in range(8):
+            ld = k + (lead + k) % 3
+            buf = torch.full((lead + m * ld + 9,), math.nan, dtype=dtype, device="cuda")
+            view = buf[lead:lead + m * ld].view(m, ld)[:, :k]
+            view.copy_(x)
+            got = D.checkpoint_int8(view)
+            assert torch.equal(got.codes, want.codes) and torch.equal(got.scales, want.scales), (k, lead)
+            buf.fill_(7)
+            N.call("dsv4_b200_restore_int8", got.codes.data_ptr(), got.scales.data_ptr(), m, k, view.data_ptr(), dt,
+                   ld, st)
+            assert torch.equal(view, back), (k, lead)
+            view.fill_(7)
+            assert (buf == 7).all(), (k, lead)
+
+
 # ---- values ----
 
 @pytest.mark.parametrize("m", [4, 300])
