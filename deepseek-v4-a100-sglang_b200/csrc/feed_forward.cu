@@ -26,6 +26,9 @@ cudaError_t pair_attrs() {
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
+// To whole elements, as every pointer to them has to be.
+bool aligned_to(const void* p, int bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
+
 F16Mat mat16(const void* p, int64_t ld) {
   return {const_cast<void*>(p), ld, aligned16(p) && ld % 8 == 0};
 }
@@ -342,8 +345,7 @@ bool takes_rows(const F16GemmParams& q, bool gated, int x_mn, int w_mn, bool ali
 template <int EPI>
 int launch_rows_gemm(const F16GemmParams& q, const void* x, int64_t ldx, const void* w, int64_t ldw,
                      bool bf16, cudaStream_t st) {
-  DSV4_REQUIRE((reinterpret_cast<uintptr_t>(x) & 1) == 0 && (reinterpret_cast<uintptr_t>(w) & 1) == 0,
-               "a and b must be aligned to their elements");
+  DSV4_REQUIRE(aligned_to(x, 2) && aligned_to(w, 2), "a and b must be aligned to their elements");
   DSV4_REQUIRE(ldx >= q.k && ldw >= q.k, "row stride below k (%lld and %lld, k %d)",
                (long long)ldx, (long long)ldw, q.k);
   F16RowsParams p = {static_cast<const uint16_t*>(x), static_cast<const uint16_t*>(w), ldx, ldw, q.m, q.n,
@@ -417,7 +419,8 @@ int feed_forward_init() {
                      &restore_kernel<DSV4_F16, true>, &restore_kernel<DSV4_F16, false>,
                      &restore_kernel<DSV4_BF16, true>, &restore_kernel<DSV4_BF16, false>,
                      &act_backward_kernel<true>, &act_backward_kernel<false>,
-                     &column_sum_kernel<true>, &column_sum_kernel<false>, &pack_rows_kernel);
+                     &column_sum_kernel<true>, &column_sum_kernel<false>, &pack_rows_kernel,
+                     &pack_windows_kernel);
   if (e != cudaSuccess)
     return fail(DSV4_ERR_CUDA, "feed-forward kernels: %s", cudaGetErrorString(e));
   return DSV4_OK;
@@ -449,6 +452,8 @@ int dsv4_b200_dense_gemm(const void* a, int64_t lda, int a_mn, const void* b, in
   if (int r = check_kept(z_codes, z_bits, z_scales)) return r;
   if (m == 0) return DSV4_OK;
   DSV4_REQUIRE(a && b && out, "null pointer argument");
+  DSV4_REQUIRE(aligned_to(bias, 2) && aligned_to(residual, 2) && aligned_to(out, 2) && aligned_to(z_scales, 4),
+               "bias, residual, out and z_scales must be aligned to their elements");
   DSV4_REQUIRE(ldo >= n && (!residual || ldr >= n || ldr == 0), "row stride below n");
   F16GemmParams p = {};
   p.m = static_cast<int>(m), p.n = static_cast<int>(n), p.k = static_cast<int>(k);
@@ -480,6 +485,7 @@ int dsv4_b200_gated_gemm(const void* x, int64_t ldx, int x_mn, const void* w13, 
   if (int r = check_limit(has_clamp, clamp_limit, &p.limit)) return r;
   if (m == 0) return DSV4_OK;
   DSV4_REQUIRE(x && w13 && h, "null pointer argument");
+  DSV4_REQUIRE(aligned_to(h, 2) && aligned_to(z_scales, 4), "h and z_scales must be aligned to their elements");
   DSV4_REQUIRE(ldh >= intermediate, "row stride below the row");
   // a TMA box starts at a multiple of 16 bytes
   DSV4_REQUIRE(!w_mn || intermediate % 8 == 0,
@@ -532,6 +538,8 @@ int dsv4_b200_gated_backward_gemm(const void* dy, int64_t lddy, int dy_mn, const
   if (int r = check_limit(has_clamp, clamp_limit, &p.limit)) return r;
   if (m == 0) return DSV4_OK;
   DSV4_REQUIRE(dy && w2 && dz, "null pointer argument");
+  DSV4_REQUIRE(aligned_to(dz, 2) && aligned_to(h, 2) && aligned_to(z_scales, 4),
+               "dz, h and z_scales must be aligned to their elements");
   DSV4_REQUIRE(z_bits != 0, "the kept g and u are needed");
   DSV4_REQUIRE(lddz >= 2 * intermediate && (!h || ldh >= intermediate), "row stride below the row");
   p.m = static_cast<int>(m), p.n = static_cast<int>(intermediate), p.k = static_cast<int>(k);
@@ -553,6 +561,8 @@ int dsv4_b200_checkpoint_int8(const void* x, int dtype, int64_t m, int64_t k, in
   if (m == 0) return DSV4_OK;
   DSV4_REQUIRE(x && codes && scales, "null pointer argument");
   DSV4_REQUIRE(aligned16(codes), "codes must be 16-byte aligned");
+  DSV4_REQUIRE(aligned_to(x, dtype == DSV4_F32 ? 4 : 2) && aligned_to(scales, 4),
+               "x and scales must be aligned to their elements");
   const int64_t k32 = round_up(k, kGroup), cb = (k32 + 255) / 256, blocks = (m + 31) / 32 * cb;
   DSV4_REQUIRE(blocks < (1ll << 31), "checkpoint too large");
   const int per = dtype == DSV4_F32 ? 4 : 8;
@@ -578,6 +588,8 @@ int dsv4_b200_restore_int8(const int8_t* codes, const float* scales, int64_t m, 
   if (m == 0) return DSV4_OK;
   DSV4_REQUIRE(out && codes && scales, "null pointer argument");
   DSV4_REQUIRE(aligned16(codes), "codes must be 16-byte aligned");
+  DSV4_REQUIRE(aligned_to(out, dtype == DSV4_F32 ? 4 : 2) && aligned_to(scales, 4),
+               "out and scales must be aligned to their elements");
   const int64_t k32 = round_up(k, kGroup), cb = (k32 + 255) / 256, blocks = (m + 31) / 32 * cb;
   DSV4_REQUIRE(blocks < (1ll << 31), "checkpoint too large");
   const int per = dtype == DSV4_F32 ? 4 : 8;
@@ -621,6 +633,8 @@ int dsv4_b200_act_backward(const void* dy, int64_t lddy, const void* z_codes, in
                    (dz && lddz >= n && z_bits != 0), "an activation needs dz and the kept z");
   DSV4_REQUIRE(m == 0 || (dy && (lddy >= n || m == 1)), "bad dy");
   DSV4_REQUIRE(need < 65536, "too many rows");
+  DSV4_REQUIRE(aligned_to(dy, 2) && aligned_to(dz, 2) && aligned_to(dbias, 2) && aligned_to(z_scales, 4) &&
+                   aligned_to(partial, 4), "pointers must be aligned to their elements");
   cudaStream_t st = as_stream(stream);
   ActBackward p = {};
   p.dy = dy, p.lddy = lddy, p.vec_dy = mat16(dy, lddy).vec;
@@ -727,8 +741,16 @@ int dsv4_b200_pack_rows(const void* in, int64_t row_stride, int64_t col_stride, 
                    col_stride >= 0 && ldo >= cols, "bad shape");
   if (rows == 0 || cols == 0) return DSV4_OK;
   DSV4_REQUIRE(in && out, "null pointer argument");
-  const int64_t cb = (cols + 31) / 32, blocks = (rows + 31) / 32 * cb;
+  DSV4_REQUIRE(aligned_to(in, 2) && aligned_to(out, 2), "in and out must be aligned to their elements");
+  const bool windows = col_stride == 1 && (row_stride >= cols || rows == 1) && aligned16(out) && ldo % 8 == 0;
+  const int64_t width = windows ? 256 : 32, cb = (cols + width - 1) / width, blocks = (rows + 31) / 32 * cb;
   DSV4_REQUIRE(blocks < (1ll << 31), "matrix too large");
+  if (windows) {
+    launch_pdl(&pack_windows_kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, as_stream(stream),
+               static_cast<const uint16_t*>(in), row_stride, rows, cols, static_cast<uint32_t>(cb),
+               static_cast<uint16_t*>(out), ldo);
+    return check_launch("pack_windows_kernel");
+  }
   launch_pdl(&pack_rows_kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, as_stream(stream),
              static_cast<const uint16_t*>(in), row_stride, col_stride, rows, cols,
              static_cast<uint32_t>(cb),

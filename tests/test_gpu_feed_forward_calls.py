@@ -632,6 +632,32 @@ def test_c_refusals():
     N.check_device_status()
 
 
+def test_c_refuses_addresses_between_elements():
+    from dsv4_b200 import _native as N
+    x, w, _, _ = dense_case(16, 64, 32, BF16, False, False)
+    st = torch.cuda.current_stream().cuda_stream
+    p, q = x.data_ptr(), w.data_ptr()
+    out, codes = torch.zeros(16, 64, device="cuda", dtype=BF16), torch.zeros(16, 64, device="cuda", dtype=torch.int8)
+    scales = torch.zeros(64, device="cuda")
+    o, c, s = out.data_ptr(), codes.data_ptr(), scales.data_ptr()
+    for name, *args in (
+            ("dense_gemm", p, 64, 0, q, 64, 0, 16, 32, 64, 2, o + 1, 0, None, 0, o, 32, None, 0, None),
+            ("dense_gemm", p, 64, 0, q, 64, 0, 16, 32, 64, 2, None, 0, o + 1, 32, o, 32, None, 0, None),
+            ("dense_gemm", p, 64, 0, q, 64, 0, 16, 32, 64, 2, None, 0, None, 0, o + 1, 32, None, 0, None),
+            ("dense_gemm", p + 1, 64, 0, q, 64, 0, 1, 32, 64, 2, None, 0, None, 0, o, 32, None, 0, None),
+            ("dense_gemm", p, 64, 0, q, 64, 0, 16, 32, 64, 2, None, 2, None, 0, o, 32, c, 8, s + 2),
+            ("gated_gemm", p, 64, 0, q, 64, 0, 16, 16, 64, 2, 2, 0, 0.0, o + 1, 16, None, 0, None),
+            ("gated_backward_gemm", p, 64, 0, q, 64, 0, 16, 16, 64, 2, 2, 0, 0.0, c, 8, s, o + 1, 32, None, 0),
+            ("checkpoint_int8", p + 1, 2, 16, 63, 64, c, s), ("checkpoint_int8", p, 2, 16, 64, 64, c, s + 1),
+            ("checkpoint_int8", p + 2, 0, 8, 31, 32, c, s), ("restore_int8", c, s, 16, 64, o + 1, 2, 64),
+            ("restore_int8", c, s, 8, 32, o + 2, 0, 32), ("restore_int8", c, s + 2, 16, 64, o, 2, 64),
+            ("pack_rows", p + 1, 64, 1, 16, 63, o, 64), ("pack_rows", p, 64, 1, 16, 63, o + 1, 64),
+            ("act_backward", p + 1, 64, None, 0, None, 16, 63, 2, 0, None, 64, s, 600, o)):
+        with pytest.raises(RuntimeError, match="aligned to"):
+            N.call("dsv4_b200_" + name, *args, st)
+    N.check_device_status()
+
+
 # ---- long ----
 
 def test_more_than_two_to_the_31_values():
