@@ -484,6 +484,11 @@ __device__ __forceinline__ float code8_value(uint32_t w, int byte) {
   return __uint_as_float(prmt(w ^ 0x80808080u, 0x4b000000u, 0x7440u + byte)) - 8388736.f;
 }
 
+// No pointer of the kernels below is __restrict__: under programmatic dependent
+// launch a kernel's blocks may be resident while the kernel before it still
+// writes what they will read, and a load from memory declared read-only may
+// take the non-coherent path, which the wait at entry says nothing about.
+
 // ---- 8 consecutive 16-bit values from any even address ----
 // A matrix's first byte and the one behind its last.
 struct Extent {
@@ -594,9 +599,9 @@ __device__ __forceinline__ uint32_t max_u16x2(uint32_t a, uint32_t b) {
 // value 53 and 155).
 template <int DT, bool VEC>
 __global__ void __launch_bounds__(256, DT == DSV4_F32 || !VEC ? 4 : 6)
-    checkpoint_kernel(const void* __restrict__ x, int64_t ld, int64_t m, int64_t k,
-                      int64_t k32, uint32_t col_blocks, int8_t* __restrict__ codes,
-                      float* __restrict__ scales) {
+    checkpoint_kernel(const void* x, int64_t ld, int64_t m, int64_t k,
+                      int64_t k32, uint32_t col_blocks, int8_t* codes,
+                      float* scales) {
   pdl_entry();
   constexpr bool F32 = DT == DSV4_F32;
   constexpr int kWords = F32 ? 8 : 4;
@@ -741,8 +746,8 @@ __device__ __forceinline__ void store_shifted8(uint16_t* p, const uint32_t (&w)[
 
 template <int DT, bool VEC>
 __global__ void __launch_bounds__(256, VEC ? 8 : 5)
-    restore_kernel(const int8_t* __restrict__ codes, const float* __restrict__ scales, int64_t m,
-                   int64_t k, int64_t k32, uint32_t col_blocks, void* __restrict__ out, int64_t ldo) {
+    restore_kernel(const int8_t* codes, const float* scales, int64_t m,
+                   int64_t k, int64_t k32, uint32_t col_blocks, void* out, int64_t ldo) {
   pdl_entry();
   __shared__ float s_scale[8][33];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -879,8 +884,8 @@ __global__ void __launch_bounds__(256, 4) act_backward_kernel(const ActBackward 
 // A block: 32 columns; its 8 warps take every eighth slab, then add up.
 template <bool BF16>
 __global__ void __launch_bounds__(256)
-    column_sum_kernel(const float* __restrict__ partial, int64_t slabs, int64_t n,
-                      void* __restrict__ out) {
+    column_sum_kernel(const float* partial, int64_t slabs, int64_t n,
+                      void* out) {
   pdl_entry();
   __shared__ float s_sum[8][32];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -901,8 +906,8 @@ __global__ void __launch_bounds__(256)
 // ---- rows of any strides -> rows that TMA can read (16-byte aligned) ----
 // 32 x 32 tiles through shared memory: reads follow the smaller stride.
 __global__ void __launch_bounds__(256)
-    pack_rows_kernel(const uint16_t* __restrict__ in, int64_t s0, int64_t s1, int64_t rows,
-                     int64_t cols, uint32_t col_blocks, uint16_t* __restrict__ out, int64_t ldo) {
+    pack_rows_kernel(const uint16_t* in, int64_t s0, int64_t s1, int64_t rows,
+                     int64_t cols, uint32_t col_blocks, uint16_t* out, int64_t ldo) {
   pdl_entry();
   __shared__ uint16_t tile[32][33];
   const int a = threadIdx.x & 31, b = threadIdx.x >> 5;
@@ -923,8 +928,8 @@ __global__ void __launch_bounds__(256)
 // Rows of contiguous values, from any even address to 16-byte aligned ones:
 // windows of two pieces, shifted (8192 x 7167: 39 us; through the tiles 110).
 __global__ void __launch_bounds__(256)
-    pack_windows_kernel(const uint16_t* __restrict__ in, int64_t ld, int64_t rows, int64_t cols,
-                        uint32_t col_blocks, uint16_t* __restrict__ out, int64_t ldo) {
+    pack_windows_kernel(const uint16_t* in, int64_t ld, int64_t rows, int64_t cols,
+                        uint32_t col_blocks, uint16_t* out, int64_t ldo) {
   pdl_entry();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t row_block = blockIdx.x / col_blocks, col_block = blockIdx.x - row_block * col_blocks;
