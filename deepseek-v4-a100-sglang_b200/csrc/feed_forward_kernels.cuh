@@ -430,14 +430,18 @@ __device__ __forceinline__ float keep_group16(const float (&v)[32], float limit,
   if (!(squares < CUDART_INF_F && most * most * live <= kStandsOut * squares))
     return keep_group16_wide(v, limit, keep_sign, codes);
   const uint32_t top = __float_as_uint(most);
-  const float inv = group_inverse(top, kSteps16), step = group_step(top, kSteps16);
+  // one step is kept free for the largest value of a group that passes the
+  // limit: its last step may have to be counted up
+  const bool passes = most > limit;
+  const float inv = passes ? group_inverse(top, kSteps16 - 1) : group_inverse(top, kSteps16);
+  const float step = passes ? group_step(top, kSteps16 - 1) : group_step(top, kSteps16);
   if (inv == 0.f) {
 #pragma unroll
     for (int j = 0; j < 16; ++j) codes[j] = 0;
     return step;
   }
   // (a kept value is at most `most`: below the limit there is no side to keep)
-  if (!(most > limit) && !keep_sign) {
+  if (!passes && !keep_sign) {
 #pragma unroll
     for (int j = 0; j < 16; ++j)
       codes[j] = prmt(__float_as_uint(__fmaf_rn(v[2 * j], inv, kWhole)),
