@@ -436,6 +436,7 @@ __device__ __forceinline__ float keep_group16(const float (&v)[32], float limit,
   const float inv = passes ? group_inverse(top, kSteps16 - 1) : group_inverse(top, kSteps16);
   const float step = passes ? group_step(top, kSteps16 - 1) : group_step(top, kSteps16);
   if (inv == 0.f) {
+    if (keep_sign && most > 0.f) return keep_group16_wide(v, limit, keep_sign, codes);
 #pragma unroll
     for (int j = 0; j < 16; ++j) codes[j] = 0;
     return step;

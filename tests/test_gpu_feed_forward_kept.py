@@ -1,5 +1,5 @@
 """Values before an activation as the backward pass reads them: their side of
-the clamp limit."""
+the clamp limit and of zero."""
 
 import math
 
@@ -85,3 +85,36 @@ def test_values_a_step_from_the_limit(limit, dtype):
         dg = 32 * z.clamp(-lim, lim) * s(c)
         assert_each(f"{kind} du", gx[:, 0], du, torch.where(z.abs() <= lim, off(du, ae(c)), torch.zeros_like(z)))
         assert_each(f"{kind} dg", gx[:, 1], dg, off(dg, 1.15 * z.abs() / 32767 + se(c) * z.abs()))
+
+
+@pytest.mark.parametrize("beside", [0.0, 1.0, -1.0, 2.0 ** -101, 2.0 ** 40])
+@pytest.mark.parametrize("e", [45, 52, 55, 61, 62])
+def test_relu_keeps_the_sign_of_tiny_values(e, beside):
+    """2^-90 to 2^-124, alone in their group or beside another value: relu's
+    slope is 1 above zero and 0 below it."""
+    import dsv4_b200 as D
+    m, n, k = 4, 64, 16
+    x = torch.zeros(m, k, device="cuda", dtype=BF16)
+    x[:, 0] = torch.tensor([1.0, -1.0, 1.0, -1.0], device="cuda") * 2.0 ** -e
+    x[:, 1] = 1
+    w = torch.zeros(n, k, device="cuda", dtype=BF16)
+    w[:, 0] = 2.0 ** -e
+    w[n // 2:, 0] *= -1
+    w[5, 0], w[n - 1, 0] = 0, 0
+    w[7, 1], w[n - 3, 1] = beside, beside
+    z = x.double() @ w.double().T
+    dy = torch.full((m, n), 0.5, device="cuda", dtype=BF16)
+    bias = torch.zeros(n, device="cuda", dtype=BF16)
+    y, saved = D.dense_forward_save(x, w, bias, activation="relu")
+    dz = 0.5 * (z > 0).double()
+    _, gw, gb = D.dense_backward(dy, saved)
+    want = dz.T @ x.double()
+    assert_each("grad_weight", gw, want, 2.0 ** -8 * want.abs())
+    assert_each("grad_bias", gb, dz.sum(0), torch.zeros(n, device="cuda", dtype=torch.float64))
+    # as the gate of a block, ups 1
+    one = torch.zeros(n, k, device="cuda", dtype=BF16)
+    one[:, 1] = 1
+    w2 = torch.full((8, n), 0.125, device="cuda", dtype=BF16)
+    _, saved = D.gated_feed_forward_save(x, torch.cat((w, one)), w2, activation="relu")
+    _, g13, _ = D.gated_feed_forward_backward(torch.full((m, 8), 0.5, device="cuda", dtype=BF16), saved)
+    assert_each("grad_w1", g13[:n], want, 2.0 ** -8 * want.abs())
