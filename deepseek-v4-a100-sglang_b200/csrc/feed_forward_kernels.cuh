@@ -245,10 +245,9 @@ constexpr int kGroup = 32;
 constexpr float kTinyGroup = 7.8886090522101181e-31f;  // 2^-100
 
 
-// Whole steps up to amax: 127 in 8 bits, 32767 in 16.  The scale is rounded
-// toward zero: that many steps never pass amax, so the largest finite value
-// stays finite.
-constexpr float kSteps8 = 127.f, kSteps16 = 32767.f;
+// Whole steps up to amax.  The scale is rounded toward zero: that many steps
+// never pass amax, so the largest finite value stays finite.
+constexpr float kSteps8 = 127.f;
 
 __device__ __forceinline__ float group_step(uint32_t amax_bits, float steps) {
   const float amax = __uint_as_float(amax_bits);
@@ -340,9 +339,9 @@ __device__ __forceinline__ uint32_t quantize4_f32(const float (&v)[4], float inv
 // What the backward pass needs of a value before its activation is kept as
 // groups too, in 8 bits or in 16: a thread's own 32 fp32 sums -> codes and the
 // scale.  (A sum next to the border of two codes is itself only known to its
-// last bits.)  16 bits hold a group to amax / 65534, where bf16 would be off by
-// 1/512 of every value: gradients are then as exact as their own rounding, at
-// 2.125 bytes a value.
+// last bits.)  16 bits hold a value to 2^-15 of the group's largest, where bf16
+// may be off by 2^-8 of every value: gradients are then as exact as their own
+// rounding, at 2.125 bytes a value.
 __device__ __forceinline__ uint32_t group_top(const float (&v)[32]) {
   uint32_t top = 0;
 #pragma unroll
@@ -365,30 +364,87 @@ __device__ __forceinline__ float keep_group8(const float (&v)[32], uint32_t (&co
   return group_step(top, kSteps8);
 }
 
-// With a clamp limit the code stays on the value's side of it: the backward
-// pass asks |z| <= limit of the kept value, and one kept over the border would
-// lose or gain its whole gradient.  For relu a value other than zero keeps its
-// sign the same way.  That is one step instead of half a step next to the
-// border.
+// 16 bits: a sign and 15 bits of magnitude that count up with the value, in
+// steps of the group's largest value / kSteps.  From kEdge steps on the code is
+// the whole number of steps; below that the leading bits of a float, kBits
+// digits behind the leading one (at code 2^14 both are kEdge steps, and both go
+// on by one step).  So a value is held to half a step (2^-15 of the largest) and,
+// where that is more, to 2^-(kBits + 1) of itself: 2^-10 for bf16 tensors, 2^-11
+// for fp16, at least as well as in the tensor's own type.  No value loses its
+// digits to larger neighbours, however many there are.  (Down to 2^-36 of the
+// largest, 2^-19 for fp16, which trades range for a digit; below that to 2^-45
+// and 2^-29 of it.)
 //
-// Equal steps serve a group as long as no value stands out: with the largest at
-// most 4 times the root of the mean square (of the `live` columns that there
-// are) they are within 6.2e-5 of that root.  A group with an outlier would lose
-// its small values, and one with an infinity or a NaN all of them: those are
-// kept as fp16 multiples of a power of two, every value within 2^-12 of itself,
-// and say so by a negative scale.
-constexpr float kStandsOut = 16.f;
+// Equal steps, with a test for a value that stands out of its group, cost less
+// but fail beside two such values: their own squares raise the mean they are
+// compared with.  Here against that: 2048 x 2048 -> 7168, z kept, gelu 59.7 us
+// (59.0), its activation backward 23.8 (22.2); gated 4096 x 1024 -> 2 x 2048 45
+// (40), its backward pass 43.8 (40.3); gated 4096 x 7168 -> 2 x 2048 174 (172).
+template <bool BF16>
+struct Kept16 {
+  static constexpr int kBits = BF16 ? 9 : 10;
+  static constexpr int kEdge = 1 << kBits;
+  static constexpr int kShift = 23 - kBits;
+  // the largest is code 32766: one is left to count it up
+  static constexpr float kSteps = 32766 - 16384 + kEdge;
+  static constexpr float kLinear = 8388608.f + (16384 - kEdge);  // 2^23 and the code of no steps
+  // kEdge times the power of two has the bits 2^14 << kShift
+  static constexpr float kToFine = BF16 ? 0x1p-104f * (1.f + 0x1p-10f) : 0x1p-121f * (1.f + 0x1p-11f);
+  static constexpr float kFromFine = BF16 ? 0x1p104f : 0x1p121f;
+};
 
-// acc += a * a, two at a time
-__device__ __forceinline__ void add_squares(float (&acc)[2], float a0, float a1) {
-  asm("{\n\t.reg .b64 a, c;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 c, {%0, %1};\n\t"
-      "fma.rn.f32x2 c, a, a, c;\n\tmov.b64 {%0, %1}, c;\n\t}"
-      : "+f"(acc[0]), "+f"(acc[1])
-      : "f"(a0), "f"(a1));
+// A value of code 16 bits `hi` of w; scale > 0.
+template <bool BF16>
+__device__ __forceinline__ float kept16_value(uint32_t w, int hi, float scale) {
+  using K = Kept16<BF16>;
+  const uint32_t p = prmt(w & 0x7fff7fffu, 0x4b000000u, hi ? 0x7432u : 0x7410u);  // 2^23 + magnitude
+  const float linear = __uint_as_float(p) - K::kLinear;
+  const float fine = __uint_as_float(p << K::kShift) * K::kFromFine;
+  const float v = scale * (linear >= K::kEdge ? linear : fine);
+  return __uint_as_float(__float_as_uint(v) | ((hi ? w : w << 16) & 0x80000000u));
 }
 
-__device__ __forceinline__ float keep_group16_wide(const float (&v)[32], float limit, bool keep_sign,
-                                                   uint32_t (&codes)[16]) {
+// Magnitude code (its low 15 bits) of |t| steps.  Below the edge the float's
+// digits are cut, not rounded: kToFine stands half a step above its power of
+// two, so that the error stays within 2^-(kBits + 1) to either side.
+template <bool BF16>
+__device__ __forceinline__ uint32_t kept16_magnitude(float t) {
+  using K = Kept16<BF16>;
+  uint32_t m;
+  asm("{\n\t.reg .pred p;\n\t.reg .f32 a;\n\t"
+      "abs.f32 a, %1;\n\t"
+      "setp.ge.f32 p, a, %2;\n\t"
+      "mul.f32 %0, %1, %3;\n\t"
+      "shr.u32 %0, %0, %4;\n\t"
+      "@p add.f32 %0, a, %5;\n\t}"
+      : "=&r"(m)
+      : "f"(t), "f"(static_cast<float>(K::kEdge)), "f"(K::kToFine), "n"(K::kShift), "f"(K::kLinear));
+  return m;
+}
+
+// Codes of two values: their magnitudes' and their signs.
+__device__ __forceinline__ uint32_t kept16_signs(uint32_t m, float v0, float v1) {
+  const uint32_t signs = prmt(__float_as_uint(v0), __float_as_uint(v1), 0x7632u);
+  return (m & 0x7fff7fffu) | (signs & 0x80008000u);
+}
+
+template <bool BF16>
+__device__ __forceinline__ uint32_t kept16_codes(float v0, float v1, float inv) {
+  const uint32_t m0 = kept16_magnitude<BF16>(v0 * inv), m1 = kept16_magnitude<BF16>(v1 * inv);
+  return kept16_signs(prmt(m0, m1, 0x5410u), v0, v1);
+}
+
+// max(|a|, |b|, |c|); NaN if one is
+__device__ __forceinline__ float max_abs_nan(float a, float b, float c) {
+  float r;
+  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
+// A group that holds an infinity or a NaN: fp16 multiples of a power of two,
+// which lose only that value, marked by a negative scale.
+__device__ __forceinline__ float keep_not_finite(const float (&v)[32], float limit, bool keep_sign,
+                                              uint32_t (&codes)[16]) {
   uint32_t top = 0;  // of the finite values
 #pragma unroll
   for (int j = 0; j < 32; ++j) {
@@ -397,91 +453,73 @@ __device__ __forceinline__ float keep_group16_wide(const float (&v)[32], float l
   }
   // the largest lands in [2^14, 2^15); scales from 2^-114 to 2^113
   const uint32_t e = max(top >> 23, 27u) - 14u;
-  const float scale = __uint_as_float(e << 23), inv = __uint_as_float((254u - e) << 23);
-  const bool limited = limit < CUDART_INF_F || keep_sign;
+  const float unit = __uint_as_float(e << 23), inv = __uint_as_float((254u - e) << 23);
 #pragma unroll
   for (int j = 0; j < 16; ++j) {
     uint32_t w = pack_16<false>(v[2 * j] * inv, v[2 * j + 1] * inv);
-    if (limited) {
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const float x = v[2 * j + i];
-        const uint32_t one = i ? 0x10000u : 1u, n = i ? w >> 16 : w & 0xffffu;
-        const bool over = fabsf(x) > limit, kept = fabsf(unpack_16<false>(w, i) * scale) > limit;
-        if (over && !kept) w += one;  // magnitudes count up away from zero
-        if (!over && kept) w -= one;
-        if (keep_sign && (n & 0x7fffu) == 0 && x != 0.f) w += one;
-      }
-    }
-    codes[j] = w;
-  }
-  return -scale;
-}
-
-__device__ __forceinline__ float keep_group16(const float (&v)[32], float limit, bool keep_sign,
-                                              int live, uint32_t (&codes)[16]) {
-  float most = 0.f, sum[2] = {};
-#pragma unroll
-  for (int j = 0; j < 16; ++j) {
-    most = fmaxf(most, fmaxf(fabsf(v[2 * j]), fabsf(v[2 * j + 1])));
-    add_squares(sum, v[2 * j], v[2 * j + 1]);
-  }
-  const float squares = sum[0] + sum[1];  // infinite or NaN where a value is
-  if (!(squares < CUDART_INF_F && most * most * live <= kStandsOut * squares))
-    return keep_group16_wide(v, limit, keep_sign, codes);
-  const uint32_t top = __float_as_uint(most);
-  // one step is kept free for the largest value of a group that passes the
-  // limit: its last step may have to be counted up
-  const bool passes = most > limit;
-  const float inv = passes ? group_inverse(top, kSteps16 - 1) : group_inverse(top, kSteps16);
-  const float step = passes ? group_step(top, kSteps16 - 1) : group_step(top, kSteps16);
-  if (inv == 0.f) {
-    if (keep_sign && most > 0.f) return keep_group16_wide(v, limit, keep_sign, codes);
-#pragma unroll
-    for (int j = 0; j < 16; ++j) codes[j] = 0;
-    return step;
-  }
-  // (a kept value is at most `most`: below the limit there is no side to keep)
-  if (!passes && !keep_sign) {
-#pragma unroll
-    for (int j = 0; j < 16; ++j)
-      codes[j] = prmt(__float_as_uint(__fmaf_rn(v[2 * j], inv, kWhole)),
-                      __float_as_uint(__fmaf_rn(v[2 * j + 1], inv, kWhole)), 0x5410u);
-    return step;
-  }
-#pragma unroll
-  for (int j = 0; j < 16; ++j) {
-    float q[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const float x = v[2 * j + i];
-      q[i] = __fmaf_rn(x, inv, kWhole);
-      const float n = q[i] - kWhole, toward = x < 0.f ? 1.f : -1.f;  // toward zero
-      const bool over = fabsf(x) > limit, kept = fabsf(n * step) > limit;
-      if (over && !kept) q[i] -= toward;
-      if (!over && kept) q[i] += toward;
-      if (keep_sign && n == 0.f && x != 0.f) q[i] -= toward;
+      const uint32_t one = i ? 0x10000u : 1u;  // magnitudes count up away from zero
+      if (keep_sign && (w & (0x7fffu * one)) == 0 && x != 0.f) w += one;
+      const bool over = fabsf(x) > limit, kept = fabsf(unit * unpack_16<false>(w, i)) > limit;
+      if (over && !kept) w += one;
+      if (!over && kept) w -= one;
     }
-    codes[j] = prmt(__float_as_uint(q[0]), __float_as_uint(q[1]), 0x5410u);
+    codes[j] = w;
   }
-  return step;
+  return -unit;
 }
 
-// Codes back to whole numbers: the code, moved to be positive, as the low bits
-// of a float 2^23 + code.
-__device__ __forceinline__ float code16_value(uint32_t w, int hi) {
-  return __uint_as_float(prmt(w ^ 0x80008000u, 0x4b000000u, hi ? 0x7432u : 0x7410u)) - 8421376.f;
+// With a clamp limit the code stays on the value's side of it: the backward
+// pass asks |z| <= limit of the kept value, and one kept over the border would
+// lose or gain its whole gradient.  Codes count up with the value, so only
+// those that share the limit's own code can be on the wrong side, and all of
+// these move by one if they are.  For relu a value other than zero keeps its
+// sign the same way.  That is one step instead of half a step next to the
+// border.
+template <bool BF16>
+__device__ __forceinline__ float keep_group16(const float (&v)[32], float limit, bool keep_sign,
+                                              uint32_t (&codes)[16]) {
+  using K = Kept16<BF16>;
+  float most = fabsf(v[0]);
+#pragma unroll
+  for (int j = 0; j < 16; ++j) most = max_abs_nan(most, v[2 * j], v[2 * j + 1]);
+  if (!(most < CUDART_INF_F)) return keep_not_finite(v, limit, keep_sign, codes);
+  const uint32_t top = __float_as_uint(fmaxf(most, kTinyGroup));
+  const float inv = group_inverse(top, K::kSteps), scale = group_step(top, K::kSteps);
+  // (no kept value is off by 2^-8 of itself: further below the limit there is no side to keep)
+  if (most * (1.f + 0x1p-8f) <= limit && !keep_sign) {
+#pragma unroll
+    for (int j = 0; j < 16; ++j) codes[j] = kept16_codes<BF16>(v[2 * j], v[2 * j + 1], inv);
+    return scale;
+  }
+  const uint32_t at = kept16_magnitude<BF16>(limit * inv);
+  const bool up = kept16_value<BF16>(at, 0, scale) <= limit;  // values over the limit go up, or the others down
+#pragma unroll
+  for (int j = 0; j < 16; ++j) {
+    uint32_t m[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const float x = fabsf(v[2 * j + i]);
+      m[i] = kept16_magnitude<BF16>(x * inv);
+      if (m[i] == at && (x > limit) == up) m[i] += up ? 1u : 0xffffffffu;
+      if (keep_sign && m[i] == 0 && x != 0.f) m[i] = 1;
+    }
+    codes[j] = kept16_signs(prmt(m[0], m[1], 0x5410u), v[2 * j], v[2 * j + 1]);
+  }
+  return scale;
 }
 
 // N 16-bit codes of a group (scale < 0: fp16 multiples) -> values
-template <int N>
+template <bool BF16, int N>
 __device__ __forceinline__ void kept16_values(const uint32_t (&w)[N / 2], float scale, float (&v)[N]) {
   if (scale < 0.f) {
 #pragma unroll
     for (int j = 0; j < N; ++j) v[j] = -scale * unpack_16<false>(w[j >> 1], j & 1);
   } else {
 #pragma unroll
-    for (int j = 0; j < N; ++j) v[j] = scale * code16_value(w[j >> 1], j & 1);
+    for (int j = 0; j < N; ++j) v[j] = kept16_value<BF16>(w[j >> 1], j & 1, scale);
   }
 }
 
@@ -858,7 +896,7 @@ __global__ void __launch_bounds__(256, 4) act_backward_kernel(const ActBackward 
 #pragma unroll
             for (int j = 0; j < 8; ++j) z[j] = s * code8_value(c[j >> 2], j & 3);
           } else {
-            kept16_values<8>(c, s, z);
+            kept16_values<BF16>(c, s, z);
           }
 #pragma unroll
           for (int j = 0; j < 8; ++j) {

@@ -354,10 +354,10 @@ __device__ __forceinline__ void codes_to_rows(uint32_t slice, int lane, const ui
   __syncwarp();
 }
 
-// A warp's 32 rows of one kept group, columns `at`.. of code rows of `ld`; the
-// first `live` of them are columns of the matrix.
+// A warp's 32 rows of one kept group, columns `at`.. of code rows of `ld`.
+template <bool BF16>
 __device__ __forceinline__ void keep_rows(const F16GemmParams& p, uint32_t slice, int lane,
-                                          const float (&v)[32], int64_t ld, int row0, int at, int live) {
+                                          const float (&v)[32], int64_t ld, int row0, int at) {
   float s;
   if (p.zbits == 8) {
     uint32_t q[8];
@@ -365,7 +365,7 @@ __device__ __forceinline__ void keep_rows(const F16GemmParams& p, uint32_t slice
     codes_store(slice, lane, q, static_cast<int8_t*>(p.zq), ld, row0, p.m, at);
   } else {
     uint32_t q[16];
-    s = keep_group16(v, p.limit, p.act == kActRelu, live, q);
+    s = keep_group16<BF16>(v, p.limit, p.act == kActRelu, q);
     chunk_store(slice, lane, q, F16Mat{p.zq, ld, 1}, row0, p.m, at, static_cast<int>(ld));
   }
   if (row0 + lane < p.m) p.zs[static_cast<int64_t>(at >> 5) * p.m + row0 + lane] = s;
@@ -384,6 +384,7 @@ __device__ __forceinline__ float kept_fetch(const F16GemmParams& p, uint4 (&r)[4
 }
 
 // 16 values of a lane's row: codes in the slice (16 bits) or in its registers.
+template <bool BF16>
 __device__ __forceinline__ void kept_half(const F16GemmParams& p, uint32_t slice, int lane, int half,
                                           const uint32_t (&q)[8], float scale, float (&v)[16]) {
   if (p.zbits == 8) {
@@ -393,7 +394,7 @@ __device__ __forceinline__ void kept_half(const F16GemmParams& p, uint32_t slice
     const uint4 a = ld_shared_v4(slice + slice_off(lane, 2 * half));
     const uint4 b = ld_shared_v4(slice + slice_off(lane, 2 * half + 1));
     const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-    kept16_values<16>(w, scale, v);
+    kept16_values<BF16>(w, scale, v);
   }
 }
 
@@ -578,7 +579,7 @@ __global__ void __launch_bounds__(F16Roles<EPI>::kThreads, 1)
               for (int j = 0; j < 32; ++j)
                 if (col + j >= p.n) v[j] = 0.f;
             }
-            keep_rows(p, slice0, lane, v, p.n32, row0, col, min(32, p.n - col));
+            keep_rows<BF16>(p, slice0, lane, v, p.n32, row0, col);
           }
           act_row(p.act, v);
           if (p.residual.p) {
@@ -599,8 +600,8 @@ __global__ void __launch_bounds__(F16Roles<EPI>::kThreads, 1)
               for (int j = 0; j < 32; ++j)
                 if (col + j >= p.n) g[j] = u[j] = 0.f;
             }
-            keep_rows(p, slice0, lane, g, 2 * p.n32, row0, col, min(32, p.n - col));
-            keep_rows(p, slice1, lane, u, 2 * p.n32, row0, static_cast<int>(p.n32) + col, min(32, p.n - col));
+            keep_rows<BF16>(p, slice0, lane, g, 2 * p.n32, row0, col);
+            keep_rows<BF16>(p, slice1, lane, u, 2 * p.n32, row0, static_cast<int>(p.n32) + col);
           }
 #pragma unroll
           for (int j = 0; j < 32; ++j) {
@@ -629,8 +630,8 @@ __global__ void __launch_bounds__(F16Roles<EPI>::kThreads, 1)
           for (int half = 0; half < 2; ++half) {
             float v[16], g[16], u[16];
             tmem_ld_f32x16(acc + c0 + 16 * half, v);
-            kept_half(p, slice0, lane, half, qg, sg, g);
-            kept_half(p, slice1, lane, half, qu, su, u);
+            kept_half<BF16>(p, slice0, lane, half, qg, sg, g);
+            kept_half<BF16>(p, slice1, lane, half, qu, su, u);
             uint32_t wg[8], wu[8], w[8];
             gated_backward_row<BF16>(p.act, p.limit, v, g, u, wg, wu, w);
 #pragma unroll

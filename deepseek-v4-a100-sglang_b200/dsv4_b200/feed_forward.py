@@ -8,8 +8,8 @@ projections), forward and backward.
 
 bf16 and fp16; sums, activations and their slopes in fp32, one rounding where
 a value is stored.  The values before an activation are kept for the backward
-pass as groups of 32 with a shared scale, in 16 bits (as whole steps, or as
-fp16 multiples where a value stands out of its group).  ``dense_forward`` and
+pass as groups of 32 with a shared scale, in 16 bits: each to 2^-15 of the
+group's largest value and to 2^-10 (fp16: 2^-11) of itself.  ``dense_forward`` and
 ``gated_feed_forward`` are differentiable; their ``*_save`` / ``*_backward``
 forms give the same steps without autograd (and are the ones to capture into a
 CUDA graph).  With ``checkpoint="int8"`` what the backward pass needs is kept

@@ -395,13 +395,19 @@ DSV4_API int dsv4_b200_mxfp4_int8_dense_gemm_noalloc(const int8_t* a_q, const fl
  * dsv4_b200_gated_gemm take any alignment.)
  * Results and `residual` have any alignment.  activation: dsv4_activation.
  * Kept values are groups of 32 values of a row that share an fp32 scale
- * amax / steps (rounded toward zero), steps 127 in 8 bits and 32767 in 16:
- * codes int8 or int16 [m][ceil32(k)], scales [ceil32(k) / 32][m], codes 16-byte
- * aligned.  code = steps v / amax to the nearest, ties to even; a group of 8
- * bits with an infinity or a NaN decodes to NaN, a group whose amax is below
- * 2^-100 to zeros.  A group of 16 bits whose amax is over 4 times its root
- * mean square, or that holds an infinity or a NaN, has a negative scale -2^e,
- * and its codes are the fp16 numbers v / 2^e.
+ * amax / steps (rounded toward zero), codes int8 or int16 [m][ceil32(k)], scales
+ * [ceil32(k) / 32][m], codes 16-byte aligned.
+ * 8 bits: steps 127, code = 127 v / amax to the nearest, ties to even; a group
+ * with an infinity or a NaN decodes to NaN, one whose amax is below 2^-100 to
+ * zeros.
+ * 16 bits: a sign (bit 15) and a magnitude code c, value = scale * t(c), with
+ * E = 512 (bf16) or 1024 (fp16) and steps 16382 + E: t = c - 16384 + E from c =
+ * 16384 on, below that t = E * 2^e * (1 + f / E) of the float with c's leading
+ * 5 (4) bits as its exponent, e = -32 (-16) at 0 and rising by one, and f the
+ * other 9 (10), subnormal at exponent 0.  Every value is held to 2^-15 of amax
+ * and to 2^-10 (fp16: 2^-11) of itself, this down to 2^-36 (2^-19) of amax.
+ * amax counts as 2^-100 at least.  A group with an infinity or a NaN has a
+ * negative scale -2^e, and its codes are the fp16 numbers v / 2^e.
  * z_bits = 0, 8 or 16 (0: z_codes and z_scales NULL). */
 typedef enum dsv4_activation {
   DSV4_ACT_NONE = 0,
