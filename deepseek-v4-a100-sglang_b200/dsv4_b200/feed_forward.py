@@ -30,6 +30,7 @@ from dataclasses import dataclass
 from typing import Optional
 
 import torch
+import torch.autograd.forward_ad as _forward_ad
 
 from . import _native as N
 
@@ -93,6 +94,15 @@ def _explain_options(activation, checkpoint, clamp_limit=None) -> None:
         raise ValueError(f'checkpoint must be None or "int8", got {checkpoint!r}')
     if clamp_limit is not None and not (0 < float(clamp_limit) < math.inf):
         raise ValueError(f"clamp_limit must be positive and finite, got {clamp_limit}")
+
+
+def _refuse_tangents(*tensors) -> None:
+    """A tensor of forward-mode autograd carries a tangent that a kernel does not see."""
+    if _forward_ad._current_level < 0 or not torch._C._is_fwd_grad_enabled():
+        return
+    for t in tensors:
+        if isinstance(t, torch.Tensor) and _forward_ad.unpack_dual(t).tangent is not None:
+            raise NotImplementedError("the feed-forward operators have no forward-mode derivative")
 
 
 def _is_matrix(t, rows, cols, dtype, dev) -> bool:
@@ -240,6 +250,7 @@ def checkpoint_int8(x: torch.Tensor) -> Int8Checkpoint:
     most half a step, ``amax / 254`` of its group, and the rounding to x's type."""
     if not isinstance(x, torch.Tensor):
         raise TypeError(f"x must be a tensor, got {type(x).__name__}")
+    _refuse_tangents(x)
     shape, dtype = x.shape, x.dtype
     if len(shape) != 2:
         raise ValueError(f"x must be 2-D, got shape {tuple(shape)}")
@@ -310,6 +321,7 @@ class SavedDense:
 
 def _check_dense(x, weight, bias, activation, residual, checkpoint):
     """(m, n, k) of a call whose arguments go together; raises otherwise."""
+    _refuse_tangents(x, weight, bias, residual)
     try:
         (m, k), n, dt, dev = x.shape, weight.shape[0], x.dtype, x.get_device()
         if (n and k and dev >= 0 and dt in _DTYPES and _is_matrix(weight, n, k, dt, dev)
@@ -419,6 +431,7 @@ def dense_backward(grad_out, saved: SavedDense, *, need_x=True, need_weight=True
     ``(grad_x, grad_weight, grad_bias)``, None where not needed.  (The
     residual's gradient is dy.)"""
     m, n, k = saved.shape
+    _refuse_tangents(grad_out)
     _explain_matrix(grad_out, "grad_out", m, n, like=saved.weight)
     _explain_device(grad_out, weight=saved.weight)
     _on_stream(saved, saved.x, saved.weight)
@@ -494,6 +507,7 @@ class _DenseFunction(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad_out):
+        _refuse_tangents(grad_out)
         need = ctx.needs_input_grad
         gx = gw = gb = None
         if need[0] or need[1] or need[2]:
@@ -521,6 +535,7 @@ class SavedFeedForward:
 
 def _check_ffn(x, w13, w2, activation, clamp_limit, residual, checkpoint):
     """(m, hidden, inter, out) of a call whose arguments go together; raises otherwise."""
+    _refuse_tangents(x, w13, w2, residual)
     try:
         (m, hidden), (out, inter), dt, dev = x.shape, w2.shape, x.dtype, x.get_device()
         if (hidden and out and inter and dev >= 0 and dt in _DTYPES
@@ -640,6 +655,7 @@ def gated_feed_forward_backward(grad_out, saved: SavedFeedForward, *, need_x=Tru
     The gradient of the gated product, ``dh = dy @ w2``, stays in the
     registers of the kernel that turns it into the gradients of gate and up."""
     m, hidden, inter, n = saved.shape
+    _refuse_tangents(grad_out)
     _explain_matrix(grad_out, "grad_out", m, n, like=saved.w2)
     _explain_device(grad_out, w2=saved.w2)
     _on_stream(saved, saved.x, saved.w13, saved.w2)
@@ -699,6 +715,7 @@ class _FeedForwardFunction(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad_out):
+        _refuse_tangents(grad_out)
         need = ctx.needs_input_grad
         gx = g13 = g2 = None
         if need[0] or need[1] or need[2]:
