@@ -24,6 +24,7 @@ backward pass).  All results are the same bits from call to call.
 from __future__ import annotations
 
 import contextlib
+import ctypes
 import functools
 import math
 from dataclasses import dataclass
@@ -359,9 +360,13 @@ def _dense_kept(m, n, k, act, bits, keep_x, keep_z):
 
 @functools.lru_cache(maxsize=4096)
 def _dense_workspace(m, n, k, act, bias, restore):
-    """Slabs of the bias gradient (those of act_backward_slabs), and the layout
-    of dz, their partial sums and the restored x."""
-    slabs = max(1, min(4 * 148 // -(-n // 256), -(-m // 32))) if bias else 0
+    """Slabs of the bias gradient, and the layout of dz, their partial sums and
+    the restored x."""
+    slabs = 0
+    if bias:
+        count = ctypes.c_int64(0)
+        _call("act_backward_slabs", m, n, ctypes.byref(count))
+        slabs = count.value
     return slabs, _layout(m * _up(n, 8) * 2 if act else None, slabs * n * 4 if bias else None,
                           m * _up(k, 8) * 2 if restore else None)
 
