@@ -206,8 +206,9 @@ int stream_tokens(int64_t m) {
 // at least 8 blocks each.  Doubling the cluster costs 2 %.  The least of all
 // tile heights and cluster sizes is taken.  (Fitted to 6 shapes, 512 x 1024 to
 // 14336 x 1024 and 4096 x 7168, at 1 to 128 tokens: the choice is on average
-// 2 %, at most 10 % slower than the best of all measured.)  A unit of this
-// count is 2.35 ns, on top of 3.2 us.
+// 2 %, at most 10 % slower than the best of all measured; the same count is used
+// up to 1,024 tokens, where only the cases beside takes_stream were measured.)  A
+// unit of this count is 2.35 ns, on top of 3.2 us.
 double pick_stream(const F16GemmParams& q, bool gated, F16StreamParams& p, bool* two_per_sm) {
   const int kblocks = (q.k + 63) / 64, step = gated ? 32 : 16;
   const int token_tiles = (q.m + p.tn - 1) / p.tn;
@@ -661,7 +662,7 @@ int dsv4_b200_act_backward(const void* dy, int64_t lddy, const void* z_codes, in
 }
 
 // dW = d^T x, with x as it is or restored from its 8-bit codes first: rounded to
-// 16 bits, 2^-9 (fp16 2^-12) of a value that the codes hold to amax / 254.
+// 16 bits, 2^-8 (fp16 2^-11) of a value that the codes hold to amax / 254.
 static int weight_gradient(const void* d, int64_t ldd, int d_mn, const void* x, int64_t ldx, int x_mn,
                            const int8_t* x_codes, const float* x_scales, void* x_restored,
                            int64_t ldxr, int64_t rows, int64_t cols, int64_t m, int dtype, void* dw,

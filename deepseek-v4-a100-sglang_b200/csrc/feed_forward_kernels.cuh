@@ -839,8 +839,8 @@ __global__ void __launch_bounds__(256, VEC ? 8 : 5)
 // result every time).  One pass over dy and z.  Without an activation only
 // the sums are formed (dz = dy).  A lane owns 8 columns, a block 256; warps
 // take every eighth row of the slab.  Bound by its arithmetic next to memory:
-// 2048 x 7168 bf16 with the bias gradient takes 21 us for gelu (30 without the
-// next row's loads in flight) and 20 for relu.
+// 2048 x 7168 bf16 and its bias gradient take 23 us for gelu (the next row's
+// loads in flight save 9) and 18 for relu.
 struct ActBackward {
   const void* dy;
   int64_t lddy;

@@ -16,7 +16,9 @@
 // warp 1 of the leader MMA issuer, the warps from 4 on epilogue.  The two 256-column accumulators in TMEM let the
 // epilogue of one tile overlap the products of the next.
 //
-// Epilogues (all arithmetic in fp32, one rounding when a value is stored):
+// Epilogues (all arithmetic in fp32, one rounding when a value is stored; h, dg
+// and du are stored in 16 bits because the next product's operands are: 2^-8 of
+// a value in bf16, 2^-11 in fp16, where h past 65,504 becomes an infinity):
 //   kEpiLinear    y = act(D + bias) + residual; optionally z = D + bias is
 //                 kept for the backward pass (groups of 32 in 16 or 8 bits)
 //   kEpiGated     B holds gate rows [0, n) and up rows [n, 2n); the tile takes
@@ -43,10 +45,10 @@ enum F16Epi : int { kEpiLinear = 0, kEpiGated = 1, kEpiGatedBwd = 2 };
 
 // Epilogue warps and their 2-KB shared slices.  The forward epilogues fit 96
 // registers and one slice: 16 warps (2048 x 2048 -> 7168 with bias, gelu,
-// residual and z kept: 61 us, 65 with 12, 71 with 8; gated 4096 x 1024 -> 2 x
-// 2048 kept: 33, 38 with 8).  The gate's backward pass turns two matrices over
+// residual and z kept: 60 us, 63 with 12, 67 with 8; gated 4096 x 1024 -> 2 x
+// 2048 with a limit and z kept: 37, 38 and 39).  The gate's backward pass turns two matrices over
 // in place and is best with few warps and all of their registers (4096 x 1024
-// -> 2048: 40 us, 46 with 12).
+// -> 2048: 43 us, 46 with 12, 50 with 16).
 template <int EPI>
 struct F16Roles {
   static constexpr int kEpiWarps = EPI == kEpiGatedBwd ? 8 : 16;

@@ -247,7 +247,7 @@ def _empty_codes(rows: int, cols: int, like: torch.Tensor):
 
 def checkpoint_int8(x: torch.Tensor) -> Int8Checkpoint:
     """Keep the rows of ``x`` [M, K] (fp32, fp16 or bf16) in 8 bits: 1.125
-    bytes per value.  ``restore_int8(checkpoint_int8(x))`` differs from x by at
+    bytes per value.  Codes have no gradient: for autograd a graph ends here.  ``restore_int8(checkpoint_int8(x))`` differs from x by at
     most half a step, ``amax / 254`` of its group, and the rounding to x's type."""
     if not isinstance(x, torch.Tensor):
         raise TypeError(f"x must be a tensor, got {type(x).__name__}")
@@ -624,7 +624,10 @@ def gated_feed_forward(x, w13, w2, *, activation="silu", clamp_limit=None, resid
     as the routed experts' W13), w2 [out, intermediate], residual [M, out];
     all fp16 or all bf16.  ``clamp_limit`` is L (none: no clamp).
     With the routed experts' output as ``residual`` the result is the whole
-    MoE layer's.  Differentiable in x, w13, w2 and residual;
+    MoE layer's.  Differentiable in x, w13, w2 and residual (the routed experts
+    have no backward pass: what x contributes through them is not in its
+    gradient).  The product between the two kernels is rounded to 16 bits; in
+    fp16 without a clamp it is infinite past 65,504.
     ``checkpoint="int8"`` keeps x, g and u in 8 bits for the backward pass and
     forms the product again there; y does not change."""
     shape = _check_ffn(x, w13, w2, activation, clamp_limit, residual, checkpoint)

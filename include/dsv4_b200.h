@@ -430,7 +430,8 @@ DSV4_API int dsv4_b200_dense_gemm(const void* a, int64_t lda, int a_mn, const vo
 /* h[m][intermediate] = act(min(g, L)) * clamp(u, -L, L), g and u the products
  * of x with rows [0, intermediate) and [intermediate, 2 intermediate) of w13.
  * z_codes [m][2 ceil32(intermediate)] and z_scales receive g and then u before
- * the clamp (in 16 bits on the same side of the limit as the sums).
+ * the clamp (in 16 bits on the same side of the limit as the sums).  h is
+ * rounded to 16 bits (fp16 without a clamp: infinite past 65,504).
  * w_mn = 1 needs intermediate % 8 == 0. */
 DSV4_API int dsv4_b200_gated_gemm(const void* x, int64_t ldx, int x_mn, const void* w13, int64_t ldw,
                                   int w_mn, int64_t m, int64_t intermediate, int64_t k, int dtype,
