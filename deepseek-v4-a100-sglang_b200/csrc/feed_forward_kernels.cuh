@@ -478,11 +478,10 @@ __device__ __forceinline__ float keep_not_finite(const float (&v)[32], float lim
 
 // With a clamp limit the code stays on the value's side of it: the backward
 // pass asks |z| <= limit of the kept value, and one kept over the border would
-// lose or gain its whole gradient.  Codes count up with the value, so only
-// those that share the limit's own code can be on the wrong side, and all of
-// these move by one if they are.  For relu a value other than zero keeps its
-// sign the same way.  That is one step instead of half a step next to the
-// border.
+// lose or gain its whole gradient.  Values read back count up with the code, so
+// codes are held below and above the border between two of them.  For relu a
+// value other than zero keeps its sign the same way.  That is one step instead
+// of half a step next to the border.
 template <bool BF16>
 __device__ __forceinline__ float keep_group16(const float (&v)[32], float limit, bool keep_sign,
                                               uint32_t (&codes)[16]) {
@@ -499,16 +498,19 @@ __device__ __forceinline__ float keep_group16(const float (&v)[32], float limit,
     for (int j = 0; j < 16; ++j) codes[j] = kept16_codes<BF16>(v[2 * j], v[2 * j + 1], inv);
     return scale;
   }
-  const uint32_t at = kept16_magnitude<BF16>(limit * inv);
-  const bool up = kept16_value<BF16>(at, 0, scale) <= limit;  // values over the limit go up, or the others down
+  // the last code that is read back within the limit (32767 where all are)
+  int last = kept16_magnitude<BF16>(fminf(limit * inv, K::kSteps + 1.f)) & 0x7fffu;
+  if (last < 32767 && kept16_value<BF16>(last + 1, 0, scale) <= limit) ++last;
+  if (kept16_value<BF16>(last, 0, scale) > limit) --last;
+  if (kept16_value<BF16>(last, 0, scale) > limit) --last;
 #pragma unroll
   for (int j = 0; j < 16; ++j) {
-    uint32_t m[2];
+    int m[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const float x = fabsf(v[2 * j + i]);
-      m[i] = kept16_magnitude<BF16>(x * inv);
-      if (m[i] == at && (x > limit) == up) m[i] += up ? 1u : 0xffffffffu;
+      m[i] = kept16_magnitude<BF16>(x * inv) & 0x7fffu;
+      m[i] = x > limit ? max(m[i], last + 1) : min(m[i], last);
       if (keep_sign && m[i] == 0 && x != 0.f) m[i] = 1;
     }
     codes[j] = kept16_signs(prmt(m[0], m[1], 0x5410u), v[2 * j], v[2 * j + 1]);

@@ -120,6 +120,60 @@ def test_relu_keeps_the_sign_of_tiny_values(e, beside):
     assert_each("grad_w1", g13[:n], want, 2.0 ** -8 * want.abs())
 
 
+def spread(t, dtype, at, x):
+    """Columns `at`, at + 16 and at + 32 of x: numbers as the products with `factors` give them exactly."""
+    for i, p in enumerate(parts(t, dtype)):
+        x[:, at + 16 * i] = p
+
+
+def factors(dtype, at, hidden=64):
+    f = torch.zeros(hidden, device="cuda", dtype=dtype)
+    f[at], f[at + 16], f[at + 32] = 1, 2.0 ** -8, 2.0 ** -16
+    return f
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_the_limit_below_a_larger_value(dtype):
+    """Sums up to three fp32 steps from the limit in a group with a larger
+    value, which is chosen so that the limit lies where one code ends and the
+    next begins, at the ends of their powers of two among them."""
+    import dsv4_b200 as D
+    digits, steps = (9, 16894) if dtype == BF16 else (10, 17406)
+    g = torch.Generator().manual_seed(7)
+    w2 = torch.full((8, 32), 0.125, device="cuda", dtype=dtype)
+    for limit in (1.3, 0.37, 7.0, *(0.5 + 9.5 * torch.rand(40, generator=g)).tolist()):
+        lim = torch.tensor(limit, dtype=torch.float32)
+        near = [lim]
+        for way in (math.inf, -math.inf):
+            t = lim
+            for _ in range(3):
+                t = torch.nextafter(t, torch.tensor(way))
+                near.append(t)
+        # the limit in steps of the largest value: borders of codes, and powers of two cut half a step below
+        at = [2.0 ** e / (1 + 2.0 ** -(digits + 1)) for e in range(3, digits + 1)]
+        at += [2.0 ** e * (1 + (0.5 + i) / 2 ** digits) for e in (3, 6, digits - 1) for i in (-1, 0, 1, 77)]
+        at += [2.0 ** digits + 0.5, 2.0 ** digits - 0.5, 3000.5, 9000.0, 12345.5]
+        big = torch.tensor([steps * float(lim) / a for a in at], dtype=torch.float64).float()
+        big = torch.cat([torch.nextafter(big, torch.zeros_like(big)), big, torch.nextafter(big, big * 2)])
+        t = torch.stack(near).repeat(big.numel()).cuda()
+        big = big.repeat_interleave(len(near)).cuda()
+        x = torch.zeros(t.numel(), 64, device="cuda", dtype=dtype)
+        spread(t, dtype, 0, x), spread(big, dtype, 4, x)
+        x[:, 1] = 0.25
+        one = torch.zeros(64, device="cuda", dtype=dtype)
+        one[1] = 1
+        row = factors(dtype, 0).expand(32, -1).clone()
+        row[9] = factors(dtype, 4)
+        dy = torch.ones(t.numel(), 8, device="cuda", dtype=dtype)
+        inside = t <= lim.cuda()
+        for gate in (True, False):
+            w13 = torch.cat((row, one.expand(32, -1)) if gate else (one.expand(32, -1), row))
+            _, saved = D.gated_feed_forward_save(x, w13, w2, activation=None, clamp_limit=limit)
+            got = D.gated_feed_forward_backward(dy, saved)[0][:, 0].double()
+            want = torch.where(inside, 31 * 0.25, 0.0).double()  # dz = 1/4 (the constant is not its group's limit)
+            assert_each(f"{limit} {gate}", got, want, 3 * bits16(dtype) * want)
+
+
 def read_back(g, u, dtype, limit=None):
     """Gate and up values (exact 16-bit numbers), kept in 16-bit groups and read again by the gate's backward
     pass: without an activation and with dh = 1 it writes them as the gradients of up and gate."""
