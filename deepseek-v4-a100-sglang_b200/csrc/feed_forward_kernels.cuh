@@ -93,9 +93,9 @@ __device__ __forceinline__ void pack_row(const float (&v)[32], uint32_t (&w)[16]
 // ---- activations: value and slope ----
 // Fast fp32: values within 2^-18 of |z| + 1 and, where they are small
 // differences, within 2^-14 of themselves (results are rounded to 2^-8 or 2^-11
-// of themselves); powers of two and reciprocals that underflow are 0.  gelu_tanh is
-// z sigmoid(2a) with a = sqrt(2/pi) (z + 0.044715 z^3), since (1 + tanh a) / 2 =
-// sigmoid(2a).
+// of themselves); powers of two and reciprocals that underflow are 0.  gelu_tanh
+// is z sigmoid(2a) with a = sqrt(2/pi) (z + 0.044715 z^3), since (1 + tanh a) / 2
+// = sigmoid(2a).
 enum Act : int { kActNone = 0, kActRelu = 1, kActSilu = 2, kActGelu = 3, kActGeluTanh = 4 };
 
 __device__ __forceinline__ float exp2_approx(float x) {
@@ -398,7 +398,7 @@ struct Kept16 {
   static constexpr float kFromFine = BF16 ? 0x1p104f : 0x1p121f;
 };
 
-// A value of code 16 bits `hi` of w; scale > 0.
+// The value of the code in the lower or upper (`hi`) half of w; scale > 0.
 template <bool BF16>
 __device__ __forceinline__ float kept16_value(uint32_t w, int hi, float scale) {
   using K = Kept16<BF16>;
@@ -449,7 +449,7 @@ __device__ __forceinline__ float max_abs_nan(float a, float b, float c) {
 // A group that holds an infinity or a NaN: fp16 multiples of a power of two,
 // which lose only that value, marked by a negative scale.
 __device__ __forceinline__ float keep_not_finite(const float (&v)[32], float limit, bool keep_sign,
-                                              uint32_t (&codes)[16]) {
+                                                 uint32_t (&codes)[16]) {
   uint32_t top = 0;  // of the finite values
 #pragma unroll
   for (int j = 0; j < 32; ++j) {

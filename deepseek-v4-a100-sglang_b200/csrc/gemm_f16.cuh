@@ -46,9 +46,9 @@ enum F16Epi : int { kEpiLinear = 0, kEpiGated = 1, kEpiGatedBwd = 2 };
 // Epilogue warps and their 2-KB shared slices.  The forward epilogues fit 96
 // registers and one slice: 16 warps (2048 x 2048 -> 7168 with bias, gelu,
 // residual and z kept: 60 us, 63 with 12, 67 with 8; gated 4096 x 1024 -> 2 x
-// 2048 with a limit and z kept: 37, 38 and 39).  The gate's backward pass turns two matrices over
-// in place and is best with few warps and all of their registers (4096 x 1024
-// -> 2048: 43 us, 46 with 12, 50 with 16).
+// 2048 with a limit and z kept: 37, 38 and 39).  The gate's backward pass turns
+// two matrices over in place and is best with few warps and all of their
+// registers (4096 x 1024 -> 2048: 43 us, 46 with 12, 50 with 16).
 template <int EPI>
 struct F16Roles {
   static constexpr int kEpiWarps = EPI == kEpiGatedBwd ? 8 : 16;

@@ -247,8 +247,9 @@ def _empty_codes(rows: int, cols: int, like: torch.Tensor):
 
 def checkpoint_int8(x: torch.Tensor) -> Int8Checkpoint:
     """Keep the rows of ``x`` [M, K] (fp32, fp16 or bf16) in 8 bits: 1.125
-    bytes per value.  Codes have no gradient: for autograd a graph ends here.  ``restore_int8(checkpoint_int8(x))`` differs from x by at
-    most half a step, ``amax / 254`` of its group, and the rounding to x's type."""
+    bytes per value.  ``restore_int8(checkpoint_int8(x))`` differs from x by at
+    most half a step, ``amax / 254`` of its group, and the rounding to x's type.
+    Codes have no gradient: for autograd a graph ends here."""
     if not isinstance(x, torch.Tensor):
         raise TypeError(f"x must be a tensor, got {type(x).__name__}")
     _refuse_tangents(x)
